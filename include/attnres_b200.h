@@ -487,6 +487,41 @@ int attnres_base_backward(int num_sources, int64_t num_tokens, int value_dim, in
                           float* grad_query, float* grad_logit_bias, void* workspace,
                           size_t workspace_bytes, void* stream);
 
+/*
+ * Split of the fused q/k/v projection into heads, with the RMS norm of each
+ * query and key head (the reference's qk_norm, model.py:28-31) and the rotation
+ * by position (RotaryEmbedding, model.py) in the same pass:
+ *   y = R(p) (w * x rsqrt(mean(x^2) + eps)),  v copied.
+ * qkv dtype [num_tokens, (q_heads + 2 kv_heads) * head_dim], rows qkv_row_stride
+ * elements apart: query heads, key heads, value heads. num_tokens is a multiple
+ * of seq_len; row n is token n % seq_len of sequence n / seq_len. cos / sin float
+ * [table_rows, rotary_dim / 2] dense; positions int32 (int64 with
+ * positions_are_64) [num_tokens], NULL for n % seq_len. A position outside
+ * [0, table_rows) makes the token's q and k rows NaN. interleaved: pairs
+ * (2i, 2i+1), else (i, i + rotary_dim/2). normalize 0 leaves the norm out.
+ * q_weight / k_weight dtype [head_dim] or NULL. q [num_tokens, q_heads, head_dim],
+ * k, v [num_tokens, kv_heads, head_dim], dense. head_dim up to 512.
+ *
+ * Backward: grad_q/k/v dtype with element strides grad_strides[9] = {sequence,
+ * token, head} of each, last dim dense; grad_qkv dense; weight gradients dtype
+ * [head_dim], NULL where not wanted, summed over tokens and heads in fp32 in a
+ * fixed order, and only they need the workspace.
+ */
+int attnres_qk_norm_rope_forward(int64_t num_tokens, int64_t seq_len, int q_heads, int kv_heads, int head_dim,
+                                 int rotary_dim, int dtype, const void* qkv, int64_t qkv_row_stride, const float* cos,
+                                 const float* sin, int64_t table_rows, const void* positions, int positions_are_64,
+                                 const void* q_weight, const void* k_weight, int normalize, float eps,
+                                 int interleaved, void* q, void* k, void* v, void* stream);
+size_t attnres_qk_norm_rope_backward_workspace_bytes(int head_dim);
+int attnres_qk_norm_rope_backward(int64_t num_tokens, int64_t seq_len, int q_heads, int kv_heads, int head_dim,
+                                  int rotary_dim, int dtype, const void* qkv, int64_t qkv_row_stride,
+                                  const float* cos, const float* sin, int64_t table_rows, const void* positions,
+                                  int positions_are_64, const void* q_weight, const void* k_weight, int normalize,
+                                  float eps, int interleaved, const void* grad_q, const void* grad_k,
+                                  const void* grad_v, const int64_t* grad_strides, void* grad_qkv,
+                                  void* grad_q_weight, void* grad_k_weight, void* workspace, size_t workspace_bytes,
+                                  void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -7,6 +7,7 @@ attnres::lrid_read / attnres::base_read operators, and exposes the reference's
 public read functions.
 """
 from . import _native
+from .layer import qk_norm_rope
 from .ops import (
     attention_residual_block_summary,
     attention_residual_read,
@@ -42,5 +43,6 @@ __all__ = [
     "lrid_read",
     "lrid_read_list",
     "lrid_read_list_backward",
+    "qk_norm_rope",
     "source_logit_bias",
 ]

@@ -54,6 +54,9 @@ EXPORTED_SYMBOLS = (
     "attnres_phase1_forward",
     "attnres_phase1_backward",
     "attnres_noalloc_scratch_bytes",
+    "attnres_qk_norm_rope_forward",
+    "attnres_qk_norm_rope_backward_workspace_bytes",
+    "attnres_qk_norm_rope_backward",
 )
 
 _lib = None
@@ -192,6 +195,20 @@ def load(path=None):
     L.attnres_base_backward.restype = I
     L.attnres_base_backward.argtypes = [
         I, I64, I, I, PP, PI64, P, I, F, P, I, F, P, P, P, PP, P, P, P, SZ, P,
+    ]
+    rope = [
+        I64, I64, I, I, I, I, I,     # tokens, seq_len, q heads, kv heads, head_dim, rotary_dim, dtype
+        P, I64, P, P, I64, P, I,     # qkv, row stride, cos, sin, table rows, positions, 64-bit positions
+        P, P, I, F, I,               # q weight, k weight, normalize, eps, interleaved
+    ]
+    L.attnres_qk_norm_rope_forward.restype = I
+    L.attnres_qk_norm_rope_forward.argtypes = rope + [P, P, P, P]  # q, k, v, stream
+    L.attnres_qk_norm_rope_backward_workspace_bytes.restype = SZ
+    L.attnres_qk_norm_rope_backward_workspace_bytes.argtypes = [I]
+    L.attnres_qk_norm_rope_backward.restype = I
+    L.attnres_qk_norm_rope_backward.argtypes = rope + [
+        P, P, P, PI64, P, P, P,      # grad q, k, v, strides, grad qkv, grad q weight, grad k weight
+        P, SZ, P,                    # workspace, bytes, stream
     ]
     if path == LIB_PATH:
         _lib = L
