@@ -172,6 +172,214 @@ __global__ void __launch_bounds__(kRopeWarps * 32) qkrope_bwd_any_kernel(const _
   }
 }
 
+// ---------------------------------------------------------------------------
+// rows of 16-byte packs: a group of G lanes holds a head row, one pack a lane
+// ---------------------------------------------------------------------------
+// Unit of work of a warp: kRopeIter rounds of 32 / G consecutive heads of one
+// token, so that a round is one contiguous stretch of the projection's row, the
+// loads of all rounds are in flight at once and the token's cosines and sines
+// are read once per unit. Element pairs: interleaved pairs lie in one lane's
+// pack; of half-split pairs lane l < h (h = rotary_dim / 2 / VEC) holds the first
+// elements and lane l + h the second, exchanged by a shuffle.
+constexpr int kRopeIter = 4;
+constexpr int kRopeVecThreads = 256;
+
+template <typename T, int VEC> struct RopeLane {
+  float c[VEC], s[VEC];  // cosine, and sine with the sign this element's partner takes
+  bool turns;
+};
+
+// y_j = x_j c_j + partner_j s_j with the sines signed: a' = a c - b s, b' = b c + a s.
+// sign = -1 turns backward (the transposed rotation).
+template <typename T, int VEC>
+__device__ __forceinline__ RopeLane<T, VEC> rope_lane(const QkRopeArgs& a, long long p, int l, float sign) {
+  RopeLane<T, VEC> r;
+  const int j0 = l * VEC, half = a.rot / 2;
+  r.turns = j0 < a.rot;
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) {
+    r.c[e] = 1.f;
+    r.s[e] = 0.f;
+  }
+  if (!r.turns) return r;
+  if (p < 0) {
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) r.c[e] = r.s[e] = quiet_nan();
+    return r;
+  }
+  if (a.interleaved) {
+    const Pack<float, VEC / 2> c = load_pack<float, VEC / 2>(a.cos + p * half + j0 / 2);
+    const Pack<float, VEC / 2> s = load_pack<float, VEC / 2>(a.sin + p * half + j0 / 2);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      r.c[e] = c.e[e / 2];
+      r.s[e] = ((e & 1) ? sign : -sign) * s.e[e / 2];
+    }
+  } else {
+    const bool second = j0 >= half;
+    const long long at = p * half + (second ? j0 - half : j0);
+#pragma unroll
+    for (int i = 0; i < VEC; i += 4) {
+      const Pack<float, 4> c = load_pack<float, 4>(a.cos + at + i), s = load_pack<float, 4>(a.sin + at + i);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        r.c[i + e] = c.e[e];
+        r.s[i + e] = (second ? sign : -sign) * s.e[e];
+      }
+    }
+  }
+  return r;
+}
+
+// Every lane of the warp takes part (the shuffle); lanes that do not turn keep x.
+template <typename T, int VEC>
+__device__ __forceinline__ void rope_turn(const QkRopeArgs& a, const RopeLane<T, VEC>& r, int l, float (&x)[VEC]) {
+  float partner[VEC];
+  if (a.interleaved) {
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) partner[e] = x[e ^ 1];
+  } else {
+    const int h = a.rot / 2 / VEC, lane = threadIdx.x & 31;
+    const int from = !r.turns ? lane : (l < h ? lane + h : lane - h);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) partner[e] = __shfl_sync(0xffffffffu, x[e], from);
+  }
+  if (!r.turns) return;
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) x[e] = fmaf(x[e], r.c[e], partner[e] * r.s[e]);
+}
+
+template <typename T, int G, bool WEIGHTED>
+__global__ void __launch_bounds__(kRopeVecThreads) qkrope_fwd_kernel(const __grid_constant__ QkRopeArgs a) {
+  constexpr int VEC = 16 / sizeof(T);
+  const int lane = threadIdx.x & 31, l = lane % G, group = lane / G;
+  const int H = a.Hq + 2 * a.Hkv, per_unit = kRopeIter * (32 / G), units = (H + per_unit - 1) / per_unit;
+  const long long unit = static_cast<long long>(blockIdx.x) * (kRopeVecThreads / 32) + (threadIdx.x >> 5);
+  if (unit >= a.N * units) return;
+  const long long n = unit / units;
+  const int r0 = static_cast<int>(unit % units) * per_unit + group;
+  const bool mine = l * VEC < a.D;  // lanes beyond the head carry zeros
+  const T* x0 = static_cast<const T*>(a.qkv) + n * a.qkv_stride + l * VEC;
+  Pack<T, VEC> x[kRopeIter];
+#pragma unroll
+  for (int i = 0; i < kRopeIter; ++i) {
+    const int r = r0 + i * (32 / G);
+    if (mine && r < H) x[i] = load_stream<T, VEC>(x0 + static_cast<long long>(r) * a.D);
+    else x[i] = Pack<T, VEC>{};
+  }
+  const RopeLane<T, VEC> lanes = rope_lane<T, VEC>(a, rope_position(a, n), l, 1.f);
+  Pack<T, VEC> w[2] = {};
+  if (WEIGHTED && mine)
+    for (int i = 0; i < 2; ++i)
+      if (a.w[i]) w[i] = load_pack<T, VEC>(static_cast<const T*>(a.w[i]) + l * VEC);
+#pragma unroll
+  for (int i = 0; i < kRopeIter; ++i) {
+    const int r = r0 + i * (32 / G);
+    const HeadRef hr = head_ref(a, r);
+    float v[VEC], ss = 0.f;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      v[e] = Elem<T>::to_f(x[i].e[e]);
+      ss = fmaf(v[e], v[e], ss);
+    }
+    ss = group_sum(ss, G);
+    const float inv = a.normalize ? rsqrtf(ss / a.D + a.eps) : 1.f;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      v[e] *= inv;
+      if (WEIGHTED && hr.part < 2 && a.w[hr.part]) v[e] *= Elem<T>::to_f(hr.part ? w[1].e[e] : w[0].e[e]);
+    }
+    rope_turn<T, VEC>(a, lanes, l, v);
+    if (!mine || r >= H) continue;
+    T* y = out_row<T>(a, n, hr) + l * VEC;
+    if (hr.part == 2) *reinterpret_cast<Pack<T, VEC>*>(y) = x[i];
+    else store_pack<T, VEC>(y, v);
+  }
+}
+
+// WEIGHTED also carries the weight gradients: a lane keeps its columns' sums over
+// the units its warp walks through, the block adds its lanes in a fixed order.
+template <typename T, int G, bool WEIGHTED>
+__global__ void __launch_bounds__(kRopeVecThreads) qkrope_bwd_kernel(const __grid_constant__ QkRopeArgs a) {
+  constexpr int VEC = 16 / sizeof(T);
+  const int lane = threadIdx.x & 31, l = lane % G, group = lane / G;
+  const int H = a.Hq + 2 * a.Hkv, per_unit = kRopeIter * (32 / G), units = (H + per_unit - 1) / per_unit;
+  const bool mine = l * VEC < a.D;
+  Pack<T, VEC> w[2] = {};
+  float acc[2][VEC] = {};
+  if (WEIGHTED && mine)
+    for (int i = 0; i < 2; ++i)
+      if (a.w[i]) w[i] = load_pack<T, VEC>(static_cast<const T*>(a.w[i]) + l * VEC);
+  const long long step = static_cast<long long>(gridDim.x) * (kRopeVecThreads / 32);
+  for (long long unit = static_cast<long long>(blockIdx.x) * (kRopeVecThreads / 32) + (threadIdx.x >> 5);
+       unit < a.N * units; unit += step) {
+    const long long n = unit / units;
+    const int r0 = static_cast<int>(unit % units) * per_unit + group;
+    const T* x0 = static_cast<const T*>(a.qkv) + n * a.qkv_stride + l * VEC;
+    Pack<T, VEC> x[kRopeIter], g[kRopeIter];
+#pragma unroll
+    for (int i = 0; i < kRopeIter; ++i) {
+      const int r = r0 + i * (32 / G);
+      x[i] = g[i] = Pack<T, VEC>{};
+      if (mine && r < H) {
+        g[i] = load_stream<T, VEC>(grad_row<T>(a, n, head_ref(a, r)) + l * VEC);
+        if (r < a.Hq + a.Hkv) x[i] = load_stream<T, VEC>(x0 + static_cast<long long>(r) * a.D);
+      }
+    }
+    const RopeLane<T, VEC> lanes = rope_lane<T, VEC>(a, rope_position(a, n), l, -1.f);
+#pragma unroll
+    for (int i = 0; i < kRopeIter; ++i) {
+      const int r = r0 + i * (32 / G);
+      const HeadRef hr = head_ref(a, r);
+      float e[VEC], xh[VEC], ss = 0.f;
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        e[j] = Elem<T>::to_f(g[i].e[j]);
+        xh[j] = Elem<T>::to_f(x[i].e[j]);
+        ss = fmaf(xh[j], xh[j], ss);
+      }
+      ss = group_sum(ss, G);
+      const float inv = a.normalize ? rsqrtf(ss / a.D + a.eps) : 1.f;
+      rope_turn<T, VEC>(a, lanes, l, e);
+      float dot = 0.f;
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        xh[j] *= inv;
+        if (WEIGHTED) {
+          if (r < a.Hq) acc[0][j] = fmaf(e[j], xh[j], acc[0][j]);
+          else if (r < a.Hq + a.Hkv) acc[1][j] = fmaf(e[j], xh[j], acc[1][j]);
+          if (hr.part < 2 && a.w[hr.part]) e[j] *= Elem<T>::to_f(hr.part ? w[1].e[j] : w[0].e[j]);
+        }
+        dot = fmaf(e[j], xh[j], dot);
+      }
+      dot = a.normalize ? group_sum(dot, G) / a.D : 0.f;
+      if (!mine || r >= H) continue;
+      T* dx = static_cast<T*>(a.dqkv) + (n * H + r) * a.D + l * VEC;
+      if (hr.part == 2) {
+        *reinterpret_cast<Pack<T, VEC>*>(dx) = g[i];
+      } else {
+        float o[VEC];
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) o[j] = inv * (e[j] - xh[j] * dot);
+        store_pack<T, VEC>(dx, o);
+      }
+    }
+  }
+  if (!WEIGHTED || a.partials == nullptr) return;
+  extern __shared__ float rope_smem[];  // [kRopeVecThreads][2][VEC]
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) rope_smem[(threadIdx.x * 2 + i) * VEC + j] = acc[i][j];
+  __syncthreads();
+  for (int col = threadIdx.x; col < 2 * a.D; col += kRopeVecThreads) {
+    const int i = col >= a.D, j = col - i * a.D;
+    float s = 0.f;
+    for (int t = j / VEC; t < kRopeVecThreads; t += G) s += rope_smem[(t * 2 + i) * VEC + j % VEC];
+    a.partials[static_cast<long long>(blockIdx.x) * 2 * a.D + col] = s;
+  }
+}
+
 // dw[j] = sum over the blocks' partials in a fixed order: one warp per column,
 // lane l adds blocks l, l + 32, ..., then a butterfly.
 template <typename T>
@@ -193,25 +401,64 @@ namespace {
 
 constexpr int kRopePartialBlocksPerSm = 4;
 
+// Lanes of a head row when it can be moved in 16-byte packs of which each turns
+// whole or not at all, else 0: rows, tables and weights 16-byte aligned, at most
+// 32 packs a head.
 template <typename T>
-cudaError_t forward_t(const QkRopeArgs& a, cudaStream_t st) {
-  const long long rows = a.N * (a.Hq + 2 * a.Hkv);
-  const long long blocks = (rows + kRopeWarps - 1) / kRopeWarps;
-  qkrope_fwd_any_kernel<T><<<static_cast<unsigned>(blocks), kRopeWarps * 32, kRopeWarps * a.D * sizeof(float), st>>>(a);
+int pack_lanes(const QkRopeArgs& a, bool backward) {
+  constexpr int VEC = 16 / sizeof(T);
+  const auto bad = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) != 0; };
+  if (a.D % VEC || a.D > 32 * VEC || a.qkv_stride % VEC || a.rot % (a.interleaved ? VEC : 2 * VEC)) return 0;
+  if (bad(a.qkv) || (a.rot && (bad(a.cos) || bad(a.sin))) || bad(a.w[0]) || bad(a.w[1])) return 0;
+  for (int i = 0; i < 3; ++i) {
+    if (backward) {
+      if (bad(a.g[i])) return 0;
+      for (int j = 0; j < 3; ++j)
+        if (a.gs[i][j] % VEC) return 0;
+    } else if (bad(a.out[i])) {
+      return 0;
+    }
+  }
+  if (backward && bad(a.dqkv)) return 0;
+  int G = 4;
+  while (G * VEC < a.D) G *= 2;
+  return G;
+}
+
+template <typename T, int G>
+cudaError_t vector_t(bool backward, const QkRopeArgs& a, unsigned blocks, cudaStream_t st) {
+  const bool weighted = a.w[0] || a.w[1];
+  const size_t smem = backward && a.partials ? kRopeVecThreads * 2 * (16 / sizeof(T)) * sizeof(float) : 0;
+  auto fn = backward ? (weighted ? qkrope_bwd_kernel<T, G, true> : qkrope_bwd_kernel<T, G, false>)
+                     : (weighted ? qkrope_fwd_kernel<T, G, true> : qkrope_fwd_kernel<T, G, false>);
+  fn<<<blocks, kRopeVecThreads, smem, st>>>(a);
   return cudaGetLastError();
 }
 
 template <typename T>
-cudaError_t backward_t(const QkRopeArgs& a, cudaStream_t st) {
+cudaError_t run_t(bool backward, const QkRopeArgs& a, cudaStream_t st) {
   int nsm = 0;
   cudaError_t e = cached_sm_count(&nsm);
   if (e != cudaSuccess) return e;
-  const long long rows = a.N * (a.Hq + 2 * a.Hkv);
-  long long blocks = (rows + kRopeWarps - 1) / kRopeWarps;
+  const int H = a.Hq + 2 * a.Hkv, G = pack_lanes<T>(a, backward);
+  const int warps = G ? kRopeVecThreads / 32 : kRopeWarps;
+  const long long units = G ? a.N * ((H + kRopeIter * (32 / G) - 1) / (kRopeIter * (32 / G))) : a.N * H;
+  long long blocks = (units + warps - 1) / warps;
   if (a.partials) blocks = std::min<long long>(blocks, static_cast<long long>(nsm) * kRopePartialBlocksPerSm);
-  const size_t smem = kRopeWarps * 2 * a.D * sizeof(float) * (a.partials ? 2 : 1);
-  qkrope_bwd_any_kernel<T><<<static_cast<unsigned>(blocks), kRopeWarps * 32, smem, st>>>(a);
-  if ((e = cudaGetLastError()) != cudaSuccess || !a.partials) return e;
+  const unsigned grid = static_cast<unsigned>(blocks);
+  switch (G) {
+    case 4: e = vector_t<T, 4>(backward, a, grid, st); break;
+    case 8: e = vector_t<T, 8>(backward, a, grid, st); break;
+    case 16: e = vector_t<T, 16>(backward, a, grid, st); break;
+    case 32: e = vector_t<T, 32>(backward, a, grid, st); break;
+    default: {
+      const size_t row = kRopeWarps * a.D * sizeof(float);
+      if (backward) qkrope_bwd_any_kernel<T><<<grid, kRopeWarps * 32, row * (a.partials ? 4 : 2), st>>>(a);
+      else qkrope_fwd_any_kernel<T><<<grid, kRopeWarps * 32, row, st>>>(a);
+      e = cudaGetLastError();
+    }
+  }
+  if (e != cudaSuccess || !a.partials) return e;
   rope_weight_sum_kernel<T><<<(2 * a.D + 3) / 4, 128, 0, st>>>(a.partials, static_cast<int>(blocks), a.D,
                                                              static_cast<T*>(a.dw[0]), static_cast<T*>(a.dw[1]));
   return cudaGetLastError();
@@ -227,9 +474,9 @@ size_t qkrope_workspace_bytes(int D) {
 
 cudaError_t qkrope_launch(bool backward, int dtype, const QkRopeArgs& a, cudaStream_t st) {
   switch (dtype) {
-    case ATTNRES_DTYPE_F32: return backward ? backward_t<float>(a, st) : forward_t<float>(a, st);
-    case ATTNRES_DTYPE_F16: return backward ? backward_t<__half>(a, st) : forward_t<__half>(a, st);
-    default: return backward ? backward_t<__nv_bfloat16>(a, st) : forward_t<__nv_bfloat16>(a, st);
+    case ATTNRES_DTYPE_F32: return run_t<float>(backward, a, st);
+    case ATTNRES_DTYPE_F16: return run_t<__half>(backward, a, st);
+    default: return run_t<__nv_bfloat16>(backward, a, st);
   }
 }
 
