@@ -78,6 +78,7 @@ attnres::QkRopeArgs qk_rope_args(int64_t num_tokens, int64_t seq_len, int q_head
   a.normalize = normalize;
   a.interleaved = interleaved;
   a.eps = eps;
+  a.inv_D = head_dim > 0 ? 1.f / head_dim : 0.f;
   return a;
 }
 

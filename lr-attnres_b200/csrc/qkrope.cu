@@ -24,9 +24,9 @@ namespace attnres {
 
 // The row of the tables for token n, or -1 when the caller's position lies
 // outside them (its q and k rows become NaN rather than reading past the end).
-__device__ __forceinline__ long long rope_position(const QkRopeArgs& a, long long n) {
+__device__ __forceinline__ long long rope_position(const QkRopeArgs& a, long long n, long long t) {
   long long p;
-  if (a.positions == nullptr) p = n % a.T;
+  if (a.positions == nullptr) p = t;
   else if (a.positions64) p = static_cast<const long long*>(a.positions)[n];
   else p = static_cast<const int*>(a.positions)[n];
   return (p >= 0 && p < a.table_rows) ? p : -1;
@@ -44,9 +44,8 @@ __device__ __forceinline__ HeadRef head_ref(const QkRopeArgs& a, int r) {
   return {2, r - a.Hq - a.Hkv};
 }
 template <typename T>
-__device__ __forceinline__ const T* grad_row(const QkRopeArgs& a, long long n, HeadRef h) {
-  return static_cast<const T*>(a.g[h.part]) + (n / a.T) * a.gs[h.part][0] + (n % a.T) * a.gs[h.part][1] +
-         h.h * a.gs[h.part][2];
+__device__ __forceinline__ const T* grad_row(const QkRopeArgs& a, long long b, long long t, HeadRef h) {
+  return static_cast<const T*>(a.g[h.part]) + b * a.gs[h.part][0] + t * a.gs[h.part][1] + h.h * a.gs[h.part][2];
 }
 template <typename T>
 __device__ __forceinline__ T* out_row(const QkRopeArgs& a, long long n, HeadRef h) {
@@ -86,7 +85,7 @@ __global__ void __launch_bounds__(kRopeWarps * 32) qkrope_fwd_any_kernel(const _
   ss = warp_sum(ss);
   const float inv = a.normalize ? rsqrtf(ss / a.D + a.eps) : 1.f;
   __syncwarp();
-  const long long p = rope_position(a, n);
+  const long long p = rope_position(a, n, n % a.T);
   const int half = a.rot / 2;
   for (int i = lane; i < half; i += 32) {
     const int i0 = a.interleaved ? 2 * i : i, i1 = a.interleaved ? 2 * i + 1 : i + half;
@@ -124,7 +123,7 @@ __global__ void __launch_bounds__(kRopeWarps * 32) qkrope_bwd_any_kernel(const _
     const long long n = row / H;
     const int r = static_cast<int>(row % H);
     const HeadRef hr = head_ref(a, r);
-    const T* g = grad_row<T>(a, n, hr);
+    const T* g = grad_row<T>(a, n / a.T, n % a.T, hr);
     T* dx = static_cast<T*>(a.dqkv) + (n * H + r) * D;
     if (hr.part == 2) {
       for (int j = lane; j < D; j += 32) dx[j] = g[j];
@@ -141,7 +140,7 @@ __global__ void __launch_bounds__(kRopeWarps * 32) qkrope_bwd_any_kernel(const _
     }
     ss = warp_sum(ss);
     const float inv = a.normalize ? rsqrtf(ss / D + a.eps) : 1.f;
-    const long long p = rope_position(a, n);
+    const long long p = rope_position(a, n, n % a.T);
     for (int i = lane; i < half; i += 32) {
       const int i0 = a.interleaved ? 2 * i : i, i1 = a.interleaved ? 2 * i + 1 : i + half;
       const float u = Elem<T>::to_f(g[i0]), v = Elem<T>::to_f(g[i1]);
@@ -180,20 +179,25 @@ __global__ void __launch_bounds__(kRopeWarps * 32) qkrope_bwd_any_kernel(const _
 // loads of all rounds are in flight at once and the token's cosines and sines
 // are read once per unit. Element pairs: interleaved pairs lie in one lane's
 // pack; of half-split pairs lane l < h (h = rotary_dim / 2 / VEC) holds the first
-// elements and lane l + h the second, exchanged by a shuffle.
+// elements and lane l + h the second, exchanged by a shuffle. Units are counted in
+// 32 bits (64-bit divisions took half the backward's time); the host sends
+// launches with more of them to the kernels above.
 constexpr int kRopeIter = 4;
 constexpr int kRopeVecThreads = 256;
 
-template <typename T, int VEC> struct RopeLane {
+// Left as single loads, divisions and conversions this was bound by issue slots,
+// not by HBM (168 instructions a round, 3.0 TB/s); hence the compile-time pairing,
+// packed fp32 arithmetic and one base pointer per part of the row.
+template <int VEC> struct RopeLane {
   float c[VEC], s[VEC];  // cosine, and sine with the sign this element's partner takes
   bool turns;
 };
 
 // y_j = x_j c_j + partner_j s_j with the sines signed: a' = a c - b s, b' = b c + a s.
 // sign = -1 turns backward (the transposed rotation).
-template <typename T, int VEC>
-__device__ __forceinline__ RopeLane<T, VEC> rope_lane(const QkRopeArgs& a, long long p, int l, float sign) {
-  RopeLane<T, VEC> r;
+template <int VEC, bool INTERLEAVED>
+__device__ __forceinline__ RopeLane<VEC> rope_lane(const QkRopeArgs& a, long long p, int l, float sign) {
+  RopeLane<VEC> r;
   const int j0 = l * VEC, half = a.rot / 2;
   r.turns = j0 < a.rot;
 #pragma unroll
@@ -207,7 +211,7 @@ __device__ __forceinline__ RopeLane<T, VEC> rope_lane(const QkRopeArgs& a, long 
     for (int e = 0; e < VEC; ++e) r.c[e] = r.s[e] = quiet_nan();
     return r;
   }
-  if (a.interleaved) {
+  if constexpr (INTERLEAVED) {
     const Pack<float, VEC / 2> c = load_pack<float, VEC / 2>(a.cos + p * half + j0 / 2);
     const Pack<float, VEC / 2> s = load_pack<float, VEC / 2>(a.sin + p * half + j0 / 2);
 #pragma unroll
@@ -231,152 +235,206 @@ __device__ __forceinline__ RopeLane<T, VEC> rope_lane(const QkRopeArgs& a, long 
   return r;
 }
 
-// Every lane of the warp takes part (the shuffle); lanes that do not turn keep x.
-template <typename T, int VEC>
-__device__ __forceinline__ void rope_turn(const QkRopeArgs& a, const RopeLane<T, VEC>& r, int l, float (&x)[VEC]) {
+// Every lane of the warp takes part (the shuffle); lanes that do not turn have
+// c = 1, s = 0 and themselves as partner.
+template <int VEC, bool INTERLEAVED>
+__device__ __forceinline__ void rope_turn(const RopeLane<VEC>& r, int from, float (&x)[VEC]) {
   float partner[VEC];
-  if (a.interleaved) {
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) partner[e] = x[e ^ 1];
-  } else {
-    const int h = a.rot / 2 / VEC, lane = threadIdx.x & 31;
-    const int from = !r.turns ? lane : (l < h ? lane + h : lane - h);
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) partner[e] = __shfl_sync(0xffffffffu, x[e], from);
-  }
-  if (!r.turns) return;
+  for (int e = 0; e < VEC; ++e)
+    partner[e] = INTERLEAVED ? x[e ^ 1] : __shfl_sync(0xffffffffu, x[e], from);
+  if (INTERLEAVED && !r.turns) return;
 #pragma unroll
   for (int e = 0; e < VEC; ++e) x[e] = fmaf(x[e], r.c[e], partner[e] * r.s[e]);
 }
 
-template <typename T, int G, bool WEIGHTED>
-__global__ void __launch_bounds__(kRopeVecThreads) qkrope_fwd_kernel(const __grid_constant__ QkRopeArgs a) {
-  constexpr int VEC = 16 / sizeof(T);
-  const int lane = threadIdx.x & 31, l = lane % G, group = lane / G;
-  const int H = a.Hq + 2 * a.Hkv, per_unit = kRopeIter * (32 / G), units = (H + per_unit - 1) / per_unit;
-  const long long unit = static_cast<long long>(blockIdx.x) * (kRopeVecThreads / 32) + (threadIdx.x >> 5);
-  if (unit >= a.N * units) return;
-  const long long n = unit / units;
-  const int r0 = static_cast<int>(unit % units) * per_unit + group;
+__device__ __forceinline__ int rope_partner_lane(const QkRopeArgs& a, bool turns, int l, int vec) {
+  const int h = a.rot / 2 / vec, lane = threadIdx.x & 31;
+  return !turns ? lane : (l < h ? lane + h : lane - h);
+}
+
+template <typename T, int VEC>
+__device__ __forceinline__ void widen(const Pack<T, VEC>& x, float (&v)[VEC]) {
+#pragma unroll
+  for (int i = 0; i < VEC / 2; ++i) unpack2<T, VEC>(x, i, v[2 * i], v[2 * i + 1]);
+}
+
+template <typename T, int VEC>
+__device__ __forceinline__ Pack<T, VEC> narrow(const float (&v)[VEC]) {
+  Pack<T, VEC> r;
+  if constexpr (std::is_same<T, float>::value) {
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) r.e[e] = v[e];
+  } else if constexpr (std::is_same<T, __half>::value) {
+#pragma unroll
+    for (int i = 0; i < VEC / 2; ++i) reinterpret_cast<__half2*>(r.e)[i] = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < VEC / 2; ++i)
+      reinterpret_cast<__nv_bfloat162*>(r.e)[i] = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+  }
+  return r;
+}
+
+template <int VEC>
+__device__ __forceinline__ float dot(const float (&x)[VEC], const float (&y)[VEC]) {
+  float a0 = 0.f, a1 = 0.f;
+#pragma unroll
+  for (int i = 0; i < VEC / 2; ++i) fma2v(a0, a1, x[2 * i], x[2 * i + 1], y[2 * i], y[2 * i + 1]);
+  return a0 + a1;
+}
+template <int VEC>
+__device__ __forceinline__ void scale(float (&x)[VEC], float w) {
+#pragma unroll
+  for (int i = 0; i < VEC / 2; ++i) mul2(x[2 * i], x[2 * i + 1], w, x[2 * i], x[2 * i + 1]);
+}
+
+template <typename T, int G, bool INTERLEAVED, bool WEIGHTED>
+__global__ void __launch_bounds__(kRopeVecThreads, sizeof(T) == 2 ? 4 : 3)
+    qkrope_fwd_kernel(const __grid_constant__ QkRopeArgs a) {
+  constexpr int VEC = 16 / sizeof(T), ROUND = 32 / G;
+  const int lane = threadIdx.x & 31, l = lane % G;
+  const int H = a.Hq + 2 * a.Hkv, Hqk = a.Hq + a.Hkv;
+  const unsigned units = (H + kRopeIter * ROUND - 1) / (kRopeIter * ROUND);
+  const unsigned unit = blockIdx.x * (kRopeVecThreads / 32) + (threadIdx.x >> 5);
+  if (unit >= static_cast<unsigned>(a.N) * units) return;
+  const unsigned n = unit / units;
+  const int first = static_cast<int>(unit - n * units) * kRopeIter * ROUND, r0 = first + lane / G;
   const bool mine = l * VEC < a.D;  // lanes beyond the head carry zeros
+  const long long p = first < Hqk ? rope_position(a, n, n % static_cast<unsigned>(a.T)) : 0;
   const T* x0 = static_cast<const T*>(a.qkv) + n * a.qkv_stride + l * VEC;
   Pack<T, VEC> x[kRopeIter];
 #pragma unroll
   for (int i = 0; i < kRopeIter; ++i) {
-    const int r = r0 + i * (32 / G);
-    if (mine && r < H) x[i] = load_stream<T, VEC>(x0 + static_cast<long long>(r) * a.D);
+    const int r = r0 + i * ROUND;
+    if (mine && r < H) x[i] = load_stream<T, VEC>(x0 + r * a.D);
     else x[i] = Pack<T, VEC>{};
   }
-  const RopeLane<T, VEC> lanes = rope_lane<T, VEC>(a, rope_position(a, n), l, 1.f);
-  Pack<T, VEC> w[2] = {};
-  if (WEIGHTED && mine)
-    for (int i = 0; i < 2; ++i)
-      if (a.w[i]) w[i] = load_pack<T, VEC>(static_cast<const T*>(a.w[i]) + l * VEC);
+  // where head r = 0 of the row would lie in each of the three outputs
+  T* const yq = static_cast<T*>(a.out[0]) + static_cast<long long>(n) * a.Hq * a.D + l * VEC;
+  T* const yk = static_cast<T*>(a.out[1]) + (static_cast<long long>(n) * a.Hkv - a.Hq) * a.D + l * VEC;
+  T* const yv = static_cast<T*>(a.out[2]) + (static_cast<long long>(n) * a.Hkv - Hqk) * a.D + l * VEC;
+  RopeLane<VEC> turn;
+  float wq[VEC], wk[VEC];
+  int from = lane;
+  if (first < Hqk) {
+    turn = rope_lane<VEC, INTERLEAVED>(a, p, l, 1.f);
+    from = rope_partner_lane(a, turn.turns, l, VEC);
+    if (WEIGHTED) {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        wq[e] = a.w[0] && mine ? Elem<T>::to_f(static_cast<const T*>(a.w[0])[l * VEC + e]) : 1.f;
+        wk[e] = a.w[1] && mine ? Elem<T>::to_f(static_cast<const T*>(a.w[1])[l * VEC + e]) : 1.f;
+      }
+    }
+  }
 #pragma unroll
   for (int i = 0; i < kRopeIter; ++i) {
-    const int r = r0 + i * (32 / G);
-    const HeadRef hr = head_ref(a, r);
-    float v[VEC], ss = 0.f;
+    const int r = r0 + i * ROUND;
+    if (first + i * ROUND < Hqk) {  // some head of the round turns (the same for the whole warp)
+      float v[VEC];
+      widen<T, VEC>(x[i], v);
+      if (a.normalize) scale<VEC>(v, rsqrtf(group_sum(dot<VEC>(v, v), G) * a.inv_D + a.eps));
+      if (WEIGHTED) {
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-      v[e] = Elem<T>::to_f(x[i].e[e]);
-      ss = fmaf(v[e], v[e], ss);
+        for (int e = 0; e < VEC; ++e) v[e] *= r < a.Hq ? wq[e] : wk[e];
+      }
+      rope_turn<VEC, INTERLEAVED>(turn, from, v);
+      if (r < Hqk) x[i] = narrow<T, VEC>(v);
     }
-    ss = group_sum(ss, G);
-    const float inv = a.normalize ? rsqrtf(ss / a.D + a.eps) : 1.f;
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-      v[e] *= inv;
-      if (WEIGHTED && hr.part < 2 && a.w[hr.part]) v[e] *= Elem<T>::to_f(hr.part ? w[1].e[e] : w[0].e[e]);
-    }
-    rope_turn<T, VEC>(a, lanes, l, v);
-    if (!mine || r >= H) continue;
-    T* y = out_row<T>(a, n, hr) + l * VEC;
-    if (hr.part == 2) *reinterpret_cast<Pack<T, VEC>*>(y) = x[i];
-    else store_pack<T, VEC>(y, v);
+    if (mine && r < H) *reinterpret_cast<Pack<T, VEC>*>((r < a.Hq ? yq : (r < Hqk ? yk : yv)) + r * a.D) = x[i];
   }
 }
 
 // WEIGHTED also carries the weight gradients: a lane keeps its columns' sums over
 // the units its warp walks through, the block adds its lanes in a fixed order.
-template <typename T, int G, bool WEIGHTED>
-__global__ void __launch_bounds__(kRopeVecThreads) qkrope_bwd_kernel(const __grid_constant__ QkRopeArgs a) {
-  constexpr int VEC = 16 / sizeof(T);
-  const int lane = threadIdx.x & 31, l = lane % G, group = lane / G;
-  const int H = a.Hq + 2 * a.Hkv, per_unit = kRopeIter * (32 / G), units = (H + per_unit - 1) / per_unit;
+template <typename T, int G, bool INTERLEAVED, bool WEIGHTED>
+__global__ void __launch_bounds__(kRopeVecThreads, WEIGHTED ? 2 : 3)
+    qkrope_bwd_kernel(const __grid_constant__ QkRopeArgs a) {
+  constexpr int VEC = 16 / sizeof(T), ROUND = 32 / G;
+  const int lane = threadIdx.x & 31, l = lane % G;
+  const int H = a.Hq + 2 * a.Hkv, Hqk = a.Hq + a.Hkv;
+  const unsigned units = (H + kRopeIter * ROUND - 1) / (kRopeIter * ROUND);
   const bool mine = l * VEC < a.D;
-  Pack<T, VEC> w[2] = {};
-  float acc[2][VEC] = {};
-  if (WEIGHTED && mine)
-    for (int i = 0; i < 2; ++i)
-      if (a.w[i]) w[i] = load_pack<T, VEC>(static_cast<const T*>(a.w[i]) + l * VEC);
-  const long long step = static_cast<long long>(gridDim.x) * (kRopeVecThreads / 32);
-  for (long long unit = static_cast<long long>(blockIdx.x) * (kRopeVecThreads / 32) + (threadIdx.x >> 5);
-       unit < a.N * units; unit += step) {
-    const long long n = unit / units;
-    const int r0 = static_cast<int>(unit % units) * per_unit + group;
+  float wq[VEC], wk[VEC], acc[2][VEC];
+  if (WEIGHTED) {
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      wq[e] = a.w[0] && mine ? Elem<T>::to_f(static_cast<const T*>(a.w[0])[l * VEC + e]) : 1.f;
+      wk[e] = a.w[1] && mine ? Elem<T>::to_f(static_cast<const T*>(a.w[1])[l * VEC + e]) : 1.f;
+      acc[0][e] = acc[1][e] = 0.f;
+    }
+  }
+  const unsigned step = gridDim.x * (kRopeVecThreads / 32), total = static_cast<unsigned>(a.N) * units;
+  for (unsigned unit = blockIdx.x * (kRopeVecThreads / 32) + (threadIdx.x >> 5); unit < total; unit += step) {
+    const unsigned n = unit / units, b = n / static_cast<unsigned>(a.T), t = n - b * static_cast<unsigned>(a.T);
+    const int first = static_cast<int>(unit - n * units) * kRopeIter * ROUND, r0 = first + lane / G;
+    const long long p = first < Hqk ? rope_position(a, n, t) : 0;
     const T* x0 = static_cast<const T*>(a.qkv) + n * a.qkv_stride + l * VEC;
+    const T* g0[3];
+    const int skip[3] = {0, a.Hq, Hqk};
+#pragma unroll
+    for (int i = 0; i < 3; ++i)
+      g0[i] = static_cast<const T*>(a.g[i]) + b * a.gs[i][0] + t * a.gs[i][1] - skip[i] * a.gs[i][2] + l * VEC;
     Pack<T, VEC> x[kRopeIter], g[kRopeIter];
 #pragma unroll
     for (int i = 0; i < kRopeIter; ++i) {
-      const int r = r0 + i * (32 / G);
+      const int r = r0 + i * ROUND, part = r < a.Hq ? 0 : (r < Hqk ? 1 : 2);
       x[i] = g[i] = Pack<T, VEC>{};
       if (mine && r < H) {
-        g[i] = load_stream<T, VEC>(grad_row<T>(a, n, head_ref(a, r)) + l * VEC);
-        if (r < a.Hq + a.Hkv) x[i] = load_stream<T, VEC>(x0 + static_cast<long long>(r) * a.D);
+        g[i] = load_stream<T, VEC>((part == 0 ? g0[0] : (part == 1 ? g0[1] : g0[2])) +
+                                   r * (part == 0 ? a.gs[0][2] : (part == 1 ? a.gs[1][2] : a.gs[2][2])));
+        if (part < 2) x[i] = load_stream<T, VEC>(x0 + r * a.D);
       }
     }
-    const RopeLane<T, VEC> lanes = rope_lane<T, VEC>(a, rope_position(a, n), l, -1.f);
+    RopeLane<VEC> turn;
+    int from = lane;
+    if (first < Hqk) {
+      turn = rope_lane<VEC, INTERLEAVED>(a, p, l, -1.f);
+      from = rope_partner_lane(a, turn.turns, l, VEC);
+    }
+    T* const dx = static_cast<T*>(a.dqkv) + static_cast<long long>(n) * H * a.D + l * VEC;
 #pragma unroll
     for (int i = 0; i < kRopeIter; ++i) {
-      const int r = r0 + i * (32 / G);
-      const HeadRef hr = head_ref(a, r);
-      float e[VEC], xh[VEC], ss = 0.f;
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        e[j] = Elem<T>::to_f(g[i].e[j]);
-        xh[j] = Elem<T>::to_f(x[i].e[j]);
-        ss = fmaf(xh[j], xh[j], ss);
-      }
-      ss = group_sum(ss, G);
-      const float inv = a.normalize ? rsqrtf(ss / a.D + a.eps) : 1.f;
-      rope_turn<T, VEC>(a, lanes, l, e);
-      float dot = 0.f;
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        xh[j] *= inv;
+      const int r = r0 + i * ROUND;
+      if (first + i * ROUND < Hqk) {
+        float e[VEC], v[VEC];
+        widen<T, VEC>(g[i], e);
+        widen<T, VEC>(x[i], v);
+        rope_turn<VEC, INTERLEAVED>(turn, from, e);
+        const float inv = a.normalize ? rsqrtf(group_sum(dot<VEC>(v, v), G) * a.inv_D + a.eps) : 1.f;
+        scale<VEC>(v, inv);
         if (WEIGHTED) {
-          if (r < a.Hq) acc[0][j] = fmaf(e[j], xh[j], acc[0][j]);
-          else if (r < a.Hq + a.Hkv) acc[1][j] = fmaf(e[j], xh[j], acc[1][j]);
-          if (hr.part < 2 && a.w[hr.part]) e[j] *= Elem<T>::to_f(hr.part ? w[1].e[j] : w[0].e[j]);
-        }
-        dot = fmaf(e[j], xh[j], dot);
-      }
-      dot = a.normalize ? group_sum(dot, G) / a.D : 0.f;
-      if (!mine || r >= H) continue;
-      T* dx = static_cast<T*>(a.dqkv) + (n * H + r) * a.D + l * VEC;
-      if (hr.part == 2) {
-        *reinterpret_cast<Pack<T, VEC>*>(dx) = g[i];
-      } else {
-        float o[VEC];
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) o[j] = inv * (e[j] - xh[j] * dot);
-        store_pack<T, VEC>(dx, o);
+          for (int j = 0; j < VEC; ++j) {
+            if (r < a.Hq) acc[0][j] = fmaf(e[j], v[j], acc[0][j]);
+            else if (r < Hqk) acc[1][j] = fmaf(e[j], v[j], acc[1][j]);
+            e[j] *= r < a.Hq ? wq[j] : wk[j];
+          }
+        }
+        const float mean = a.normalize ? group_sum(dot<VEC>(e, v), G) * a.inv_D : 0.f;
+#pragma unroll
+        for (int j = 0; j < VEC / 2; ++j) fma2(e[2 * j], e[2 * j + 1], -mean, v[2 * j], v[2 * j + 1]);
+        scale<VEC>(e, inv);
+        if (r < Hqk) g[i] = narrow<T, VEC>(e);
       }
+      if (mine && r < H) *reinterpret_cast<Pack<T, VEC>*>(dx + r * a.D) = g[i];
     }
   }
-  if (!WEIGHTED || a.partials == nullptr) return;
-  extern __shared__ float rope_smem[];  // [kRopeVecThreads][2][VEC]
+  if constexpr (WEIGHTED) {
+    if (a.partials == nullptr) return;
+    extern __shared__ float rope_smem[];  // [kRopeVecThreads][2][VEC]
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < 2; ++i)
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) rope_smem[(threadIdx.x * 2 + i) * VEC + j] = acc[i][j];
-  __syncthreads();
-  for (int col = threadIdx.x; col < 2 * a.D; col += kRopeVecThreads) {
-    const int i = col >= a.D, j = col - i * a.D;
-    float s = 0.f;
-    for (int t = j / VEC; t < kRopeVecThreads; t += G) s += rope_smem[(t * 2 + i) * VEC + j % VEC];
-    a.partials[static_cast<long long>(blockIdx.x) * 2 * a.D + col] = s;
+      for (int j = 0; j < VEC; ++j) rope_smem[(threadIdx.x * 2 + i) * VEC + j] = acc[i][j];
+    __syncthreads();
+    for (int col = threadIdx.x; col < 2 * a.D; col += kRopeVecThreads) {
+      const int i = col >= a.D, j = col - i * a.D;
+      float s = 0.f;
+      for (int t = j / VEC; t < kRopeVecThreads; t += G) s += rope_smem[(t * 2 + i) * VEC + j % VEC];
+      a.partials[static_cast<long long>(blockIdx.x) * 2 * a.D + col] = s;
+    }
   }
 }
 
@@ -420,18 +478,21 @@ int pack_lanes(const QkRopeArgs& a, bool backward) {
     }
   }
   if (backward && bad(a.dqkv)) return 0;
-  int G = 4;
+  int G = 8;
   while (G * VEC < a.D) G *= 2;
-  return G;
+  return a.N * (a.Hq + 2 * a.Hkv) < (1LL << 30) ? G : 0;  // units in 32 bits
 }
 
 template <typename T, int G>
 cudaError_t vector_t(bool backward, const QkRopeArgs& a, unsigned blocks, cudaStream_t st) {
-  const bool weighted = a.w[0] || a.w[1];
-  const size_t smem = backward && a.partials ? kRopeVecThreads * 2 * (16 / sizeof(T)) * sizeof(float) : 0;
-  auto fn = backward ? (weighted ? qkrope_bwd_kernel<T, G, true> : qkrope_bwd_kernel<T, G, false>)
-                     : (weighted ? qkrope_fwd_kernel<T, G, true> : qkrope_fwd_kernel<T, G, false>);
-  fn<<<blocks, kRopeVecThreads, smem, st>>>(a);
+  using Kernel = void (*)(QkRopeArgs);
+  static const Kernel kernels[2][2][2] = {
+      {{qkrope_fwd_kernel<T, G, false, false>, qkrope_fwd_kernel<T, G, false, true>},
+       {qkrope_fwd_kernel<T, G, true, false>, qkrope_fwd_kernel<T, G, true, true>}},
+      {{qkrope_bwd_kernel<T, G, false, false>, qkrope_bwd_kernel<T, G, false, true>},
+       {qkrope_bwd_kernel<T, G, true, false>, qkrope_bwd_kernel<T, G, true, true>}}};
+  const size_t smem = a.partials ? kRopeVecThreads * 2 * (16 / sizeof(T)) * sizeof(float) : 0;
+  kernels[backward][a.interleaved != 0][a.w[0] || a.w[1]]<<<blocks, kRopeVecThreads, smem, st>>>(a);
   return cudaGetLastError();
 }
 
@@ -447,7 +508,6 @@ cudaError_t run_t(bool backward, const QkRopeArgs& a, cudaStream_t st) {
   if (a.partials) blocks = std::min<long long>(blocks, static_cast<long long>(nsm) * kRopePartialBlocksPerSm);
   const unsigned grid = static_cast<unsigned>(blocks);
   switch (G) {
-    case 4: e = vector_t<T, 4>(backward, a, grid, st); break;
     case 8: e = vector_t<T, 8>(backward, a, grid, st); break;
     case 16: e = vector_t<T, 16>(backward, a, grid, st); break;
     case 32: e = vector_t<T, 32>(backward, a, grid, st); break;

@@ -19,7 +19,7 @@ struct QkRopeArgs {
   int positions64;
   const void* w[2];  // q and k weights [D], or null
   int normalize, interleaved;
-  float eps;
+  float eps, inv_D;
   void* out[3];  // q [N, Hq, D], k, v [N, Hkv, D]
   // backward
   const void* g[3];     // dq, dk, dv
