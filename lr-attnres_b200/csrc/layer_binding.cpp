@@ -1,0 +1,243 @@
+// PyTorch binding of the transformer-layer operators: argument checks, output
+// allocation, autograd and the calls into the C ABI, in C++ because at a decoding
+// step's sizes the same steps in Python and ctypes take several times the kernels'
+// own time (split + norm + rotation of four tokens: 26 us in Python, 3 us on the
+// GPU). Errors are C++ exceptions that pybind11 turns into RuntimeError.
+#include <c10/cuda/CUDAGuard.h>
+#include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/extension.h>
+
+#include "attnres_b200.h"
+
+namespace {
+
+using at::Tensor;
+using OptTensor = std::optional<Tensor>;
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+int dtype_code(const Tensor& t) {
+  switch (t.scalar_type()) {
+    case at::kFloat: return ATTNRES_DTYPE_F32;
+    case at::kHalf: return ATTNRES_DTYPE_F16;
+    case at::kBFloat16: return ATTNRES_DTYPE_BF16;
+    default:
+      TORCH_CHECK(false, "attnres_b200: unsupported dtype ", t.scalar_type(), "; use float32, float16 or bfloat16");
+  }
+}
+
+void check_status(int rc, const char* what) {
+  static const char* const names[] = {"ok", "invalid argument", "unsupported", "CUDA error", "workspace too small"};
+  TORCH_CHECK(rc == ATTNRES_OK, what, " failed (", rc >= 0 && rc <= 4 ? names[rc] : "?", "): ", attnres_last_error());
+}
+
+void check_cuda(const char* what, const Tensor& t) {
+  TORCH_CHECK(t.is_cuda(), "attnres_b200: ", what, " inputs must be CUDA tensors (there is no CPU path)");
+}
+void check_device(const char* what, const Tensor& first, const Tensor& t) {
+  TORCH_CHECK(!t.defined() || t.device() == first.device(), "attnres_b200: ", what,
+              " inputs must be on one device, got ", first.device(), " and ", t.device());
+}
+
+Tensor or_undefined(const OptTensor& t) { return t.has_value() ? *t : Tensor(); }
+const void* ptr(const Tensor& t) { return t.defined() ? t.const_data_ptr() : nullptr; }
+void* mut(const Tensor& t) { return t.defined() ? t.mutable_data_ptr() : nullptr; }
+
+// Makes the tensor's device current and hands out its current stream.
+struct Launch {
+  c10::cuda::CUDAGuard guard;
+  void* stream;
+  explicit Launch(const Tensor& t) : guard(t.device()), stream(c10::cuda::getCurrentCUDAStream().stream()) {}
+};
+
+// The backward kernels have no gradient of their own: better no second derivative
+// than a silent zero.
+void check_first_order(const char* what) {
+  TORCH_CHECK(!at::GradMode::is_enabled(), "attnres_b200: ", what, " cannot be differentiated twice (create_graph)");
+}
+
+// ---------------------------------------------------------------------------
+// qk_norm_rope
+// ---------------------------------------------------------------------------
+struct RopeHow {
+  int64_t q_heads, kv_heads;
+  bool normalize;
+  double eps;
+  bool interleaved;
+};
+
+// The checked arguments of one call, rows made uniform where they were not.
+struct RopeCall {
+  Tensor qkv, cos, sin, positions, wq, wk;
+  int64_t B, T, D, stride;
+  int code, wide;
+  RopeHow how;
+
+  RopeCall(const Tensor& qkv_, const Tensor& cos_, const Tensor& sin_, const Tensor& positions_, const Tensor& wq_,
+           const Tensor& wk_, const RopeHow& h)
+      : qkv(qkv_), positions(positions_), wide(0), how(h) {
+    const char* what = "qk_norm_rope";
+    check_cuda(what, qkv);
+    for (const Tensor* t : {&cos_, &sin_, &positions_, &wq_, &wk_}) check_device(what, qkv, *t);
+    TORCH_CHECK(h.q_heads >= 1 && h.kv_heads >= 1 && h.q_heads <= 4096 && h.kv_heads <= 4096,
+                "attnres_b200: qk_norm_rope needs 1 to 4096 query and key heads, got ", h.q_heads, " and ", h.kv_heads);
+    const int64_t heads = h.q_heads + 2 * h.kv_heads;
+    TORCH_CHECK(qkv.dim() == 3 && qkv.size(2) > 0 && qkv.size(2) % heads == 0, "attnres_b200: qk_norm_rope takes qkv [B, T, (",
+                h.q_heads, " + 2 * ", h.kv_heads, ") * head_dim], got ", qkv.sizes());
+    B = qkv.size(0);
+    T = qkv.size(1);
+    const int64_t width = qkv.size(2);
+    D = width / heads;
+    code = dtype_code(qkv);
+    stride = T > 1 ? qkv.stride(1) : (B > 1 ? qkv.stride(0) : width);
+    if (qkv.stride(2) != 1 || stride < width || (T > 1 && B > 1 && qkv.stride(0) != T * stride)) {
+      qkv = qkv.contiguous();  // rows of one stride that do not overlap
+      stride = width;
+    }
+    TORCH_CHECK(cos_.dim() == 2 && cos_.sizes() == sin_.sizes(),
+                "attnres_b200: qk_norm_rope takes cos and sin [positions, rotary_dim / 2], got ", cos_.sizes(), " and ",
+                sin_.sizes());
+    TORCH_CHECK(cos_.scalar_type() == at::kFloat && sin_.scalar_type() == at::kFloat,
+                "attnres_b200: qk_norm_rope takes float32 cos and sin");
+    cos = cos_.contiguous();
+    sin = sin_.contiguous();
+    TORCH_CHECK(2 * cos.size(1) <= D, "attnres_b200: qk_norm_rope rotary_dim ", 2 * cos.size(1), " exceeds head_dim ", D);
+    if (positions.defined()) {
+      wide = positions.scalar_type() == at::kLong;
+      TORCH_CHECK((wide || positions.scalar_type() == at::kInt) && positions.dim() == 2 && positions.size(0) == B &&
+                      positions.size(1) == T,
+                  "attnres_b200: qk_norm_rope takes positions [B, T] int32 or int64");
+      positions = positions.contiguous();
+    } else {
+      TORCH_CHECK(B == 0 || cos.size(1) == 0 || T <= cos.size(0), "attnres_b200: qk_norm_rope has ", T,
+                  " tokens and tables of ", cos.size(0), " positions");
+    }
+    for (const Tensor* w : {&wq_, &wk_})
+      TORCH_CHECK(!w->defined() || (w->dim() == 1 && w->size(0) == D),
+                  "attnres_b200: qk_norm_rope weights are [head_dim] = [", D, "]");
+    if (wq_.defined()) wq = wq_.to(qkv.scalar_type()).contiguous();
+    if (wk_.defined()) wk = wk_.to(qkv.scalar_type()).contiguous();
+  }
+  int64_t tokens() const { return B * T; }
+  int64_t seq() const { return T > 0 ? T : 1; }
+};
+
+std::vector<Tensor> rope_forward(const Tensor& qkv, const Tensor& cos, const Tensor& sin, const Tensor& positions,
+                                 const Tensor& wq, const Tensor& wk, const RopeHow& how) {
+  const RopeCall c(qkv, cos, sin, positions, wq, wk, how);
+  const Tensor q = at::empty({c.B, c.T, how.q_heads, c.D}, qkv.options());
+  const Tensor k = at::empty({c.B, c.T, how.kv_heads, c.D}, qkv.options());
+  const Tensor v = at::empty({c.B, c.T, how.kv_heads, c.D}, qkv.options());
+  const Launch on(c.qkv);
+  check_status(attnres_qk_norm_rope_forward(
+                   c.tokens(), c.seq(), how.q_heads, how.kv_heads, c.D, 2 * c.cos.size(1), c.code, ptr(c.qkv), c.stride,
+                   static_cast<const float*>(ptr(c.cos)), static_cast<const float*>(ptr(c.sin)), c.cos.size(0),
+                   ptr(c.positions), c.wide, ptr(c.wq), ptr(c.wk), how.normalize, how.eps, how.interleaved, mut(q),
+                   mut(k), mut(v), on.stream),
+               "attnres_qk_norm_rope_forward");
+  return {q, k, v};
+}
+
+// {d qkv, d q weight, d k weight}, undefined where not wanted.
+std::vector<Tensor> rope_backward(const std::array<Tensor, 3>& grads, const Tensor& qkv, const Tensor& cos,
+                                  const Tensor& sin, const Tensor& positions, const Tensor& wq, const Tensor& wk,
+                                  const RopeHow& how, bool want_wq, bool want_wk) {
+  const RopeCall c(qkv, cos, sin, positions, wq, wk, how);
+  Tensor g[3];
+  int64_t strides[9];
+  for (int i = 0; i < 3; ++i) {
+    const int64_t heads = i == 0 ? how.q_heads : how.kv_heads;
+    g[i] = grads[i];
+    if (!g[i].defined()) {  // an output that took no part in the loss
+      g[i] = at::zeros({1}, qkv.options()).expand({c.B, c.T, heads, c.D});
+    }
+    TORCH_CHECK(g[i].dim() == 4 && g[i].size(0) == c.B && g[i].size(1) == c.T && g[i].size(2) == heads &&
+                    g[i].size(3) == c.D,
+                "attnres_b200: qk_norm_rope backward takes gradients of its outputs' shapes");
+    check_device("qk_norm_rope", qkv, g[i]);
+    if (g[i].scalar_type() != qkv.scalar_type() || g[i].stride(3) != 1) g[i] = g[i].to(qkv.scalar_type()).contiguous();
+    for (int j = 0; j < 3; ++j) strides[3 * i + j] = g[i].stride(j);
+  }
+  const Tensor dqkv = at::empty({c.B, c.T, (how.q_heads + 2 * how.kv_heads) * c.D}, qkv.options());
+  Tensor dwq, dwk, workspace;
+  size_t bytes = 0;
+  if (want_wq || want_wk) {
+    const Launch on(c.qkv);
+    bytes = attnres_qk_norm_rope_backward_workspace_bytes(c.D);
+    workspace = at::empty({static_cast<int64_t>(bytes)}, qkv.options().dtype(at::kByte));
+    if (want_wq) dwq = at::empty({c.D}, qkv.options());
+    if (want_wk) dwk = at::empty({c.D}, qkv.options());
+  }
+  const Launch on(c.qkv);
+  check_status(attnres_qk_norm_rope_backward(
+                   c.tokens(), c.seq(), how.q_heads, how.kv_heads, c.D, 2 * c.cos.size(1), c.code, ptr(c.qkv), c.stride,
+                   static_cast<const float*>(ptr(c.cos)), static_cast<const float*>(ptr(c.sin)), c.cos.size(0),
+                   ptr(c.positions), c.wide, ptr(c.wq), ptr(c.wk), how.normalize, how.eps, how.interleaved, ptr(g[0]),
+                   ptr(g[1]), ptr(g[2]), strides, mut(dqkv), mut(dwq), mut(dwk), mut(workspace), bytes, on.stream),
+               "attnres_qk_norm_rope_backward");
+  if (dwq.defined()) dwq = dwq.to(wq.scalar_type());
+  if (dwk.defined()) dwk = dwk.to(wk.scalar_type());
+  return {dqkv, dwq, dwk};
+}
+
+struct QkNormRope : torch::autograd::Function<QkNormRope> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& qkv, const Tensor& cos, const Tensor& sin,
+                               const OptTensor& positions, const OptTensor& q_weight, const OptTensor& k_weight,
+                               const RopeHow& how) {
+    const Tensor pos = or_undefined(positions), wq = or_undefined(q_weight), wk = or_undefined(k_weight);
+    ctx->save_for_backward({qkv, cos, sin, pos, wq, wk});
+    ctx->saved_data["heads"] = std::vector<int64_t>{how.q_heads, how.kv_heads, how.normalize, how.interleaved};
+    ctx->saved_data["eps"] = how.eps;
+    ctx->set_materialize_grads(false);
+    return rope_forward(qkv, cos, sin, pos, wq, wk, how);
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& g) {
+    check_first_order("qk_norm_rope");
+    const auto s = ctx->get_saved_variables();
+    const auto h = ctx->saved_data["heads"].toIntVector();
+    const RopeHow how{h[0], h[1], h[2] != 0, ctx->saved_data["eps"].toDouble(), h[3] != 0};
+    // the context numbers the inputs that are there: qkv, cos, sin, positions, weights
+    size_t at = s[3].defined() ? 4 : 3;
+    const bool want_wq = s[4].defined() && ctx->needs_input_grad(at++);
+    const bool want_wk = s[5].defined() && ctx->needs_input_grad(at);
+    const auto d = rope_backward({g[0], g[1], g[2]}, s[0], s[1], s[2], s[3], s[4], s[5], how, want_wq, want_wk);
+    return {d[0], Tensor(), Tensor(), Tensor(), d[1], d[2], Tensor()};
+  }
+};
+
+py::tuple tuple3(const std::vector<Tensor>& t) { return py::make_tuple(t[0], t[1], t[2]); }
+
+bool wants_grad(std::initializer_list<const Tensor*> ts) {
+  if (!at::GradMode::is_enabled()) return false;
+  for (const Tensor* t : ts)
+    if (t->defined() && t->requires_grad()) return true;
+  return false;
+}
+
+py::tuple py_qk_norm_rope(const Tensor& qkv, int64_t q_heads, int64_t kv_heads, const Tensor& cos, const Tensor& sin,
+                          const OptTensor& positions, const OptTensor& q_weight, const OptTensor& k_weight, double eps,
+                          bool normalize, bool interleaved) {
+  const RopeHow how{q_heads, kv_heads, normalize, eps, interleaved};
+  const Tensor pos = or_undefined(positions), wq = or_undefined(q_weight), wk = or_undefined(k_weight);
+  if (wants_grad({&qkv, &wq, &wk}))
+    return tuple3(QkNormRope::apply(qkv, cos, sin, positions, q_weight, k_weight, how));
+  return tuple3(rope_forward(qkv, cos, sin, pos, wq, wk, how));
+}
+
+py::tuple py_qk_norm_rope_backward(const Tensor& gq, const Tensor& gk, const Tensor& gv, const Tensor& qkv,
+                                   const Tensor& cos, const Tensor& sin, const OptTensor& positions,
+                                   const OptTensor& q_weight, const OptTensor& k_weight, int64_t q_heads,
+                                   int64_t kv_heads, bool normalize, double eps, bool interleaved, bool want_wq,
+                                   bool want_wk) {
+  const RopeHow how{q_heads, kv_heads, normalize, eps, interleaved};
+  return tuple3(rope_backward({gq, gk, gv}, qkv, cos, sin, or_undefined(positions), or_undefined(q_weight),
+                              or_undefined(k_weight), how, want_wq, want_wk));
+}
+
+}  // namespace
+
+PYBIND11_MODULE(_layer, m) {
+  m.def("qk_norm_rope", &py_qk_norm_rope);
+  m.def("qk_norm_rope_backward", &py_qk_norm_rope_backward);
+}

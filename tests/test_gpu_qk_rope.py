@@ -265,6 +265,13 @@ def test_op_traces_under_compile():
         assert torch.equal(a, b)
 
 
+def test_second_derivative_is_refused():
+    qkv, _, grads, cos, sin, pos = inputs(1, 4, 2, 1, 64, torch.float32, weighted=False)
+    out = A.qk_norm_rope(qkv.requires_grad_(True), 2, 1, cos, sin, positions=pos)
+    with pytest.raises(RuntimeError, match="twice"):
+        torch.autograd.grad(out, [qkv], grads, create_graph=True)
+
+
 def test_refusals():
     cos, sin = tables(8, 32)
     qkv = torch.zeros(1, 4, 4 * 64, device="cuda")
