@@ -522,6 +522,28 @@ int attnres_qk_norm_rope_backward(int64_t num_tokens, int64_t seq_len, int q_hea
                                   void* grad_q_weight, void* grad_k_weight, void* workspace, size_t workspace_bytes,
                                   void* stream);
 
+/*
+ * Gated projection of the model's MLP (the reference's MLP.forward up to its
+ * output projection: fc1, chunk, silu, product): with W = [Wv; Wg] dtype
+ * [2 hidden, in_dim], the value rows first,
+ *   h = (x Wv^T) * silu(x Wg^T),   h dtype [num_tokens, hidden] dense.
+ * x dtype [num_tokens, in_dim], rows of x and W strided. bf16 / fp16 only, in_dim,
+ * hidden and the strides multiples of 8, 16-byte aligned buffers: anything else
+ * answers ATTNRES_ERR_UNSUPPORTED, launching nothing. Sums in fp32, h rounded once.
+ *
+ * Backward: u and g are formed again from x and W; grad_x dtype [num_tokens,
+ * in_dim] dense and grad_weight dtype [2 hidden, in_dim] dense, either NULL when
+ * not wanted. The workspace holds their gradients, rounded to dtype, between the
+ * products: attnres_swiglu_backward_workspace_bytes.
+ */
+int attnres_swiglu_forward(int64_t num_tokens, int in_dim, int hidden, int dtype, const void* x, int64_t x_row_stride,
+                           const void* weight, int64_t weight_row_stride, void* h, void* stream);
+size_t attnres_swiglu_backward_workspace_bytes(int64_t num_tokens, int hidden);
+int attnres_swiglu_backward(int64_t num_tokens, int in_dim, int hidden, int dtype, const void* x, int64_t x_row_stride,
+                            const void* weight, int64_t weight_row_stride, const void* grad_h,
+                            int64_t grad_h_row_stride, void* grad_x, void* grad_weight, void* workspace,
+                            size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -7,7 +7,7 @@ attnres::lrid_read / attnres::base_read operators, and exposes the reference's
 public read functions.
 """
 from . import _native
-from .layer import qk_norm_rope
+from .layer import qk_norm_rope, swiglu_projection
 from .ops import (
     attention_residual_block_summary,
     attention_residual_read,
@@ -45,4 +45,5 @@ __all__ = [
     "lrid_read_list_backward",
     "qk_norm_rope",
     "source_logit_bias",
+    "swiglu_projection",
 ]

@@ -57,6 +57,9 @@ EXPORTED_SYMBOLS = (
     "attnres_qk_norm_rope_forward",
     "attnres_qk_norm_rope_backward_workspace_bytes",
     "attnres_qk_norm_rope_backward",
+    "attnres_swiglu_forward",
+    "attnres_swiglu_backward_workspace_bytes",
+    "attnres_swiglu_backward",
 )
 
 _lib = None
@@ -209,6 +212,16 @@ def load(path=None):
     L.attnres_qk_norm_rope_backward.argtypes = rope + [
         P, P, P, PI64, P, P, P,      # grad q, k, v, strides, grad qkv, grad q weight, grad k weight
         P, SZ, P,                    # workspace, bytes, stream
+    ]
+    L.attnres_swiglu_forward.restype = I
+    L.attnres_swiglu_forward.argtypes = [I64, I, I, I, P, I64, P, I64, P, P]
+    L.attnres_swiglu_backward_workspace_bytes.restype = SZ
+    L.attnres_swiglu_backward_workspace_bytes.argtypes = [I64, I]
+    L.attnres_swiglu_backward.restype = I
+    L.attnres_swiglu_backward.argtypes = [
+        I64, I, I, I, P, I64, P, I64,  # tokens, in_dim, hidden, dtype, x, stride, weight, stride
+        P, I64, P, P,                  # grad h, stride, grad x, grad weight
+        P, SZ, P,                      # workspace, bytes, stream
     ]
     if path == LIB_PATH:
         _lib = L

@@ -3,6 +3,7 @@
   qk_norm_rope(...)       q/k/v split of a fused projection, per-head RMS norm of q and k and the
                           rotation by position in one pass (the steps of the reference's attention
                           between its projection and scaled_dot_product_attention)
+  swiglu_projection(...)  the gated half of the MLP: both projections, silu and the product in one kernel
 
 Every tensor argument must live on one CUDA device; the work is enqueued on that
 device's current stream through the C ABI. There is no CPU fallback: a CPU tensor
@@ -123,3 +124,55 @@ def qk_norm_rope(qkv: Tensor, num_heads: int, num_kv_heads: int, cos: Tensor, si
                                     interleaved)
     return qk_norm_rope_op(qkv, cos, sin, positions, q_weight, k_weight, int(num_heads), int(num_kv_heads),
                            bool(normalize), float(eps), bool(interleaved))
+
+
+# ---------------------------------------------------------------------------
+# gated projection
+# ---------------------------------------------------------------------------
+@torch.library.custom_op("attnres::swiglu_projection", mutates_args=())
+def swiglu_projection_op(x: Tensor, weight: Tensor) -> Tensor:
+    return _load().swiglu_projection(x, weight)
+
+
+@swiglu_projection_op.register_fake
+def _(x, weight):
+    return x.new_empty((*x.shape[:-1], weight.shape[0] // 2))
+
+
+@torch.library.custom_op("attnres::swiglu_projection_backward", mutates_args=())
+def swiglu_projection_backward_op(grad_h: Tensor, x: Tensor, weight: Tensor, want_x: bool,
+                                  want_weight: bool) -> tuple[Tensor, Tensor]:
+    """Empty tensors where a gradient is not wanted."""
+    dx, dw = _load().swiglu_projection_backward(grad_h, x, weight, want_x, want_weight)
+    return x.new_empty(0) if dx is None else dx, weight.new_empty(0) if dw is None else dw
+
+
+@swiglu_projection_backward_op.register_fake
+def _(grad_h, x, weight, want_x, want_weight):
+    return x.new_empty(x.shape if want_x else (0,)), weight.new_empty(weight.shape if want_weight else (0,))
+
+
+def _swiglu_setup(ctx, inputs, output):
+    ctx.save_for_backward(*inputs)
+
+
+def _swiglu_bwd(ctx, grad_h):
+    x, weight = ctx.saved_tensors
+    need = ctx.needs_input_grad
+    dx, dw = swiglu_projection_backward_op(grad_h, x, weight, need[0], need[1])
+    return dx if need[0] else None, dw if need[1] else None
+
+
+swiglu_projection_op.register_autograd(_swiglu_bwd, setup_context=_swiglu_setup)
+
+
+def swiglu_projection(x: Tensor, weight: Tensor) -> Tensor:
+    """h = v * silu(g) with [v, g] = x weight^T, the model's MLP up to its output projection.
+
+    x [..., in] float16 or bfloat16; weight [2 * hidden, in] holds the value rows, then the gate rows
+    (the layout of the model's fc1), and is cast to x's type. Both widths are multiples of 8. The
+    products are summed and gated in fp32, h [..., hidden] is rounded once. Differentiable in both;
+    the backward forms v and g again rather than keeping them."""
+    if _eager(x, weight):
+        return _load().swiglu_projection(x, weight)
+    return swiglu_projection_op(x, weight)

@@ -9,6 +9,7 @@
 
 #include "common.cuh"
 #include "plan.h"
+#include "swiglu.h"
 
 namespace {
 
@@ -148,6 +149,8 @@ int attnres_device_status(unsigned* status, int reset) {
   if (e == cudaSuccess) e = attnres::read_kvfused_status(&s4, reset != 0);
   s3 |= s4;
   if (e == cudaSuccess) e = attnres::read_kvbwd_status(&s4, reset != 0);
+  s3 |= s4;
+  if (e == cudaSuccess) e = attnres::read_swiglu_status(&s4, reset != 0);
   s3 |= s4;
   if (e != cudaSuccess) return cuda_fail(e, "attnres_device_status");
   *status = s1 | s2 | s3;

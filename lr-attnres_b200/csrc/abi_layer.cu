@@ -6,6 +6,7 @@
 #include "common.cuh"
 #include "plan.h"
 #include "qkrope.h"
+#include "swiglu.h"
 
 namespace {
 
@@ -82,6 +83,25 @@ attnres::QkRopeArgs qk_rope_args(int64_t num_tokens, int64_t seq_len, int q_head
   return a;
 }
 
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+int check_swiglu(int64_t n, int in_dim, int hidden, int dtype, const void* x, int64_t xs, const void* w, int64_t ws) {
+  if (n < 0 || in_dim < 1 || hidden < 1)
+    return fail(ATTNRES_ERR_INVALID_ARGUMENT, "swiglu: num_tokens=%lld, in_dim=%d, hidden=%d must be positive",
+                (long long)n, in_dim, hidden);
+  if (!known_dtype(dtype)) return fail(ATTNRES_ERR_INVALID_ARGUMENT, "unknown dtype %d", dtype);
+  if (dtype == ATTNRES_DTYPE_F32) return fail(ATTNRES_ERR_UNSUPPORTED, "swiglu: float16 and bfloat16 only");
+  if (in_dim % 8 || hidden % 8 || hidden > (1 << 28))
+    return fail(ATTNRES_ERR_UNSUPPORTED, "swiglu: in_dim=%d and hidden=%d must be multiples of 8", in_dim, hidden);
+  if (n > 0x7fffffffLL || (n / 128 + 1) * (hidden / 128 + 1) > 0x7fffffffLL)
+    return fail(ATTNRES_ERR_UNSUPPORTED, "swiglu: num_tokens=%lld is too many for one launch", (long long)n);
+  if (xs < in_dim || ws < in_dim) return fail(ATTNRES_ERR_INVALID_ARGUMENT, "swiglu: a row stride below in_dim");
+  if (!w || (n > 0 && !x)) return fail(ATTNRES_ERR_INVALID_ARGUMENT, "swiglu: x or weight is NULL");
+  if (xs % 8 || ws % 8 || !aligned16(x) || !aligned16(w))
+    return fail(ATTNRES_ERR_UNSUPPORTED, "swiglu: rows of x and weight must start on 16-byte boundaries");
+  return ATTNRES_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -149,6 +169,66 @@ int attnres_qk_norm_rope_backward(int64_t num_tokens, int64_t seq_len, int q_hea
     a.partials = static_cast<float*>(workspace);
   }
   return launched(attnres::qkrope_launch(true, dtype, a, st), "attnres_qk_norm_rope_backward launch");
+}
+
+int attnres_swiglu_forward(int64_t num_tokens, int in_dim, int hidden, int dtype, const void* x, int64_t x_row_stride,
+                           const void* weight, int64_t weight_row_stride, void* h, void* stream) {
+  int rc = check_swiglu(num_tokens, in_dim, hidden, dtype, x, x_row_stride, weight, weight_row_stride);
+  if (rc || num_tokens == 0) return rc;
+  if (!h) return fail(ATTNRES_ERR_INVALID_ARGUMENT, "swiglu: h is NULL");
+  if (!aligned16(h)) return fail(ATTNRES_ERR_UNSUPPORTED, "swiglu: h must start on a 16-byte boundary");
+  attnres::SwigluArgs a{};
+  a.N = num_tokens;
+  a.C = in_dim;
+  a.F = hidden;
+  a.x = x;
+  a.w = weight;
+  a.x_stride = x_row_stride;
+  a.w_stride = weight_row_stride;
+  a.out = h;
+  return launched(attnres::swiglu_launch(false, dtype, a, static_cast<cudaStream_t>(stream)),
+                  "attnres_swiglu_forward launch");
+}
+
+size_t attnres_swiglu_backward_workspace_bytes(int64_t num_tokens, int hidden) {
+  return num_tokens < 1 || hidden < 1 ? 0 : static_cast<size_t>(num_tokens) * 4 * hidden;
+}
+
+int attnres_swiglu_backward(int64_t num_tokens, int in_dim, int hidden, int dtype, const void* x, int64_t x_row_stride,
+                            const void* weight, int64_t weight_row_stride, const void* grad_h,
+                            int64_t grad_h_row_stride, void* grad_x, void* grad_weight, void* workspace,
+                            size_t workspace_bytes, void* stream) {
+  int rc = check_swiglu(num_tokens, in_dim, hidden, dtype, x, x_row_stride, weight, weight_row_stride);
+  if (rc) return rc;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (num_tokens == 0)
+    return launched(grad_weight ? cudaMemsetAsync(grad_weight, 0, static_cast<size_t>(hidden) * in_dim * 4, st)
+                                : cudaSuccess,
+                    "attnres_swiglu_backward memset");
+  if (!grad_x && !grad_weight) return ATTNRES_OK;
+  if (!grad_h) return fail(ATTNRES_ERR_INVALID_ARGUMENT, "swiglu backward: grad_h is NULL");
+  if (grad_h_row_stride < hidden)
+    return fail(ATTNRES_ERR_INVALID_ARGUMENT, "swiglu backward: grad_h_row_stride below hidden");
+  if (grad_h_row_stride % 8 || !aligned16(grad_h) || !aligned16(grad_x) || !aligned16(grad_weight) ||
+      !aligned16(workspace))
+    return fail(ATTNRES_ERR_UNSUPPORTED, "swiglu backward: buffers and rows must start on 16-byte boundaries");
+  const size_t need = attnres_swiglu_backward_workspace_bytes(num_tokens, hidden);
+  if (!workspace || workspace_bytes < need)
+    return fail(ATTNRES_ERR_WORKSPACE, "swiglu backward: workspace of %zu bytes, %zu needed", workspace_bytes, need);
+  attnres::SwigluArgs a{};
+  a.N = num_tokens;
+  a.C = in_dim;
+  a.F = hidden;
+  a.x = x;
+  a.w = weight;
+  a.x_stride = x_row_stride;
+  a.w_stride = weight_row_stride;
+  a.dh = grad_h;
+  a.dh_stride = grad_h_row_stride;
+  a.dx = grad_x;
+  a.dw = grad_weight;
+  a.workspace = workspace;
+  return launched(attnres::swiglu_launch(true, dtype, a, st), "attnres_swiglu_backward launch");
 }
 
 }  // extern "C"

@@ -235,9 +235,108 @@ py::tuple py_qk_norm_rope_backward(const Tensor& gq, const Tensor& gk, const Ten
                               or_undefined(k_weight), how, want_wq, want_wk));
 }
 
+// ---------------------------------------------------------------------------
+// swiglu_projection
+// ---------------------------------------------------------------------------
+// t as [rows, width] with 16-byte aligned rows that do not overlap, copied only if
+// it is not.
+Tensor packed_rows(const Tensor& t, int64_t rows, int64_t width) {
+  Tensor m = t.reshape({rows, width});
+  const int64_t stride = m.size(0) > 1 ? m.stride(0) : width;
+  const bool aligned = reinterpret_cast<uintptr_t>(m.const_data_ptr()) % 16 == 0;
+  if (m.stride(1) == 1 && stride >= width && stride % 8 == 0 && aligned) return m;
+  return m.is_contiguous() ? m.clone() : m.contiguous();
+}
+int64_t row_stride(const Tensor& m) { return m.size(0) > 1 ? m.stride(0) : m.size(1); }
+
+struct SwigluCall {
+  Tensor x, w;
+  int64_t N, C, F;
+  int code;
+
+  SwigluCall(const Tensor& x_, const Tensor& w_) {
+    const char* what = "swiglu_projection";
+    check_cuda(what, x_);
+    check_device(what, x_, w_);
+    TORCH_CHECK(x_.scalar_type() == at::kHalf || x_.scalar_type() == at::kBFloat16,
+                "attnres_b200: swiglu_projection takes float16 or bfloat16, got ", x_.scalar_type());
+    TORCH_CHECK(x_.dim() >= 1 && w_.dim() == 2 && w_.size(1) == x_.size(-1) && w_.size(0) % 2 == 0,
+                "attnres_b200: swiglu_projection takes x [..., in] and weight [2 * hidden, in], got ", x_.sizes(), " and ",
+                w_.sizes());
+    C = x_.size(-1);
+    F = w_.size(0) / 2;
+    TORCH_CHECK(C > 0 && F > 0 && C % 8 == 0 && F % 8 == 0 && C < (1 << 28) && F < (1 << 28),
+                "attnres_b200: swiglu_projection takes widths that are multiples of 8, got in ", C, " and hidden ", F);
+    N = x_.numel() / C;
+    code = dtype_code(x_);
+    x = packed_rows(x_, N, C);
+    w = packed_rows(w_.to(x_.scalar_type()), 2 * F, C);
+  }
+};
+
+std::vector<int64_t> with_last(const Tensor& x, int64_t last) {
+  std::vector<int64_t> shape = x.sizes().vec();
+  shape.back() = last;
+  return shape;
+}
+
+Tensor swiglu_forward(const Tensor& x, const Tensor& w) {
+  const SwigluCall c(x, w);
+  const Tensor h = at::empty(with_last(x, c.F), x.options());
+  const Launch on(c.x);
+  check_status(attnres_swiglu_forward(c.N, c.C, c.F, c.code, ptr(c.x), row_stride(c.x), ptr(c.w), row_stride(c.w), mut(h),
+                                      on.stream),
+               "attnres_swiglu_forward");
+  return h;
+}
+
+// {dx, dW}, undefined where not wanted.
+std::vector<Tensor> swiglu_backward(const Tensor& grad_h, const Tensor& x, const Tensor& w, bool want_x, bool want_w) {
+  const SwigluCall c(x, w);
+  check_device("swiglu_projection", x, grad_h);
+  TORCH_CHECK(grad_h.dim() == x.dim() && grad_h.numel() == c.N * c.F && (x.dim() == 0 || grad_h.size(-1) == c.F),
+              "attnres_b200: swiglu_projection backward takes a gradient of its output's shape");
+  const Tensor g = packed_rows(grad_h.to(x.scalar_type()), c.N, c.F);
+  Tensor dx, dw;
+  if (want_x) dx = at::empty(x.sizes(), x.options());
+  if (want_w) dw = at::empty({2 * c.F, c.C}, x.options());
+  const int64_t bytes = attnres_swiglu_backward_workspace_bytes(c.N, c.F);
+  const Tensor workspace = at::empty({bytes}, x.options().dtype(at::kByte));
+  const Launch on(c.x);
+  check_status(attnres_swiglu_backward(c.N, c.C, c.F, c.code, ptr(c.x), row_stride(c.x), ptr(c.w), row_stride(c.w), ptr(g),
+                                       row_stride(g), mut(dx), mut(dw), mut(workspace), bytes, on.stream),
+               "attnres_swiglu_backward");
+  if (want_w) dw = dw.to(w.scalar_type());
+  return {dx, dw};
+}
+
+struct Swiglu : torch::autograd::Function<Swiglu> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w) {
+    ctx->save_for_backward({x, w});
+    return swiglu_forward(x, w);
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& g) {
+    check_first_order("swiglu_projection");
+    const auto s = ctx->get_saved_variables();
+    return swiglu_backward(g[0], s[0], s[1], ctx->needs_input_grad(0), ctx->needs_input_grad(1));
+  }
+};
+
+Tensor py_swiglu(const Tensor& x, const Tensor& w) {
+  if (wants_grad({&x, &w})) return Swiglu::apply(x, w);
+  return swiglu_forward(x, w);
+}
+
+py::tuple py_swiglu_backward(const Tensor& grad_h, const Tensor& x, const Tensor& w, bool want_x, bool want_w) {
+  const auto d = swiglu_backward(grad_h, x, w, want_x, want_w);
+  return py::make_tuple(d[0], d[1]);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_layer, m) {
+  m.def("swiglu_projection", &py_swiglu);
+  m.def("swiglu_projection_backward", &py_swiglu_backward);
   m.def("qk_norm_rope", &py_qk_norm_rope);
   m.def("qk_norm_rope_backward", &py_qk_norm_rope_backward);
 }
