@@ -544,6 +544,58 @@ int attnres_swiglu_backward(int64_t num_tokens, int in_dim, int hidden, int dtyp
                             int64_t grad_h_row_stride, void* grad_x, void* grad_weight, void* workspace,
                             size_t workspace_bytes, void* stream);
 
+/*
+ * Keys and values of past tokens in 4 bits, in pages. A group of 32 elements of a
+ * head holds step and low (float16) and 32 codes: element = low + step * code. With
+ * G = head_dim / 32, the pool's arrays are
+ *   k_params, v_params  [num_pages, kv_heads, page_size, G] pairs {step, low}
+ *   k_codes, v_codes    [num_pages, kv_heads, page_size] rows of head_dim / 2 bytes:
+ *     keys    4 x G 32-bit words; word (c, g) at byte 4 (c G + g): elements 32 g + 8 c + 0..7
+ *     values  8 x G 16-bit words; word (r, g) at byte 2 (r G + g): elements 32 g + 4 r + 0..3
+ *     (the lower element in the lower bits): the order in which the attention's
+ *     tensor-core lanes take them.
+ * 16-byte aligned; page_size a multiple of 16, head_dim of 32 up to 512. Place t of
+ * sequence b lies in page page_table[b][t / page_size] (int32, rows
+ * page_table_stride apart, max_pages entries each). A place that the table has no
+ * valid page for is neither written nor read, and sets bit 8 of the status word
+ * (attnres_device_status).
+ *
+ * attnres_kv4_append quantises k and v dtype [batch, new_tokens, kv_heads, head_dim]
+ * (element strides {sequence, token, head}, last dim dense) into places start[b] ..
+ * start[b] + counts[b] (counts NULL: new_tokens each):
+ *   step = f16((max - min) / 15), low = f16(min), code = clamp(rint((x - low) / step))
+ * A group with an infinity or NaN reads back as NaN.
+ * attnres_kv4_read writes the values of the same places, dtype [batch, new_tokens,
+ * kv_heads, head_dim] dense, zeros where there is none.
+ */
+int attnres_kv4_append(void* k_codes, void* k_params, void* v_codes, void* v_params, int64_t num_pages, int kv_heads,
+                       int page_size, int head_dim, const int* page_table, int64_t page_table_stride, int max_pages,
+                       const int* start, const int* counts, int batch, int new_tokens, int dtype, const void* k,
+                       const int64_t* k_strides, const void* v, const int64_t* v_strides, void* stream);
+int attnres_kv4_read(const void* k_codes, const void* k_params, const void* v_codes, const void* v_params,
+                     int64_t num_pages, int kv_heads, int page_size, int head_dim, const int* page_table,
+                     int64_t page_table_stride, int max_pages, const int* start, const int* counts, int batch,
+                     int new_tokens, int dtype, void* k, void* v, void* stream);
+
+/*
+ * Attention of new tokens over that cache, their own keys and values in it already.
+ * lengths[b] counts the sequence's keys with the new ones; token t < counts[b]
+ * (NULL: new_tokens) stands at place lengths[b] - counts[b] + t and sees the places
+ * up to its own. q dtype [batch, new_tokens, q_heads, head_dim] with element strides
+ * {sequence, token, head}; query head h reads key head h / (q_heads / kv_heads). out
+ * dtype [batch, new_tokens, q_heads, head_dim] and lse float [batch, new_tokens,
+ * q_heads] (log of the softmax's sum, NULL if not wanted), dense. A row that sees
+ * nothing is zeros, its lse -inf. bf16 / fp16, head_dim 64 or 128. Workspace:
+ * attnres_kv4_attention_workspace_bytes (may be 0).
+ */
+size_t attnres_kv4_attention_workspace_bytes(int kv_heads, int page_size, int head_dim, int max_pages, int batch,
+                                             int new_tokens, int q_heads);
+int attnres_kv4_attention(const void* k_codes, const void* k_params, const void* v_codes, const void* v_params,
+                          int64_t num_pages, int kv_heads, int page_size, int head_dim, const int* page_table,
+                          int64_t page_table_stride, int max_pages, const int* lengths, const int* counts, int batch,
+                          int new_tokens, int q_heads, int dtype, const void* q, const int64_t* q_strides, float scale,
+                          void* out, float* lse, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -7,7 +7,7 @@ attnres::lrid_read / attnres::base_read operators, and exposes the reference's
 public read functions.
 """
 from . import _native
-from .layer import qk_norm_rope, swiglu_projection
+from .layer import KV4Cache, kv4_append, kv4_attention, kv4_read, qk_norm_rope, swiglu_projection
 from .ops import (
     attention_residual_block_summary,
     attention_residual_read,
@@ -28,12 +28,16 @@ from .ops import (
 )
 
 __all__ = [
+    "KV4Cache",
     "attention_residual_block_summary",
     "attention_residual_read",
     "block_summary",
     "block_summary_norm",
     "base_read",
     "is_fused_attnres_available",
+    "kv4_append",
+    "kv4_attention",
+    "kv4_read",
     "lrid_attention_residual_read",
     "lrid_attention_residual_read_gated",
     "lrid_attention_residual_read_key_from_value",

@@ -60,6 +60,10 @@ EXPORTED_SYMBOLS = (
     "attnres_swiglu_forward",
     "attnres_swiglu_backward_workspace_bytes",
     "attnres_swiglu_backward",
+    "attnres_kv4_append",
+    "attnres_kv4_read",
+    "attnres_kv4_attention_workspace_bytes",
+    "attnres_kv4_attention",
 )
 
 _lib = None
@@ -222,6 +226,19 @@ def load(path=None):
         I64, I, I, I, P, I64, P, I64,  # tokens, in_dim, hidden, dtype, x, stride, weight, stride
         P, I64, P, P,                  # grad h, stride, grad x, grad weight
         P, SZ, P,                      # workspace, bytes, stream
+    ]
+    pool = [P, P, P, P, I64, I, I, I, P, I64, I]  # codes / params x2, pages, kv heads, page size, head_dim, table, stride, max pages
+    L.attnres_kv4_append.restype = I
+    L.attnres_kv4_append.argtypes = pool + [P, P, I, I, I, P, PI64, P, PI64, P]
+    L.attnres_kv4_read.restype = I
+    L.attnres_kv4_read.argtypes = pool + [P, P, I, I, I, P, P, P]
+    L.attnres_kv4_attention_workspace_bytes.restype = SZ
+    L.attnres_kv4_attention_workspace_bytes.argtypes = [I] * 7
+    L.attnres_kv4_attention.restype = I
+    L.attnres_kv4_attention.argtypes = pool + [
+        P, P, I, I, I, I,            # lengths, counts, batch, new tokens, q heads, dtype
+        P, PI64, F, P, P,            # q, strides, scale, out, lse
+        P, SZ, P,                    # workspace, bytes, stream
     ]
     if path == LIB_PATH:
         _lib = L

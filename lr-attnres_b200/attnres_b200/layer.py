@@ -4,6 +4,9 @@
                           rotation by position in one pass (the steps of the reference's attention
                           between its projection and scaled_dot_product_attention)
   swiglu_projection(...)  the gated half of the MLP: both projections, silu and the product in one kernel
+  KV4Cache, kv4_append, kv4_read, kv4_attention
+                          keys and values of past tokens in 4 bits, in pages: written, read back, and
+                          attended to by new tokens
 
 Every tensor argument must live on one CUDA device; the work is enqueued on that
 device's current stream through the C ABI. There is no CPU fallback: a CPU tensor
@@ -176,3 +179,120 @@ def swiglu_projection(x: Tensor, weight: Tensor) -> Tensor:
     if _eager(x, weight):
         return _load().swiglu_projection(x, weight)
     return swiglu_projection_op(x, weight)
+
+
+# ---------------------------------------------------------------------------
+# 4-bit key/value cache
+# ---------------------------------------------------------------------------
+class KV4Cache:
+    """A pool of pages of keys and values in 4 bits.
+
+    Groups of 32 elements of a head: element = low + step * code. k_codes, v_codes uint8 [pages,
+    kv_heads, page_size, head_dim / 2]; k_params, v_params float16 [pages, kv_heads, page_size,
+    head_dim / 32, 2] hold each group's step and low. A row's codes lie in the order in which the
+    attention's tensor-core lanes take them (include/attnres_b200.h). page_size is a multiple of 16,
+    head_dim of 32; 5 bits an element in all.
+
+    The sequences' pages are the caller's to hand out: place t of sequence b is in page
+    page_table[b, t // page_size]. Calls touch the places they are given and nothing else; a place
+    without a valid page is skipped (bit 8 of the device status word tells)."""
+
+    __slots__ = ("k_codes", "k_params", "v_codes", "v_params")
+
+    def __init__(self, k_codes: Tensor, k_params: Tensor, v_codes: Tensor, v_params: Tensor):
+        self.k_codes, self.k_params, self.v_codes, self.v_params = k_codes, k_params, v_codes, v_params
+
+    @classmethod
+    def empty(cls, num_pages: int, page_size: int, num_kv_heads: int, head_dim: int, device="cuda"):
+        """A pool whose places hold nothing yet."""
+        if page_size < 16 or page_size % 16 or head_dim < 32 or head_dim % 32:
+            raise RuntimeError(f"attnres_b200: KV4Cache takes a page_size that is a multiple of 16 and a head_dim that is "
+                               f"a multiple of 32, got {page_size} and {head_dim}")
+        codes = (num_pages, num_kv_heads, page_size, head_dim // 2)
+        params = (num_pages, num_kv_heads, page_size, head_dim // 32, 2)
+        make = [torch.empty(shape, device=device, dtype=dt)
+                for _ in range(2) for shape, dt in ((codes, torch.uint8), (params, torch.float16))]
+        return cls(*make)
+
+    def tensors(self):
+        return self.k_codes, self.k_params, self.v_codes, self.v_params
+
+
+@torch.library.custom_op("attnres::kv4_append", mutates_args=("k_codes", "k_params", "v_codes", "v_params"))
+def kv4_append_op(k_codes: Tensor, k_params: Tensor, v_codes: Tensor, v_params: Tensor, k: Tensor, v: Tensor,
+                  page_table: Tensor, start: Tensor, counts: Optional[Tensor]) -> None:
+    _load().kv4_append(k_codes, k_params, v_codes, v_params, k, v, page_table, start, counts)
+
+
+@kv4_append_op.register_fake
+def _(k_codes, k_params, v_codes, v_params, k, v, page_table, start, counts):
+    return None
+
+
+@torch.library.custom_op("attnres::kv4_read", mutates_args=())
+def kv4_read_op(k_codes: Tensor, k_params: Tensor, v_codes: Tensor, v_params: Tensor, page_table: Tensor, start: Tensor,
+                tokens: int, counts: Optional[Tensor], dtype: torch.dtype) -> tuple[Tensor, Tensor]:
+    return _load().kv4_read(k_codes, k_params, v_codes, v_params, page_table, start, tokens, counts, dtype)
+
+
+@kv4_read_op.register_fake
+def _(k_codes, k_params, v_codes, v_params, page_table, start, tokens, counts, dtype):
+    shape = (page_table.shape[0], tokens, k_codes.shape[1], 2 * k_codes.shape[3])
+    return k_codes.new_empty(shape, dtype=dtype), k_codes.new_empty(shape, dtype=dtype)
+
+
+@torch.library.custom_op("attnres::kv4_attention", mutates_args=())
+def kv4_attention_op(q: Tensor, k_codes: Tensor, k_params: Tensor, v_codes: Tensor, v_params: Tensor, page_table: Tensor,
+                     lengths: Tensor, counts: Optional[Tensor], scale: float) -> tuple[Tensor, Tensor]:
+    return _load().kv4_attention(q, k_codes, k_params, v_codes, v_params, page_table, lengths, counts, scale, True)
+
+
+@kv4_attention_op.register_fake
+def _(q, k_codes, k_params, v_codes, v_params, page_table, lengths, counts, scale):
+    return q.new_empty(q.shape), q.new_empty(q.shape[:3], dtype=torch.float32)
+
+
+def kv4_append(cache: KV4Cache, k: Tensor, v: Tensor, page_table: Tensor, start: Tensor,
+               counts: Optional[Tensor] = None) -> None:
+    """Quantises the new tokens' keys and values into places start[b] .. of the cache.
+
+    k, v [B, T, kv_heads, head_dim] float32, float16 or bfloat16, any strides; page_table int32
+    [B, max_pages]; start int32 [B] (how many keys the sequence holds already); counts int32 [B]
+    (default T): how many of the T tokens sequence b really has. Step and low are rounded to float16
+    and each code is the nearest value to what will be read back. Groups that hold an infinity or a NaN
+    read back as NaN. No gradient."""
+    if _eager(k, v, page_table, start, counts):
+        _load().kv4_append(cache.k_codes, cache.k_params, cache.v_codes, cache.v_params, k, v, page_table, start, counts)
+    else:
+        kv4_append_op(*cache.tensors(), k, v, page_table, start, counts)
+
+
+def kv4_read(cache: KV4Cache, page_table: Tensor, start: Tensor, tokens: int, counts: Optional[Tensor] = None,
+             dtype: torch.dtype = torch.bfloat16):
+    """The keys and values in places start[b] .. start[b] + tokens of each sequence: two tensors
+    [B, tokens, kv_heads, head_dim], zeros from counts[b] on and where there is no page."""
+    if _eager(cache.k_codes, page_table, start, counts):
+        return _load().kv4_read(cache.k_codes, cache.k_params, cache.v_codes, cache.v_params, page_table, start, tokens,
+                                counts, dtype)
+    return kv4_read_op(*cache.tensors(), page_table, start, int(tokens), counts, dtype)
+
+
+def kv4_attention(q: Tensor, cache: KV4Cache, page_table: Tensor, lengths: Tensor, counts: Optional[Tensor] = None,
+                  scale: Optional[float] = None, return_lse: bool = False):
+    """Attention of new tokens over the cache, which holds their own keys and values already.
+
+    q [B, T, heads, head_dim] float16 or bfloat16, head_dim 64 or 128; query head h reads key head
+    h // (heads / kv_heads). lengths int32 [B] counts a sequence's keys, the new ones among them; its
+    token t < counts[b] (int32, default T) stands at place lengths[b] - counts[b] + t and sees the
+    places up to its own. scale defaults to head_dim ** -0.5. Returns out [B, T, heads, head_dim] in
+    q's type, with return_lse also the log of the softmax's sum, float32 [B, T, heads]. A token that
+    sees nothing gives zeros and -inf. Meant for one to a few new tokens: the cache is read once for
+    every 16 query rows of a key head. No gradient."""
+    if scale is None:
+        scale = q.shape[-1] ** -0.5
+    if _eager(q, cache.k_codes, page_table, lengths, counts):
+        out, lse = _load().kv4_attention(q, cache.k_codes, cache.k_params, cache.v_codes, cache.v_params, page_table,
+                                         lengths, counts, scale, return_lse)
+    else:
+        out, lse = kv4_attention_op(q, *cache.tensors(), page_table, lengths, counts, float(scale))
+    return (out, lse) if return_lse else out

@@ -17,7 +17,7 @@ INCLUDE = os.path.join(os.path.dirname(HERE), "include")
 OUT = os.path.join(HERE, "attnres_b200", "libattnres_b200.so")
 SOURCES = ["abi.cu", "lrid.cu", "lrid_warp.cu", "lrid_stream_fwd.cu", "lrid_stream_bwd_f32.cu",
            "lrid_stream_bwd_f16.cu", "lrid_stream_bwd_bf16.cu", "base.cu", "keyproj.cu", "kvfused.cu", "keyproj_bwd.cu", "kvbwd.cu", "phase1.cu", "phase2.cu", "headnorm.cu", "summary.cu", "noalloc.cu", "launch_cache.cu",
-           "abi_layer.cu", "qkrope.cu", "swiglu.cu"]
+           "abi_layer.cu", "qkrope.cu", "swiglu.cu", "kv4_cache.cu", "kv4_attn.cu"]
 BINDING = os.path.join(HERE, "attnres_b200", "_layer.so")  # PyTorch binding of the layer operators, over OUT
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC,-O2", "--expt-relaxed-constexpr"]

@@ -8,6 +8,7 @@
 #include <string>
 
 #include "common.cuh"
+#include "kv4.h"
 #include "plan.h"
 #include "swiglu.h"
 
@@ -151,6 +152,10 @@ int attnres_device_status(unsigned* status, int reset) {
   if (e == cudaSuccess) e = attnres::read_kvbwd_status(&s4, reset != 0);
   s3 |= s4;
   if (e == cudaSuccess) e = attnres::read_swiglu_status(&s4, reset != 0);
+  s3 |= s4;
+  if (e == cudaSuccess) e = attnres::read_kv4_status(&s4, reset != 0);
+  s3 |= s4;
+  if (e == cudaSuccess) e = attnres::read_kv4_attn_status(&s4, reset != 0);
   s3 |= s4;
   if (e != cudaSuccess) return cuda_fail(e, "attnres_device_status");
   *status = s1 | s2 | s3;

@@ -4,6 +4,7 @@
 #include <stdio.h>
 
 #include "common.cuh"
+#include "kv4.h"
 #include "plan.h"
 #include "qkrope.h"
 #include "swiglu.h"
@@ -99,6 +100,45 @@ int check_swiglu(int64_t n, int in_dim, int hidden, int dtype, const void* x, in
   if (!w || (n > 0 && !x)) return fail(ATTNRES_ERR_INVALID_ARGUMENT, "swiglu: x or weight is NULL");
   if (xs % 8 || ws % 8 || !aligned16(x) || !aligned16(w))
     return fail(ATTNRES_ERR_UNSUPPORTED, "swiglu: rows of x and weight must start on 16-byte boundaries");
+  return ATTNRES_OK;
+}
+
+// The pool, the page table and the counts, as every cache entry takes them.
+int check_kv4(const attnres::Kv4Cache& c, int max_pages, int64_t table_stride, int batch, int new_tokens) {
+  if (c.pages < 0 || c.heads < 1 || c.page < 1 || c.D < 1 || max_pages < 0 || batch < 0 || new_tokens < 0)
+    return fail(ATTNRES_ERR_INVALID_ARGUMENT, "kv4 cache: a size is negative or zero");
+  if (c.page % 16 || c.D % attnres::kKv4Group || c.D > attnres::kKv4MaxDim)
+    return fail(ATTNRES_ERR_UNSUPPORTED, "kv4 cache: page_size=%d must be a multiple of 16, head_dim=%d of 32 up to %d",
+                c.page, c.D, attnres::kKv4MaxDim);
+  if (batch > 65535 || c.heads > 65535)
+    return fail(ATTNRES_ERR_UNSUPPORTED, "kv4 cache: batch=%d and kv_heads=%d up to 65535", batch, c.heads);
+  if (static_cast<int64_t>(max_pages) * c.page > (1LL << 30))
+    return fail(ATTNRES_ERR_UNSUPPORTED, "kv4 cache: a sequence of %d pages of %d places is too long", max_pages, c.page);
+  if (table_stride < max_pages && batch > 1)
+    return fail(ATTNRES_ERR_INVALID_ARGUMENT, "kv4 cache: page_table_stride below max_pages");
+  return ATTNRES_OK;
+}
+
+int check_kv4_buffers(const attnres::Kv4Cache& c, const int* table, int max_pages, const int* per_sequence) {
+  if (c.pages > 0 && (!c.k_codes || !c.k_params || !c.v_codes || !c.v_params))
+    return fail(ATTNRES_ERR_INVALID_ARGUMENT, "kv4 cache: a buffer of the pool is NULL");
+  if (!per_sequence || (max_pages > 0 && !table))
+    return fail(ATTNRES_ERR_INVALID_ARGUMENT, "kv4 cache: page_table, start or lengths is NULL");
+  if (!aligned16(c.k_codes) || !aligned16(c.k_params) || !aligned16(c.v_codes) || !aligned16(c.v_params))
+    return fail(ATTNRES_ERR_UNSUPPORTED, "kv4 cache: the pool's buffers must start on 16-byte boundaries");
+  return ATTNRES_OK;
+}
+
+attnres::Kv4Cache kv4_cache(const void* k_codes, const void* k_params, const void* v_codes, const void* v_params,
+                            int64_t pages, int heads, int page, int D) {
+  return {const_cast<void*>(k_codes), const_cast<void*>(k_params), const_cast<void*>(v_codes),
+          const_cast<void*>(v_params), pages, heads, page, D};
+}
+
+// One thread for 8 elements of a key and its value in 32-bit block counts.
+int check_kv4_rows(const attnres::Kv4RowsArgs& a) {
+  if (static_cast<double>(a.B) * a.T * a.c.heads * (a.c.D / 8) > 256.0 * 0x7fffffff)
+    return fail(ATTNRES_ERR_UNSUPPORTED, "kv4 cache: too many tokens for one launch");
   return ATTNRES_OK;
 }
 
@@ -229,6 +269,119 @@ int attnres_swiglu_backward(int64_t num_tokens, int in_dim, int hidden, int dtyp
   a.dw = grad_weight;
   a.workspace = workspace;
   return launched(attnres::swiglu_launch(true, dtype, a, st), "attnres_swiglu_backward launch");
+}
+
+int attnres_kv4_append(void* k_codes, void* k_params, void* v_codes, void* v_params, int64_t num_pages, int kv_heads,
+                       int page_size, int head_dim, const int* page_table, int64_t page_table_stride, int max_pages,
+                       const int* start, const int* counts, int batch, int new_tokens, int dtype, const void* k,
+                       const int64_t* k_strides, const void* v, const int64_t* v_strides, void* stream) {
+  attnres::Kv4RowsArgs a{};
+  a.c = kv4_cache(k_codes, k_params, v_codes, v_params, num_pages, kv_heads, page_size, head_dim);
+  int rc = check_kv4(a.c, max_pages, page_table_stride, batch, new_tokens);
+  if (rc) return rc;
+  if (!known_dtype(dtype)) return fail(ATTNRES_ERR_INVALID_ARGUMENT, "unknown dtype %d", dtype);
+  if (batch == 0 || new_tokens == 0) return ATTNRES_OK;
+  if ((rc = check_kv4_buffers(a.c, page_table, max_pages, start))) return rc;
+  if (!k || !v || !k_strides || !v_strides) return fail(ATTNRES_ERR_INVALID_ARGUMENT, "kv4 append: k or v is NULL");
+  a.table = page_table;
+  a.table_stride = page_table_stride;
+  a.max_pages = max_pages;
+  a.start = start;
+  a.counts = counts;
+  a.B = batch;
+  a.T = new_tokens;
+  a.k = k;
+  a.v = v;
+  for (int i = 0; i < 3; ++i) {
+    a.ks[i] = k_strides[i];
+    a.vs[i] = v_strides[i];
+  }
+  if ((rc = check_kv4_rows(a))) return rc;
+  return launched(attnres::kv4_append_launch(dtype, a, static_cast<cudaStream_t>(stream)), "attnres_kv4_append launch");
+}
+
+int attnres_kv4_read(const void* k_codes, const void* k_params, const void* v_codes, const void* v_params,
+                     int64_t num_pages, int kv_heads, int page_size, int head_dim, const int* page_table,
+                     int64_t page_table_stride, int max_pages, const int* start, const int* counts, int batch,
+                     int new_tokens, int dtype, void* k, void* v, void* stream) {
+  attnres::Kv4RowsArgs a{};
+  a.c = kv4_cache(k_codes, k_params, v_codes, v_params, num_pages, kv_heads, page_size, head_dim);
+  int rc = check_kv4(a.c, max_pages, page_table_stride, batch, new_tokens);
+  if (rc) return rc;
+  if (!known_dtype(dtype)) return fail(ATTNRES_ERR_INVALID_ARGUMENT, "unknown dtype %d", dtype);
+  if (batch == 0 || new_tokens == 0) return ATTNRES_OK;
+  if ((rc = check_kv4_buffers(a.c, page_table, max_pages, start))) return rc;
+  if (!k || !v) return fail(ATTNRES_ERR_INVALID_ARGUMENT, "kv4 read: k or v is NULL");
+  if (!aligned16(k) || !aligned16(v))
+    return fail(ATTNRES_ERR_UNSUPPORTED, "kv4 read: k and v must start on 16-byte boundaries");
+  a.table = page_table;
+  a.table_stride = page_table_stride;
+  a.max_pages = max_pages;
+  a.start = start;
+  a.counts = counts;
+  a.B = batch;
+  a.T = new_tokens;
+  a.k_out = k;
+  a.v_out = v;
+  if ((rc = check_kv4_rows(a))) return rc;
+  return launched(attnres::kv4_read_launch(dtype, a, static_cast<cudaStream_t>(stream)), "attnres_kv4_read launch");
+}
+
+size_t attnres_kv4_attention_workspace_bytes(int kv_heads, int page_size, int head_dim, int max_pages, int batch,
+                                             int new_tokens, int q_heads) {
+  if (kv_heads < 1 || page_size < 1 || head_dim < 1 || max_pages < 0 || batch < 1 || new_tokens < 1 || q_heads < kv_heads)
+    return 0;
+  attnres::Kv4AttnArgs a{};
+  a.c = kv4_cache(nullptr, nullptr, nullptr, nullptr, 0, kv_heads, page_size, head_dim);
+  a.max_pages = max_pages;
+  a.B = batch;
+  a.T = new_tokens;
+  a.Hq = q_heads;
+  return attnres::kv4_attention_workspace_bytes(a);
+}
+
+int attnres_kv4_attention(const void* k_codes, const void* k_params, const void* v_codes, const void* v_params,
+                          int64_t num_pages, int kv_heads, int page_size, int head_dim, const int* page_table,
+                          int64_t page_table_stride, int max_pages, const int* lengths, const int* counts, int batch,
+                          int new_tokens, int q_heads, int dtype, const void* q, const int64_t* q_strides, float scale,
+                          void* out, float* lse, void* workspace, size_t workspace_bytes, void* stream) {
+  attnres::Kv4AttnArgs a{};
+  a.c = kv4_cache(k_codes, k_params, v_codes, v_params, num_pages, kv_heads, page_size, head_dim);
+  int rc = check_kv4(a.c, max_pages, page_table_stride, batch, new_tokens);
+  if (rc) return rc;
+  if (!known_dtype(dtype)) return fail(ATTNRES_ERR_INVALID_ARGUMENT, "unknown dtype %d", dtype);
+  if (dtype == ATTNRES_DTYPE_F32) return fail(ATTNRES_ERR_UNSUPPORTED, "kv4 attention: float16 and bfloat16 only");
+  if (head_dim != 64 && head_dim != 128)
+    return fail(ATTNRES_ERR_UNSUPPORTED, "kv4 attention: head_dim=%d, 64 and 128 are built", head_dim);
+  if (q_heads < 1 || q_heads % kv_heads)
+    return fail(ATTNRES_ERR_INVALID_ARGUMENT, "kv4 attention: q_heads=%d must be a multiple of kv_heads=%d", q_heads,
+                kv_heads);
+  if (static_cast<double>(batch) * new_tokens * q_heads > 0x3fffffff)
+    return fail(ATTNRES_ERR_UNSUPPORTED, "kv4 attention: too many query rows for one launch");
+  if (batch == 0 || new_tokens == 0) return ATTNRES_OK;
+  if ((rc = check_kv4_buffers(a.c, page_table, max_pages, lengths))) return rc;
+  if (!q || !q_strides || !out) return fail(ATTNRES_ERR_INVALID_ARGUMENT, "kv4 attention: q or out is NULL");
+  if (!aligned16(out) || !aligned16(workspace))
+    return fail(ATTNRES_ERR_UNSUPPORTED, "kv4 attention: out and workspace must start on 16-byte boundaries");
+  a.table = page_table;
+  a.table_stride = page_table_stride;
+  a.max_pages = max_pages;
+  a.lengths = lengths;
+  a.counts = counts;
+  a.B = batch;
+  a.T = new_tokens;
+  a.Hq = q_heads;
+  a.q = q;
+  for (int i = 0; i < 3; ++i) a.qs[i] = q_strides[i];
+  a.scale = scale;
+  a.out = out;
+  a.lse = lse;
+  a.workspace = workspace;
+  const size_t need = attnres::kv4_attention_workspace_bytes(a);
+  if (need && (!workspace || workspace_bytes < need))
+    return fail(ATTNRES_ERR_WORKSPACE, "kv4 attention: workspace of %zu bytes, %zu needed", workspace_bytes, need);
+  return launched(attnres::kv4_attention_launch(dtype, a, static_cast<cudaStream_t>(stream)),
+                  "attnres_kv4_attention launch");
 }
 
 }  // extern "C"

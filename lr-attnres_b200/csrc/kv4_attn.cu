@@ -1,0 +1,599 @@
+// Attention of new query tokens over the 4-bit paged cache (format: kv4.h).
+//
+//   z_j = scale <q, k_j>, k_j = low_j + step_j n_j (a group of 32 elements at a time)
+//   out = sum_j softmax(z)_j v_j over the places j that the token may see
+// Token t of a sequence with `length` keys and `count` new tokens stands at place
+// length - count + t and sees the places up to its own. Query head h reads key head
+// h / (Hq / Hkv): the query heads of one key head, times the new tokens, are the rows
+// that share one pass over its keys. A row that sees nothing gives zeros.
+//
+// One pass with the running maximum and sum of the softmax. The products run on
+// mma.sync with the cache as the 16-row operand and the query rows as its 8 columns
+// (one token of one head fills one column: the tensor cores have time to spare, HBM has
+// not). A logic operation turns two codes into 16-bit floats: bits 0x4300 | n of bf16
+// are 128 + n; of f16, 0x6400 | n is 1024 + n and 0x5400 | n << 4 is 64 + n.
+//   scores  sum_d q_d (OFF + n_d) is exact up to fp32 sums that start at -sum_d q_d OFF;
+//           z = step * that + low Q, with Q the sum of the group's q
+//   output  values are f16 whatever q's type (step and low are): (OFF + n) - OFF is
+//           exact, step n + low is rounded once; weights, 0 to 1, are rounded to f16 too
+// The row of a key is an accumulator's row and a value's column: weights change sides
+// by movmatrix. Keys are taken in the order i ^ ((i >> 1) & 1) so that lanes that differ
+// in their keys read different halves of the banks.
+//
+// A value that some rows may not see must not reach them as 0 * NaN: in the 32 places
+// around a sequence's end, values that nobody sees count as zero, and so do those with
+// an infinity or NaN, which turn the rows that do see them into NaN through their sum.
+//
+// A CTA takes a stretch of places of one (sequence, key head, 8 NT query rows); its four
+// warps walk through it 32 places at a time, each with a ring of its own that bulk
+// copies fill (codes and params of 16 or 32 places are contiguous in a page). Sums of
+// the warps are joined in shared memory, those of the stretches by kv4_join_kernel.
+// Every mbarrier wait is bounded (~2 s, a status bit on timeout).
+#include <algorithm>
+
+#include "common.cuh"
+#include "kv4.h"
+#include "launch_cache.h"
+#include "mma.cuh"
+#include "tma.cuh"
+
+namespace attnres {
+
+static __device__ unsigned int g_kv4_attn_status = 0;
+
+constexpr int kAtWarps = 4;
+constexpr int kAtStages = 3;       // 32 places each, per warp
+constexpr int kAtKeys = 32;
+constexpr int kAtMaxStretch = 4096;
+constexpr float kLog2e = 1.4426950408889634f;
+
+struct AttnLaunch {
+  Kv4AttnArgs a;
+  int group, rows, row_tiles;  // query heads a key head; rows = T * group; tiles of 8 NT rows
+  int stretch, splits;         // places of a CTA, stretches of the longest possible sequence
+  float* part_o;               // [B, heads, row_tiles, splits, 8 NT, D]
+  float2* part_ml;             // [B, heads, row_tiles, splits, 8 NT]
+};
+
+// Code pair k of a word (bits 4 k and 16 + 4 k) as two 16-bit floats offset by kOff[k].
+template <typename T> struct Codes16;
+template <> struct Codes16<__nv_bfloat16> {
+  static __device__ __forceinline__ uint32_t pair(uint32_t w, int k) { return ((w >> (4 * k)) & 0x000f000fu) | 0x43004300u; }
+  static __device__ __forceinline__ uint32_t off(int) { return 0x43004300u; }  // 128, 128
+  static constexpr uint32_t kOnes = 0x3f803f80u;
+};
+template <> struct Codes16<__half> {
+  static __device__ __forceinline__ uint32_t pair(uint32_t w, int k) {
+    const uint32_t x = k >= 2 ? w >> 8 : w;
+    return (k & 1) ? (x & 0x00f000f0u) | 0x54005400u : (x & 0x000f000fu) | 0x64006400u;
+  }
+  static __device__ __forceinline__ uint32_t off(int k) { return (k & 1) ? 0x54005400u : 0x64006400u; }  // 64 or 1024
+  static constexpr uint32_t kOnes = 0x3c003c00u;
+};
+
+__device__ __forceinline__ uint32_t half_sub(uint32_t a, uint32_t b) {
+  const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t half_fma(uint32_t a, uint32_t b, uint32_t c) {
+  const __half2 r = __hfma2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b),
+                            *reinterpret_cast<const __half2*>(&c));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t half_pack(float a, float b) {
+  const __half2 r = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+// Whether either half of a pair of params is an infinity or NaN.
+__device__ __forceinline__ bool not_finite(uint32_t p) {
+  return (p & 0x7c00u) == 0x7c00u || (p & 0x7c000000u) == 0x7c000000u;
+}
+
+__device__ __forceinline__ uint32_t transposed(uint32_t x) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+  return r;
+}
+
+// G words at p, as one load where the size allows.
+template <int G>
+__device__ __forceinline__ void load_words(const unsigned char* p, uint32_t (&w)[G]) {
+  if constexpr (G == 4) {
+    const uint4 x = *reinterpret_cast<const uint4*>(p);
+    w[0] = x.x, w[1] = x.y, w[2] = x.z, w[3] = x.w;
+  } else if constexpr (G == 2) {
+    const uint2 x = *reinterpret_cast<const uint2*>(p);
+    w[0] = x.x, w[1] = x.y;
+  } else {
+    w[0] = *reinterpret_cast<const uint32_t*>(p);
+  }
+}
+
+// Sequence b's keys and new tokens: the length clipped to what its page table can hold.
+struct SeqFacts {
+  int length, count;
+};
+__device__ __forceinline__ SeqFacts seq_facts(const Kv4AttnArgs& a, int b) {
+  SeqFacts s;
+  const long long room = static_cast<long long>(a.max_pages) * a.c.page;
+  s.length = static_cast<int>(min(static_cast<long long>(max(a.lengths[b], 0)), room));
+  s.count = a.counts ? min(max(a.counts[b], 0), a.T) : a.T;
+  return s;
+}
+// The places that a token sees: 0 .. last (negative: none).
+__device__ __forceinline__ int last_place(const SeqFacts& s, int t) {
+  return t < s.count ? s.length - s.count + t : -1;
+}
+
+// Writes one finished row.
+template <typename T>
+__device__ __forceinline__ long long out_index(const AttnLaunch& L, int b, int h, int row) {
+  const int t = row / L.group, head = h * L.group + row - t * L.group;
+  return (static_cast<long long>(b) * L.a.T + t) * L.a.Hq + head;
+}
+
+template <typename T, int D, int NT>
+__global__ void __launch_bounds__(kAtWarps * 32, NT == 1 ? 3 : 2) kv4_attn_kernel(const __grid_constant__ AttnLaunch L) {
+  constexpr int G = D / kKv4Group, HALF = D / 2;
+  constexpr int kCode = kAtKeys * HALF, kParam = kAtKeys * G * 4;  // bytes of a stage
+  constexpr int kStage = 2 * (kCode + kParam);
+  constexpr int ROWS = 8 * NT;
+  const Kv4AttnArgs& a = L.a;
+  extern __shared__ __align__(128) unsigned char smem[];
+  __shared__ int pages[kAtMaxStretch / 16];
+  __shared__ uint64_t bars[kAtWarps][kAtStages];
+  __shared__ float warp_m[kAtWarps][ROWS], warp_l[kAtWarps][ROWS];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+  const int split = blockIdx.x % L.splits, tile = blockIdx.x / L.splits, h = blockIdx.y, b = blockIdx.z;
+  const SeqFacts seq = seq_facts(a, b);
+  const int from = split * L.stretch, to = min(from + L.stretch, seq.length);
+  if (from >= to && L.splits > 1) return;  // the join knows how many stretches there are
+
+  // pages of the stretch, 16 places at a time; -1 where the table has none
+  for (int i = threadIdx.x; i * 16 < to - from; i += kAtWarps * 32) {
+    const int at = from + i * 16, slot = at / a.c.page;
+    const int p = a.table[b * a.table_stride + slot];
+    const bool there = p >= 0 && p < a.c.pages;
+    if (!there) atomicOr(&g_kv4_attn_status, kStatusCacheRange);
+    pages[i] = there ? p : -1;
+  }
+  if (lane == 0)
+    for (int i = 0; i < kAtStages; ++i) mbar_init(&bars[warp][i], 1);
+  fence_mbar_init();
+  __syncthreads();
+
+  const int first = warp, count = (to - from + kAtKeys - 1) / kAtKeys;  // this warp's stages: first, first + 4, ...
+  unsigned char* ring = smem + warp * kAtStages * kStage;
+  const unsigned char* const src[4] = {static_cast<const unsigned char*>(a.c.k_codes),
+                                       static_cast<const unsigned char*>(a.c.k_params),
+                                       static_cast<const unsigned char*>(a.c.v_codes),
+                                       static_cast<const unsigned char*>(a.c.v_params)};
+  // Lane 0 posts the bytes of a stage, lanes 0 .. 7 copy: 16 places x {keys, key
+  // params, values, value params} each.
+  auto fetch = [&](int stage, int slot) {
+    const int at = stage * kAtKeys;  // from the stretch's start
+    uint32_t bytes = 0;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      if (at + 16 * i < to - from && pages[(at >> 4) + i] >= 0) bytes += kStage / 2;
+    if (lane == 0) {
+      if (bytes) mbar_arrive_expect_tx(&bars[warp][slot], bytes);
+      else mbar_arrive(&bars[warp][slot]);
+    }
+    __syncwarp();
+    const int i = lane >> 2, what = lane & 3;
+    if (lane < 8 && at + 16 * i < to - from) {
+      const int p = pages[(at >> 4) + i];
+      if (p >= 0) {
+        const uint32_t row = (what & 1) ? G * 4 : HALF;
+        const int place = (from + at + 16 * i) % a.c.page;
+        const long long where = ((static_cast<long long>(p) * a.c.heads + h) * a.c.page + place) * row;
+        unsigned char* dst = ring + slot * kStage + (what & 1 ? 2 * kCode + (what >> 1) * kParam : (what >> 1) * kCode);
+        bulk_g2s(dst + 16 * i * row, src[what] + where, 16 * row, &bars[warp][slot]);
+      }
+    }
+  };
+#pragma unroll
+  for (int i = 0; i < kAtStages; ++i)
+    if (first + i * kAtWarps < count) fetch(first + i * kAtWarps, i);
+
+  // the query rows as the second operand: column g of tile j is row 8 j + g
+  uint32_t qf[NT][G][4];
+  float qsum[NT][G][2], qoff[NT][G][2];  // of columns 2 c, 2 c + 1: sum q, -sum q OFF
+  int last[NT][2];  // of rows 8 j + 2 c, 2 c + 1
+#pragma unroll
+  for (int j = 0; j < NT; ++j) {
+    const int row = tile * ROWS + 8 * j + g;
+    const T* q = static_cast<const T*>(a.q);
+    const bool there = row < L.rows;
+    if (there) {
+      const int t = row / L.group, head = h * L.group + row - t * L.group;
+      q += b * a.qs[0] + t * a.qs[1] + head * a.qs[2];
+    }
+#pragma unroll
+    for (int i = 0; i < G; ++i) {
+      uint16_t e[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        e[k] = there ? reinterpret_cast<const uint16_t*>(q)[i * 32 + c * 8 + k] : static_cast<uint16_t>(0);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) qf[j][i][k] = e[k] | (static_cast<uint32_t>(e[k + 4]) << 16);
+      float s[4] = {}, f[4] = {};
+      const uint32_t one = Codes16<T>::kOnes, o0 = Codes16<T>::off(0), o1 = Codes16<T>::off(1);
+      mma_16816<T>(s, one, one, one, one, qf[j][i][0], qf[j][i][1]);
+      mma_16816<T>(s, one, one, one, one, qf[j][i][2], qf[j][i][3]);
+      mma_16816<T>(f, o0, o0, o1, o1, qf[j][i][0], qf[j][i][1]);
+      mma_16816<T>(f, o0, o0, o1, o1, qf[j][i][2], qf[j][i][3]);
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        qsum[j][i][e] = s[e];
+        qoff[j][i][e] = -f[e];
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int r = tile * ROWS + 8 * j + 2 * c + e;
+      last[j][e] = r < L.rows ? last_place(seq, r / L.group) : -1;
+    }
+  }
+  int least = 0x7fffffff;  // places up to this one are seen by all rows that see any
+#pragma unroll
+  for (int j = 0; j < NT; ++j)
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+      if (tile * ROWS + 8 * j + 2 * c + e < L.rows) least = min(least, last[j][e]);
+#pragma unroll
+  for (int o = 1; o < 4; o <<= 1) least = min(least, __shfl_xor_sync(0xffffffffu, least, o));
+
+  float o[NT][2 * G][4] = {}, m[NT][2], l[NT][2] = {};
+#pragma unroll
+  for (int j = 0; j < NT; ++j) m[j][0] = m[j][1] = -INFINITY;
+  const float zscale = a.scale * kLog2e;
+  const int swap = (g >> 1) & 1;          // keys in the order i ^ ((i >> 1) & 1)
+  bool ok = true;
+  int n = 0;
+  for (int stage = first; stage < count; stage += kAtWarps, ++n) {
+    const int slot = n % kAtStages;
+    ok = ok && mbar_wait_bounded(&bars[warp][slot], static_cast<uint32_t>((n / kAtStages) & 1));
+    if (!__all_sync(0xffffffffu, ok)) {
+      ok = false;
+      break;
+    }
+    const unsigned char* kc = ring + slot * kStage;
+    const unsigned char* vc = kc + kCode;
+    const unsigned char* kp = kc + 2 * kCode;
+    const unsigned char* vp = kp + kParam;
+    const int at = from + stage * kAtKeys;
+    const bool whole0 = pages[(stage * kAtKeys) >> 4] >= 0;
+    const bool whole1 = stage * kAtKeys + 16 < to - from && pages[((stage * kAtKeys) >> 4) + 1] >= 0;
+    // nothing masked: 32 places that every row sees
+    const bool open = whole0 && whole1 && at + kAtKeys <= to && at + kAtKeys - 1 <= least;
+
+    // ---- scores: accumulator row g (and g + 8) is a key, columns 2c, 2c + 1 rows
+    float z[2][NT][4];
+#pragma unroll
+    for (int mt = 0; mt < 2; ++mt) {
+      const int key0 = mt * 16 + (g ^ swap), key1 = key0 + 8;
+      uint32_t w0[G], w1[G], p0[G], p1[G];
+      load_words<G>(kc + key0 * HALF + c * 4 * G, w0);
+      load_words<G>(kc + key1 * HALF + c * 4 * G, w1);
+      load_words<G>(kp + key0 * 4 * G, p0);
+      load_words<G>(kp + key1 * 4 * G, p1);
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) z[mt][j][e] = 0.f;
+#pragma unroll
+      for (int i = 0; i < G; ++i) {
+        uint32_t f0[4], f1[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          f0[k] = Codes16<T>::pair(w0[i], k);
+          f1[k] = Codes16<T>::pair(w1[i], k);
+        }
+        const float2 s0 = __half22float2(*reinterpret_cast<const __half2*>(&p0[i]));
+        const float2 s1 = __half22float2(*reinterpret_cast<const __half2*>(&p1[i]));
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+          float acc[4] = {qoff[j][i][0], qoff[j][i][1], qoff[j][i][0], qoff[j][i][1]};
+          mma_16816<T>(acc, f0[0], f1[0], f0[1], f1[1], qf[j][i][0], qf[j][i][1]);
+          mma_16816<T>(acc, f0[2], f1[2], f0[3], f1[3], qf[j][i][2], qf[j][i][3]);
+          z[mt][j][0] = fmaf(s0.x, acc[0], fmaf(s0.y, qsum[j][i][0], z[mt][j][0]));
+          z[mt][j][1] = fmaf(s0.x, acc[1], fmaf(s0.y, qsum[j][i][1], z[mt][j][1]));
+          z[mt][j][2] = fmaf(s1.x, acc[2], fmaf(s1.y, qsum[j][i][0], z[mt][j][2]));
+          z[mt][j][3] = fmaf(s1.x, acc[3], fmaf(s1.y, qsum[j][i][1], z[mt][j][3]));
+        }
+      }
+      const bool whole = mt ? whole1 : whole0;
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          z[mt][j][e] *= zscale;
+          if (!open) {
+            const int place = at + (e < 2 ? key0 : key1);
+            if (!whole || place >= to || place > last[j][e & 1]) z[mt][j][e] = -INFINITY;
+          }
+        }
+    }
+
+    // ---- running maximum; the sums o and l follow it
+    bool grew = false;
+    float shrink[NT][2];
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float x = fmaxf(fmaxf(z[0][j][e], z[0][j][2 + e]), fmaxf(z[1][j][e], z[1][j][2 + e]));
+#pragma unroll
+        for (int s = 4; s < 32; s <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, s));
+        const float mine = fmaxf(m[j][e], x);
+        grew |= mine > m[j][e];
+        shrink[j][e] = m[j][e] == mine ? 1.f : exp2f(m[j][e] - mine);
+        m[j][e] = mine;
+      }
+    if (__any_sync(0xffffffffu, grew)) {
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+#pragma unroll
+        for (int i = 0; i < 2 * G; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[j][i][e] *= shrink[j][e & 1];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) l[j][e] *= shrink[j][e];
+      }
+    }
+#pragma unroll
+    for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float top = m[j][e & 1] == -INFINITY ? 0.f : m[j][e & 1];
+          z[mt][j][e] = exp2f(z[mt][j][e] - top);
+          l[j][e & 1] += z[mt][j][e];
+        }
+
+    // ---- output: accumulator rows are elements of the value, columns query rows
+#pragma unroll
+    for (int mt = 0; mt < 2; ++mt) {
+      uint32_t words[4][(G + 1) / 2], par[4][G];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {  // MMA columns 2c, 2c + 1, 2c + 8, 2c + 9
+        const int i = 2 * c + (k & 1), key = mt * 16 + (i ^ ((i >> 1) & 1)) + (k >> 1) * 8;
+        load_words<(G + 1) / 2>(vc + key * HALF + g * 2 * G, words[k]);
+        load_words<G>(vp + key * 4 * G, par[k]);
+        if (!open) {
+          const bool there = (mt ? whole1 : whole0) && at + key < to;
+#pragma unroll
+          for (int i2 = 0; i2 < G; ++i2)
+            if (!there || not_finite(par[k][i2])) par[k][i2] = 0;
+        }
+      }
+      if (!open) {
+        const int key0 = mt * 16 + (g ^ swap);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          uint32_t mine[G];
+          load_words<G>(vp + (key0 + 8 * e) * 4 * G, mine);
+          bool odd = false;
+#pragma unroll
+          for (int i = 0; i < G; ++i) odd |= not_finite(mine[i]);
+#pragma unroll
+          for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int r = 0; r < 2; ++r)
+              if (odd && z[mt][j][2 * e + r] > 0.f) l[j][r] = __int_as_float(0x7fffffff);
+        }
+      }
+      uint32_t pa[NT], pb[NT];
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        pa[j] = transposed(half_pack(z[mt][j][0], z[mt][j][1]));
+        pb[j] = transposed(half_pack(z[mt][j][2], z[mt][j][3]));
+      }
+#pragma unroll
+      for (int i = 0; i < G; ++i) {
+        const uint32_t pick = (i & 1) ? 0x7632u : 0x5410u;
+        uint32_t f[2][4];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {  // the pairs of keys 2c, 2c + 1 and 2c + 8, 2c + 9
+          const uint32_t w = __byte_perm(words[2 * e][i >> 1], words[2 * e + 1][i >> 1], pick);
+          const uint32_t step = __byte_perm(par[2 * e][i], par[2 * e + 1][i], 0x5410u);
+          const uint32_t low = __byte_perm(par[2 * e][i], par[2 * e + 1][i], 0x7632u);
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            f[e][k] = half_fma(half_sub(Codes16<__half>::pair(w, k), Codes16<__half>::off(k)), step, low);
+        }
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+          mma_16816<__half>(o[j][2 * i], f[0][0], f[0][1], f[1][0], f[1][1], pa[j], pb[j]);
+          mma_16816<__half>(o[j][2 * i + 1], f[0][2], f[0][3], f[1][2], f[1][3], pa[j], pb[j]);
+        }
+      }
+    }
+    __syncwarp();  // every lane has read the stage
+    if (stage + kAtStages * kAtWarps < count) fetch(stage + kAtStages * kAtWarps, slot);
+  }
+  if (!ok) {
+    if (lane == 0) atomicOr(&g_kv4_attn_status, kStatusFullWaitTimeout);
+    // copies still in flight land before the CTA's shared memory is given away
+    for (int i = 0; i < kAtStages; ++i, ++n)
+      if (first + n * kAtWarps < count &&
+          !mbar_wait_bounded(&bars[warp][n % kAtStages], static_cast<uint32_t>((n / kAtStages) & 1)) && lane == 0)
+        atomicOr(&g_kv4_attn_status, kStatusDrainTimeout);
+  }
+
+  // ---- join the warps: l over the lanes of a column first
+#pragma unroll
+  for (int j = 0; j < NT; ++j) {
+#pragma unroll
+    for (int s = 4; s < 32; s <<= 1) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) l[j][e] += __shfl_xor_sync(0xffffffffu, l[j][e], s);
+    }
+    if (g == 0) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        warp_m[warp][8 * j + 2 * c + e] = m[j][e];
+        warp_l[warp][8 * j + 2 * c + e] = l[j][e];
+      }
+    }
+  }
+  __syncthreads();  // every warp is done with its ring
+  float* sums = reinterpret_cast<float*>(smem);  // [warps][ROWS][D + 4]
+  constexpr int PITCH = D + 4;
+#pragma unroll
+  for (int j = 0; j < NT; ++j)
+#pragma unroll
+    for (int i = 0; i < 2 * G; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        // element 32 (i / 2) + 4 g + 2 (i & 1) + (e / 2) of row 8 j + 2 c + (e & 1)
+        const int element = 32 * (i >> 1) + 4 * g + 2 * (i & 1) + (e >> 1);
+        sums[(warp * ROWS + 8 * j + 2 * c + (e & 1)) * PITCH + element] = o[j][i][e];
+      }
+  __syncthreads();
+  const long long unit = ((static_cast<long long>(b) * a.c.heads + h) * L.row_tiles + tile) * L.splits + split;
+  for (int i = threadIdx.x; i < ROWS * D; i += kAtWarps * 32) {
+    const int r = i / D, d = i - r * D, row = tile * ROWS + r;
+    if (row >= L.rows) break;
+    float top = warp_m[0][r];
+#pragma unroll
+    for (int w = 1; w < kAtWarps; ++w) top = fmaxf(top, warp_m[w][r]);
+    float total = 0.f, y = 0.f;
+#pragma unroll
+    for (int w = 0; w < kAtWarps; ++w) {
+      const float f = warp_m[w][r] == -INFINITY ? 0.f : exp2f(warp_m[w][r] - top);
+      total += f * warp_l[w][r];
+      y += f * sums[(w * ROWS + r) * PITCH + d];
+    }
+    if (L.splits == 1) {
+      const long long to_row = out_index<T>(L, b, h, row);
+      static_cast<T*>(a.out)[to_row * D + d] = Elem<T>::from_f(top == -INFINITY ? 0.f : y / total);
+      if (a.lse && d == 0) a.lse[to_row] = top == -INFINITY ? -INFINITY : (top + log2f(total)) / kLog2e;
+    } else {
+      L.part_o[(unit * ROWS + r) * D + d] = y;
+      if (d == 0) L.part_ml[unit * ROWS + r] = make_float2(top, total);
+    }
+  }
+}
+
+// One warp a row: adds the stretches of its sequence in order.
+template <typename T, int D>
+__global__ void __launch_bounds__(128) kv4_join_kernel(const __grid_constant__ AttnLaunch L, int tile_rows) {
+  const Kv4AttnArgs& a = L.a;
+  const long long index = static_cast<long long>(blockIdx.x) * 4 + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  if (index >= static_cast<long long>(a.B) * a.c.heads * L.rows) return;
+  const int row = static_cast<int>(index % L.rows);
+  const long long bh = index / L.rows;
+  const int h = static_cast<int>(bh % a.c.heads), b = static_cast<int>(bh / a.c.heads);
+  const SeqFacts seq = seq_facts(a, b);
+  const int n = (seq.length + L.stretch - 1) / L.stretch;
+  const long long unit = (bh * L.row_tiles + row / tile_rows) * L.splits;
+  const int r = row % tile_rows;
+  float top = -INFINITY;
+  for (int s = lane; s < n; s += 32) top = fmaxf(top, L.part_ml[(unit + s) * tile_rows + r].x);
+  top = warp_max(top);
+  constexpr int VEC = D / 32;
+  float y[VEC] = {}, total = 0.f;
+  if (top != -INFINITY) {
+    for (int s = 0; s < n; ++s) {
+      const float2 ml = L.part_ml[(unit + s) * tile_rows + r];
+      const float f = ml.x == -INFINITY ? 0.f : exp2f(ml.x - top);
+      total += f * ml.y;
+      const Pack<float, VEC> p = load_pack<float, VEC>(L.part_o + ((unit + s) * tile_rows + r) * D + lane * VEC);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) y[e] += f * p.e[e];
+    }
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) y[e] /= total;
+  }
+  const long long to_row = out_index<T>(L, b, h, row);
+  store_pack<T, VEC>(static_cast<T*>(a.out) + to_row * D + lane * VEC, y);
+  if (a.lse && lane == 0) a.lse[to_row] = top == -INFINITY ? -INFINITY : (top + log2f(total)) / kLog2e;
+}
+
+namespace {
+
+int tiles_of_rows(int rows) { return rows <= 8 ? 1 : 2; }  // NT
+
+int stage_bytes(int D) { return 2 * kAtKeys * (D / 2 + D / kKv4Group * 4); }
+
+size_t attn_smem(int D, int NT) {
+  const size_t ring = static_cast<size_t>(kAtWarps) * kAtStages * stage_bytes(D);
+  const size_t sums = static_cast<size_t>(kAtWarps) * 8 * NT * (D + 4) * sizeof(float);
+  return std::max(ring, sums);
+}
+
+// Stretches: about four CTAs for every one that fits on the GPU, so that ragged
+// lengths even out, of at least 128 places (one stage a warp).
+AttnLaunch plan(const Kv4AttnArgs& a) {
+  AttnLaunch L{};
+  L.a = a;
+  L.group = a.Hq / a.c.heads;
+  L.rows = a.T * L.group;
+  const int NT = tiles_of_rows(L.rows);
+  L.row_tiles = (L.rows + 8 * NT - 1) / (8 * NT);
+  int nsm = 0;
+  if (cached_sm_count(&nsm) != cudaSuccess) nsm = 148;
+  const long long room = std::max(1LL, static_cast<long long>(a.max_pages) * a.c.page);
+  const long long all = room * a.B * a.c.heads * L.row_tiles;
+  const long long wish = all / (4LL * nsm * 3) + 1;
+  long long stretch = (std::min<long long>(wish, room) + 127) / 128 * 128;
+  stretch = std::min<long long>(std::max<long long>(stretch, 128), kAtMaxStretch);
+  L.stretch = static_cast<int>(stretch);
+  L.splits = static_cast<int>((room + stretch - 1) / stretch);
+  return L;
+}
+
+size_t parts(const AttnLaunch& L) {
+  const int NT = tiles_of_rows(L.rows);
+  return static_cast<size_t>(L.a.B) * L.a.c.heads * L.row_tiles * L.splits * 8 * NT;
+}
+
+template <typename T, int D, int NT>
+cudaError_t attn_t(const AttnLaunch& L, cudaStream_t st) {
+  const void* fn = reinterpret_cast<const void*>(&kv4_attn_kernel<T, D, NT>);
+  const size_t smem = attn_smem(D, NT);
+  cudaError_t e = ensure_dynamic_smem(fn, static_cast<int>(smem));
+  if (e != cudaSuccess) return e;
+  const dim3 grid(static_cast<unsigned>(L.splits) * L.row_tiles, L.a.c.heads, L.a.B);
+  kv4_attn_kernel<T, D, NT><<<grid, kAtWarps * 32, smem, st>>>(L);
+  if ((e = cudaGetLastError()) != cudaSuccess || L.splits == 1) return e;
+  const long long rows = static_cast<long long>(L.a.B) * L.a.c.heads * L.rows;
+  kv4_join_kernel<T, D><<<static_cast<unsigned>((rows + 3) / 4), 128, 0, st>>>(L, 8 * NT);
+  return cudaGetLastError();
+}
+
+template <typename T>
+cudaError_t attn_dt(const AttnLaunch& L, cudaStream_t st) {
+  const int NT = tiles_of_rows(L.rows);
+  if (L.a.c.D == 64) return NT == 1 ? attn_t<T, 64, 1>(L, st) : attn_t<T, 64, 2>(L, st);
+  return NT == 1 ? attn_t<T, 128, 1>(L, st) : attn_t<T, 128, 2>(L, st);
+}
+
+}  // namespace
+
+size_t kv4_attention_workspace_bytes(const Kv4AttnArgs& a) {
+  const AttnLaunch L = plan(a);
+  if (L.splits == 1) return 0;
+  return parts(L) * (a.c.D + 2) * sizeof(float);
+}
+
+cudaError_t kv4_attention_launch(int dtype, const Kv4AttnArgs& a, cudaStream_t st) {
+  AttnLaunch L = plan(a);
+  L.part_o = static_cast<float*>(a.workspace);
+  L.part_ml = reinterpret_cast<float2*>(L.part_o + parts(L) * a.c.D);
+  return dtype == ATTNRES_DTYPE_BF16 ? attn_dt<__nv_bfloat16>(L, st) : attn_dt<__half>(L, st);
+}
+
+cudaError_t read_kv4_attn_status(unsigned* status, bool reset) {
+  cudaError_t e = cudaMemcpyFromSymbol(status, g_kv4_attn_status, sizeof(unsigned));
+  if (e != cudaSuccess || !reset) return e;
+  const unsigned zero = 0;
+  return cudaMemcpyToSymbol(g_kv4_attn_status, &zero, sizeof(unsigned));
+}
+
+}  // namespace attnres

@@ -332,9 +332,132 @@ py::tuple py_swiglu_backward(const Tensor& grad_h, const Tensor& x, const Tensor
   return py::make_tuple(d[0], d[1]);
 }
 
+// ---------------------------------------------------------------------------
+// 4-bit cache
+// ---------------------------------------------------------------------------
+struct PoolCall {
+  Tensor kc, kp, vc, vp, table, per_sequence, counts;
+  int64_t pages, heads, page, D, B, max_pages;
+
+  PoolCall(const char* what, const Tensor& kc_, const Tensor& kp_, const Tensor& vc_, const Tensor& vp_,
+           const Tensor& table_, const Tensor& per_, const OptTensor& counts_)
+      : kc(kc_), kp(kp_), vc(vc_), vp(vp_), table(table_), per_sequence(per_), counts(or_undefined(counts_)) {
+    check_cuda(what, kc);
+    for (const Tensor* t : {&kp, &vc, &vp, &table, &per_sequence, &counts}) check_device(what, kc, *t);
+    TORCH_CHECK(kc.dim() == 4 && kc.scalar_type() == at::kByte, "attnres_b200: ", what,
+                " takes codes uint8 [pages, kv_heads, page_size, head_dim / 2]");
+    pages = kc.size(0);
+    heads = kc.size(1);
+    page = kc.size(2);
+    D = 2 * kc.size(3);
+    TORCH_CHECK(page > 0 && page % 16 == 0 && D > 0 && D % 32 == 0 && D <= 512 && heads > 0, "attnres_b200: ", what,
+                " takes a page_size that is a multiple of 16 and a head_dim that is a multiple of 32 up to 512, got ", page,
+                " and ", D);
+    TORCH_CHECK(vc.sizes() == kc.sizes() && vc.scalar_type() == at::kByte, "attnres_b200: ", what,
+                " takes key and value codes of one shape");
+    for (const Tensor* p : {&kp, &vp})
+      TORCH_CHECK(p->scalar_type() == at::kHalf && p->dim() == 5 && p->size(0) == pages && p->size(1) == heads &&
+                      p->size(2) == page && p->size(3) == D / 32 && p->size(4) == 2,
+                  "attnres_b200: ", what, " takes params float16 [pages, kv_heads, page_size, head_dim / 32, 2]");
+    for (const Tensor* p : {&kc, &kp, &vc, &vp})
+      TORCH_CHECK(p->is_contiguous() && reinterpret_cast<uintptr_t>(p->const_data_ptr()) % 16 == 0, "attnres_b200: ", what,
+                  " takes contiguous, 16-byte aligned pool tensors");
+    TORCH_CHECK(table.dim() == 2 && table.scalar_type() == at::kInt, "attnres_b200: ", what,
+                " takes page_table int32 [batch, max_pages]");
+    B = table.size(0);
+    max_pages = table.size(1);
+    TORCH_CHECK(per_sequence.dim() == 1 && per_sequence.size(0) == B && per_sequence.scalar_type() == at::kInt,
+                "attnres_b200: ", what, " takes start or lengths int32 [batch]");
+    TORCH_CHECK(!counts.defined() || (counts.dim() == 1 && counts.size(0) == B && counts.scalar_type() == at::kInt),
+                "attnres_b200: ", what, " takes counts int32 [batch]");
+    if (!table.is_contiguous()) table = table.contiguous();
+    if (!per_sequence.is_contiguous()) per_sequence = per_sequence.contiguous();
+    if (counts.defined() && !counts.is_contiguous()) counts = counts.contiguous();
+  }
+  const int* ints(const Tensor& t) const { return static_cast<const int*>(ptr(t)); }
+};
+
+// A [B, T, heads, D] tensor with a dense last dim; its strides.
+Tensor rows4(const char* what, const char* name, const Tensor& t, int64_t B, int64_t heads, int64_t D, int64_t (&strides)[3]) {
+  TORCH_CHECK(t.dim() == 4 && t.size(0) == B && t.size(2) == heads && t.size(3) == D, "attnres_b200: ", what, " takes ",
+              name, " [", B, ", tokens, ", heads, ", ", D, "], got ", t.sizes());
+  const Tensor r = t.stride(3) == 1 ? t : t.contiguous();
+  for (int i = 0; i < 3; ++i) strides[i] = r.stride(i);
+  return r;
+}
+
+void no_gradient(const char* what, std::initializer_list<const Tensor*> ts) {
+  TORCH_CHECK(!wants_grad(ts), "attnres_b200: ", what, " has no gradient; call it under torch.no_grad() or detach its inputs");
+}
+
+void py_kv4_append(const Tensor& kc, const Tensor& kp, const Tensor& vc, const Tensor& vp, const Tensor& k, const Tensor& v,
+                   const Tensor& table, const Tensor& start, const OptTensor& counts) {
+  const char* what = "kv4_append";
+  const PoolCall c(what, kc, kp, vc, vp, table, start, counts);
+  check_device(what, kc, k);
+  check_device(what, kc, v);
+  no_gradient(what, {&k, &v});
+  int64_t ks[3], vs[3];
+  const Tensor kr = rows4(what, "k", k, c.B, c.heads, c.D, ks), vr = rows4(what, "v", v, c.B, c.heads, c.D, vs);
+  TORCH_CHECK(kr.size(1) == vr.size(1) && kr.scalar_type() == vr.scalar_type(),
+              "attnres_b200: kv4_append takes k and v of one shape and type");
+  const Launch on(kc);
+  check_status(attnres_kv4_append(mut(kc), mut(kp), mut(vc), mut(vp), c.pages, c.heads, c.page, c.D, c.ints(c.table),
+                                  c.max_pages, c.max_pages, c.ints(c.per_sequence), c.ints(c.counts), c.B, kr.size(1),
+                                  dtype_code(kr), ptr(kr), ks, ptr(vr), vs, on.stream),
+               "attnres_kv4_append");
+}
+
+py::tuple py_kv4_read(const Tensor& kc, const Tensor& kp, const Tensor& vc, const Tensor& vp, const Tensor& table,
+                      const Tensor& start, int64_t tokens, const OptTensor& counts, at::ScalarType dtype) {
+  const PoolCall c("kv4_read", kc, kp, vc, vp, table, start, counts);
+  TORCH_CHECK(tokens >= 0 && tokens < (1 << 30), "attnres_b200: kv4_read takes a number of tokens, got ", tokens);
+  const Tensor k = at::empty({c.B, tokens, c.heads, c.D}, kc.options().dtype(dtype));
+  const Tensor v = at::empty({c.B, tokens, c.heads, c.D}, kc.options().dtype(dtype));
+  const Launch on(kc);
+  check_status(attnres_kv4_read(ptr(kc), ptr(kp), ptr(vc), ptr(vp), c.pages, c.heads, c.page, c.D, c.ints(c.table),
+                                c.max_pages, c.max_pages, c.ints(c.per_sequence), c.ints(c.counts), c.B, tokens,
+                                dtype_code(k), mut(k), mut(v), on.stream),
+               "attnres_kv4_read");
+  return py::make_tuple(k, v);
+}
+
+py::tuple py_kv4_attention(const Tensor& q, const Tensor& kc, const Tensor& kp, const Tensor& vc, const Tensor& vp,
+                           const Tensor& table, const Tensor& lengths, const OptTensor& counts, double scale,
+                           bool want_lse) {
+  const char* what = "kv4_attention";
+  const PoolCall c(what, kc, kp, vc, vp, table, lengths, counts);
+  check_device(what, kc, q);
+  no_gradient(what, {&q});
+  TORCH_CHECK(q.dim() == 4 && q.size(2) > 0 && q.size(2) % c.heads == 0, "attnres_b200: kv4_attention takes q [", c.B,
+              ", tokens, a multiple of ", c.heads, " heads, ", c.D, "], got ", q.sizes());
+  TORCH_CHECK(q.scalar_type() == at::kHalf || q.scalar_type() == at::kBFloat16,
+              "attnres_b200: kv4_attention takes float16 or bfloat16 queries, got ", q.scalar_type());
+  TORCH_CHECK(c.D == 64 || c.D == 128, "attnres_b200: kv4_attention is built for head_dim 64 and 128, got ", c.D);
+  const int64_t T = q.size(1), Hq = q.size(2);
+  int64_t qs[3];
+  const Tensor qr = rows4(what, "q", q, c.B, Hq, c.D, qs);
+  const Tensor out = at::empty({c.B, T, Hq, c.D}, q.options());
+  Tensor lse, workspace;
+  if (want_lse) lse = at::empty({c.B, T, Hq}, q.options().dtype(at::kFloat));
+  const Launch on(kc);
+  const int64_t bytes =
+      c.B && T ? attnres_kv4_attention_workspace_bytes(c.heads, c.page, c.D, c.max_pages, c.B, T, Hq) : 0;
+  if (bytes) workspace = at::empty({bytes}, kc.options());
+  check_status(attnres_kv4_attention(ptr(kc), ptr(kp), ptr(vc), ptr(vp), c.pages, c.heads, c.page, c.D, c.ints(c.table),
+                                     c.max_pages, c.max_pages, c.ints(c.per_sequence), c.ints(c.counts), c.B, T, Hq,
+                                     dtype_code(qr), ptr(qr), qs, scale, mut(out), static_cast<float*>(mut(lse)),
+                                     mut(workspace), bytes, on.stream),
+               "attnres_kv4_attention");
+  return py::make_tuple(out, lse);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_layer, m) {
+  m.def("kv4_append", &py_kv4_append);
+  m.def("kv4_read", &py_kv4_read);
+  m.def("kv4_attention", &py_kv4_attention);
   m.def("swiglu_projection", &py_swiglu);
   m.def("swiglu_projection_backward", &py_swiglu_backward);
   m.def("qk_norm_rope", &py_qk_norm_rope);

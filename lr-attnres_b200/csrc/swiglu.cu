@@ -27,6 +27,7 @@
 
 #include "common.cuh"
 #include "launch_cache.h"
+#include "mma.cuh"
 #include "swiglu.h"
 #include "tma.cuh"
 #include "umma.cuh"
@@ -302,21 +303,6 @@ __global__ void __launch_bounds__(kGmThreads, 1) swiglu_gemm_kernel(const __grid
 // agree. Bound by reading W once; the tensor cores of this kernel idle most of the
 // time, so the older instruction, whose operands come from registers, suffices.
 constexpr int kFewWarps = 8;
-
-template <typename T>
-__device__ __forceinline__ void mma_16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
-                                          uint32_t b0, uint32_t b1) {
-  if constexpr (std::is_same<T, __half>::value)
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-  else
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
 
 struct FewArgs {
   const void *x, *w;

@@ -10,12 +10,14 @@
 
 namespace attnres {
 
-// Bit flags written (atomicOr) by a kernel that gave up waiting. Read and
+// Bit flags written (atomicOr) by a kernel that gave up waiting or was given a
+// page table that does not cover what it was asked for. Read and
 // reset from the host with attnres_device_status().
 enum DeviceStatusBits : unsigned {
   kStatusFullWaitTimeout = 1u,   // consumers waited > kWaitLimitNs for a stage to land
   kStatusEmptyWaitTimeout = 2u,  // producer waited > kWaitLimitNs for a stage to drain
   kStatusDrainTimeout = 4u,      // producer gave up waiting for its own copies on exit
+  kStatusCacheRange = 8u,        // a cache position without a page: not written, read as empty
 };
 
 constexpr unsigned long long kWaitLimitNs = 2000000000ull;  // 2 s
