@@ -114,6 +114,8 @@ int check_kv4(const attnres::Kv4Cache& c, int max_pages, int64_t table_stride, i
     return fail(ATTNRES_ERR_UNSUPPORTED, "kv4 cache: batch=%d and kv_heads=%d up to 65535", batch, c.heads);
   if (static_cast<int64_t>(max_pages) * c.page > (1LL << 30))
     return fail(ATTNRES_ERR_UNSUPPORTED, "kv4 cache: a sequence of %d pages of %d places is too long", max_pages, c.page);
+  if (static_cast<double>(c.pages) * c.heads * (c.page / 16) > 0x7fffffff)
+    return fail(ATTNRES_ERR_UNSUPPORTED, "kv4 cache: a pool of %lld pages is too large", c.pages);
   if (table_stride < max_pages && batch > 1)
     return fail(ATTNRES_ERR_INVALID_ARGUMENT, "kv4 cache: page_table_stride below max_pages");
   return ATTNRES_OK;

@@ -46,6 +46,10 @@ constexpr int kAtStages = 3;       // 32 places each, per warp
 constexpr int kAtKeys = 32;
 constexpr int kAtMaxStretch = 4096;
 constexpr float kLog2e = 1.4426950408889634f;
+// The running maximum is raised only when a score passes it by this much (in powers of
+// two): weights then reach 2^kSlack, far from f16's 2^16, and almost every step goes
+// without the shuffles and the rescaling.
+constexpr float kSlack = 8.f;
 
 struct AttnLaunch {
   Kv4AttnArgs a;
@@ -95,6 +99,12 @@ __device__ __forceinline__ uint32_t transposed(uint32_t x) {
   return r;
 }
 
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 // G words at p, as one load where the size allows.
 template <int G>
 __device__ __forceinline__ void load_words(const unsigned char* p, uint32_t (&w)[G]) {
@@ -140,7 +150,7 @@ __global__ void __launch_bounds__(kAtWarps * 32, NT == 1 ? 3 : 2) kv4_attn_kerne
   constexpr int ROWS = 8 * NT;
   const Kv4AttnArgs& a = L.a;
   extern __shared__ __align__(128) unsigned char smem[];
-  __shared__ int pages[kAtMaxStretch / 16];
+  __shared__ int rows16[kAtMaxStretch / 16];  // row of the pool / 16 of each 16 places, -1 where there is no page
   __shared__ uint64_t bars[kAtWarps][kAtStages];
   __shared__ float warp_m[kAtWarps][ROWS], warp_l[kAtWarps][ROWS];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
@@ -149,13 +159,13 @@ __global__ void __launch_bounds__(kAtWarps * 32, NT == 1 ? 3 : 2) kv4_attn_kerne
   const int from = split * L.stretch, to = min(from + L.stretch, seq.length);
   if (from >= to && L.splits > 1) return;  // the join knows how many stretches there are
 
-  // pages of the stretch, 16 places at a time; -1 where the table has none
   for (int i = threadIdx.x; i * 16 < to - from; i += kAtWarps * 32) {
     const int at = from + i * 16, slot = at / a.c.page;
     const int p = a.table[b * a.table_stride + slot];
     const bool there = p >= 0 && p < a.c.pages;
     if (!there) atomicOr(&g_kv4_attn_status, kStatusCacheRange);
-    pages[i] = there ? p : -1;
+    const int place16 = (at - slot * a.c.page) >> 4;
+    rows16[i] = there ? static_cast<int>((static_cast<long long>(p) * a.c.heads + h) * (a.c.page >> 4)) + place16 : -1;
   }
   if (lane == 0)
     for (int i = 0; i < kAtStages; ++i) mbar_init(&bars[warp][i], 1);
@@ -164,34 +174,24 @@ __global__ void __launch_bounds__(kAtWarps * 32, NT == 1 ? 3 : 2) kv4_attn_kerne
 
   const int first = warp, count = (to - from + kAtKeys - 1) / kAtKeys;  // this warp's stages: first, first + 4, ...
   unsigned char* ring = smem + warp * kAtStages * kStage;
-  const unsigned char* const src[4] = {static_cast<const unsigned char*>(a.c.k_codes),
-                                       static_cast<const unsigned char*>(a.c.k_params),
-                                       static_cast<const unsigned char*>(a.c.v_codes),
-                                       static_cast<const unsigned char*>(a.c.v_params)};
-  // Lane 0 posts the bytes of a stage, lanes 0 .. 7 copy: 16 places x {keys, key
-  // params, values, value params} each.
+  // Lanes 0 .. 7 copy 16 places each: lane & 3 is keys, key params, values, value params.
+  const unsigned char* const my_src = static_cast<const unsigned char*>(
+      (lane & 2) ? ((lane & 1) ? a.c.v_params : a.c.v_codes) : ((lane & 1) ? a.c.k_params : a.c.k_codes));
+  const uint32_t my_bytes = 16 * ((lane & 1) ? G * 4 : HALF);
+  unsigned char* const my_dst = ring + ((lane & 1) ? 2 * kCode + ((lane >> 1) & 1) * kParam : ((lane >> 1) & 1) * kCode) +
+                                ((lane >> 2) & 1) * my_bytes;
   auto fetch = [&](int stage, int slot) {
-    const int at = stage * kAtKeys;  // from the stretch's start
-    uint32_t bytes = 0;
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-      if (at + 16 * i < to - from && pages[(at >> 4) + i] >= 0) bytes += kStage / 2;
+    const int i = 2 * stage;
+    const int r0 = rows16[i], r1 = (i + 1) * 16 < to - from ? rows16[i + 1] : -1;
     if (lane == 0) {
+      const uint32_t bytes = (r0 >= 0 ? kStage / 2 : 0) + (r1 >= 0 ? kStage / 2 : 0);
       if (bytes) mbar_arrive_expect_tx(&bars[warp][slot], bytes);
       else mbar_arrive(&bars[warp][slot]);
     }
     __syncwarp();
-    const int i = lane >> 2, what = lane & 3;
-    if (lane < 8 && at + 16 * i < to - from) {
-      const int p = pages[(at >> 4) + i];
-      if (p >= 0) {
-        const uint32_t row = (what & 1) ? G * 4 : HALF;
-        const int place = (from + at + 16 * i) % a.c.page;
-        const long long where = ((static_cast<long long>(p) * a.c.heads + h) * a.c.page + place) * row;
-        unsigned char* dst = ring + slot * kStage + (what & 1 ? 2 * kCode + (what >> 1) * kParam : (what >> 1) * kCode);
-        bulk_g2s(dst + 16 * i * row, src[what] + where, 16 * row, &bars[warp][slot]);
-      }
-    }
+    const int r = lane < 4 ? r0 : r1;
+    if (lane < 8 && r >= 0)
+      bulk_g2s(my_dst + slot * kStage, my_src + static_cast<long long>(r) * my_bytes, my_bytes, &bars[warp][slot]);
   };
 #pragma unroll
   for (int i = 0; i < kAtStages; ++i)
@@ -251,10 +251,10 @@ __global__ void __launch_bounds__(kAtWarps * 32, NT == 1 ? 3 : 2) kv4_attn_kerne
   const float zscale = a.scale * kLog2e;
   const int swap = (g >> 1) & 1;          // keys in the order i ^ ((i >> 1) & 1)
   bool ok = true;
-  int n = 0;
+  int slot = 0, n = 0;
+  uint32_t phase = 0;
   for (int stage = first; stage < count; stage += kAtWarps, ++n) {
-    const int slot = n % kAtStages;
-    ok = ok && mbar_wait_bounded(&bars[warp][slot], static_cast<uint32_t>((n / kAtStages) & 1));
+    ok = mbar_wait_bounded(&bars[warp][slot], phase);
     if (!__all_sync(0xffffffffu, ok)) {
       ok = false;
       break;
@@ -264,10 +264,9 @@ __global__ void __launch_bounds__(kAtWarps * 32, NT == 1 ? 3 : 2) kv4_attn_kerne
     const unsigned char* kp = kc + 2 * kCode;
     const unsigned char* vp = kp + kParam;
     const int at = from + stage * kAtKeys;
-    const bool whole0 = pages[(stage * kAtKeys) >> 4] >= 0;
-    const bool whole1 = stage * kAtKeys + 16 < to - from && pages[((stage * kAtKeys) >> 4) + 1] >= 0;
-    // nothing masked: 32 places that every row sees
-    const bool open = whole0 && whole1 && at + kAtKeys <= to && at + kAtKeys - 1 <= least;
+    const bool whole0 = rows16[2 * stage] >= 0, whole1 = at + 16 < to && rows16[2 * stage + 1] >= 0;
+    // nothing masked: 32 places that every row sees (least < to)
+    const bool open = whole0 && whole1 && at + kAtKeys - 1 <= least;
 
     // ---- scores: accumulator row g (and g + 8) is a key, columns 2c, 2c + 1 rows
     float z[2][NT][4];
@@ -280,10 +279,6 @@ __global__ void __launch_bounds__(kAtWarps * 32, NT == 1 ? 3 : 2) kv4_attn_kerne
       load_words<G>(kp + key0 * 4 * G, p0);
       load_words<G>(kp + key1 * 4 * G, p1);
 #pragma unroll
-      for (int j = 0; j < NT; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) z[mt][j][e] = 0.f;
-#pragma unroll
       for (int i = 0; i < G; ++i) {
         uint32_t f0[4], f1[4];
 #pragma unroll
@@ -295,13 +290,16 @@ __global__ void __launch_bounds__(kAtWarps * 32, NT == 1 ? 3 : 2) kv4_attn_kerne
         const float2 s1 = __half22float2(*reinterpret_cast<const __half2*>(&p1[i]));
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
-          float acc[4] = {qoff[j][i][0], qoff[j][i][1], qoff[j][i][0], qoff[j][i][1]};
-          mma_16816<T>(acc, f0[0], f1[0], f0[1], f1[1], qf[j][i][0], qf[j][i][1]);
+          float acc[4];
+          mma_16816<T>(acc, f0[0], f1[0], f0[1], f1[1], qf[j][i][0], qf[j][i][1], qoff[j][i][0], qoff[j][i][1],
+                       qoff[j][i][0], qoff[j][i][1]);
           mma_16816<T>(acc, f0[2], f1[2], f0[3], f1[3], qf[j][i][2], qf[j][i][3]);
-          z[mt][j][0] = fmaf(s0.x, acc[0], fmaf(s0.y, qsum[j][i][0], z[mt][j][0]));
-          z[mt][j][1] = fmaf(s0.x, acc[1], fmaf(s0.y, qsum[j][i][1], z[mt][j][1]));
-          z[mt][j][2] = fmaf(s1.x, acc[2], fmaf(s1.y, qsum[j][i][0], z[mt][j][2]));
-          z[mt][j][3] = fmaf(s1.x, acc[3], fmaf(s1.y, qsum[j][i][1], z[mt][j][3]));
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float2 s = e < 2 ? s0 : s1;
+            const float y = fmaf(s.x, acc[e], s.y * qsum[j][i][e & 1]);
+            z[mt][j][e] = i == 0 ? y : z[mt][j][e] + y;
+          }
         }
       }
       const bool whole = mt ? whole1 : whole0;
@@ -318,41 +316,45 @@ __global__ void __launch_bounds__(kAtWarps * 32, NT == 1 ? 3 : 2) kv4_attn_kerne
     }
 
     // ---- running maximum; the sums o and l follow it
-    bool grew = false;
-    float shrink[NT][2];
+    bool passed = false;
+    float top[NT][2];
 #pragma unroll
     for (int j = 0; j < NT; ++j)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        float x = fmaxf(fmaxf(z[0][j][e], z[0][j][2 + e]), fmaxf(z[1][j][e], z[1][j][2 + e]));
-#pragma unroll
-        for (int s = 4; s < 32; s <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, s));
-        const float mine = fmaxf(m[j][e], x);
-        grew |= mine > m[j][e];
-        shrink[j][e] = m[j][e] == mine ? 1.f : exp2f(m[j][e] - mine);
-        m[j][e] = mine;
+        top[j][e] = fmaxf(fmaxf(z[0][j][e], z[0][j][2 + e]), fmaxf(z[1][j][e], z[1][j][2 + e]));
+        passed |= top[j][e] > m[j][e] + kSlack;  // also the first score of a row: m is -inf
       }
-    if (__any_sync(0xffffffffu, grew)) {
+    if (__any_sync(0xffffffffu, passed)) {
 #pragma unroll
       for (int j = 0; j < NT; ++j) {
+        float shrink[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+#pragma unroll
+          for (int s = 4; s < 32; s <<= 1) top[j][e] = fmaxf(top[j][e], __shfl_xor_sync(0xffffffffu, top[j][e], s));
+          const float mine = fmaxf(m[j][e], top[j][e]);
+          shrink[e] = m[j][e] == mine ? 1.f : exp2_fast(m[j][e] - mine);
+          m[j][e] = mine;
+          l[j][e] *= shrink[e];
+        }
 #pragma unroll
         for (int i = 0; i < 2 * G; ++i)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) o[j][i][e] *= shrink[j][e & 1];
-#pragma unroll
-        for (int e = 0; e < 2; ++e) l[j][e] *= shrink[j][e];
+          for (int e = 0; e < 4; ++e) o[j][i][e] *= shrink[e & 1];
       }
     }
 #pragma unroll
-    for (int mt = 0; mt < 2; ++mt)
+    for (int j = 0; j < NT; ++j) {
+      const float less[2] = {m[j][0] == -INFINITY ? 0.f : m[j][0], m[j][1] == -INFINITY ? 0.f : m[j][1]};
 #pragma unroll
-      for (int j = 0; j < NT; ++j)
+      for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float top = m[j][e & 1] == -INFINITY ? 0.f : m[j][e & 1];
-          z[mt][j][e] = exp2f(z[mt][j][e] - top);
+          z[mt][j][e] = exp2_fast(z[mt][j][e] - less[e & 1]);
           l[j][e & 1] += z[mt][j][e];
         }
+    }
 
     // ---- output: accumulator rows are elements of the value, columns query rows
 #pragma unroll
@@ -414,6 +416,10 @@ __global__ void __launch_bounds__(kAtWarps * 32, NT == 1 ? 3 : 2) kv4_attn_kerne
     }
     __syncwarp();  // every lane has read the stage
     if (stage + kAtStages * kAtWarps < count) fetch(stage + kAtStages * kAtWarps, slot);
+    if (++slot == kAtStages) {
+      slot = 0;
+      phase ^= 1u;
+    }
   }
   if (!ok) {
     if (lane == 0) atomicOr(&g_kv4_attn_status, kStatusFullWaitTimeout);
