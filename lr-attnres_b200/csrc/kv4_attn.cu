@@ -250,24 +250,13 @@ __global__ void __launch_bounds__(kAtWarps * 32, NT == 1 ? 3 : 2) kv4_attn_kerne
   for (int j = 0; j < NT; ++j) m[j][0] = m[j][1] = -INFINITY;
   const float zscale = a.scale * kLog2e;
   const int swap = (g >> 1) & 1;          // keys in the order i ^ ((i >> 1) & 1)
-  bool ok = true;
-  int slot = 0, n = 0;
-  uint32_t phase = 0;
-  for (int stage = first; stage < count; stage += kAtWarps, ++n) {
-    ok = mbar_wait_bounded(&bars[warp][slot], phase);
-    if (!__all_sync(0xffffffffu, ok)) {
-      ok = false;
-      break;
-    }
-    const unsigned char* kc = ring + slot * kStage;
+  // One stage. MASKED: some of its 32 places may not be seen by some row; a copy of its own,
+  // as the tests, predicated away, would still take a third of the common one's issue slots.
+  auto attend = [&](const unsigned char* kc, int at, bool whole0, bool whole1, auto masked) {
+    constexpr bool MASKED = decltype(masked)::value;
     const unsigned char* vc = kc + kCode;
     const unsigned char* kp = kc + 2 * kCode;
     const unsigned char* vp = kp + kParam;
-    const int at = from + stage * kAtKeys;
-    const bool whole0 = rows16[2 * stage] >= 0, whole1 = at + 16 < to && rows16[2 * stage + 1] >= 0;
-    // nothing masked: 32 places that every row sees (least < to)
-    const bool open = whole0 && whole1 && at + kAtKeys - 1 <= least;
-
     // ---- scores: accumulator row g (and g + 8) is a key, columns 2c, 2c + 1 rows
     float z[2][NT][4];
 #pragma unroll
@@ -308,7 +297,7 @@ __global__ void __launch_bounds__(kAtWarps * 32, NT == 1 ? 3 : 2) kv4_attn_kerne
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           z[mt][j][e] *= zscale;
-          if (!open) {
+          if constexpr (MASKED) {
             const int place = at + (e < 2 ? key0 : key1);
             if (!whole || place >= to || place > last[j][e & 1]) z[mt][j][e] = -INFINITY;
           }
@@ -365,14 +354,14 @@ __global__ void __launch_bounds__(kAtWarps * 32, NT == 1 ? 3 : 2) kv4_attn_kerne
         const int i = 2 * c + (k & 1), key = mt * 16 + (i ^ ((i >> 1) & 1)) + (k >> 1) * 8;
         load_words<(G + 1) / 2>(vc + key * HALF + g * 2 * G, words[k]);
         load_words<G>(vp + key * 4 * G, par[k]);
-        if (!open) {
+        if constexpr (MASKED) {
           const bool there = (mt ? whole1 : whole0) && at + key < to;
 #pragma unroll
           for (int i2 = 0; i2 < G; ++i2)
             if (!there || not_finite(par[k][i2])) par[k][i2] = 0;
         }
       }
-      if (!open) {
+      if constexpr (MASKED) {
         const int key0 = mt * 16 + (g ^ swap);
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
@@ -414,6 +403,24 @@ __global__ void __launch_bounds__(kAtWarps * 32, NT == 1 ? 3 : 2) kv4_attn_kerne
         }
       }
     }
+  };
+
+  bool ok = true;
+  int slot = 0, n = 0;
+  uint32_t phase = 0;
+  for (int stage = first; stage < count; stage += kAtWarps, ++n) {
+    ok = mbar_wait_bounded(&bars[warp][slot], phase);
+    if (!__all_sync(0xffffffffu, ok)) {
+      ok = false;
+      break;
+    }
+    const int at = from + stage * kAtKeys;
+    const bool whole0 = rows16[2 * stage] >= 0, whole1 = at + 16 < to && rows16[2 * stage + 1] >= 0;
+    // nothing masked: 32 places that every row sees (least < to)
+    const bool open = whole0 && whole1 && at + kAtKeys - 1 <= least;
+
+    if (open) attend(ring + slot * kStage, at, true, true, std::false_type{});
+    else attend(ring + slot * kStage, at, whole0, whole1, std::true_type{});
     __syncwarp();  // every lane has read the stage
     if (stage + kAtStages * kAtWarps < count) fetch(stage + kAtStages * kAtWarps, slot);
     if (++slot == kAtStages) {
