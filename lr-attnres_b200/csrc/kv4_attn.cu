@@ -10,12 +10,14 @@
 // One pass with the running maximum and sum of the softmax. The products run on
 // mma.sync with the cache as the 16-row operand and the query rows as its 8 columns
 // (one token of one head fills one column: the tensor cores have time to spare, HBM has
-// not). A logic operation turns two codes into 16-bit floats: bits 0x4300 | n of bf16
-// are 128 + n; of f16, 0x6400 | n is 1024 + n and 0x5400 | n << 4 is 64 + n.
-//   scores  sum_d q_d (OFF + n_d) is exact up to fp32 sums that start at -sum_d q_d OFF;
-//           z = step * that + low Q, with Q the sum of the group's q
-//   output  values are f16 whatever q's type (step and low are): (OFF + n) - OFF is
-//           exact, step n + low is rounded once; weights, 0 to 1, are rounded to f16 too
+// not). Both multiply f16. A logic operation takes two codes out of a word:
+//   scores  the bits n and n << 4 alone are f16's small numbers 2^-24 n and 2^-20 n; q is
+//           scaled by a power of two per row (its largest element to 2^10 .. 2^11), and by
+//           16 more where it meets the smaller ones, so its elements are exact down to
+//           2^-24 of the largest. z = step * sum_d q_d n_d + low Q, Q the sum of the
+//           group's q: exact products, fp32 sums
+//   output  0x6400 | n is 1024 + n and 0x5400 | n << 4 is 64 + n; the difference to 1024 or
+//           64 is exact, step n + low is rounded once, weights (0 to 1) are too
 // The row of a key is an accumulator's row and a value's column: weights change sides
 // by movmatrix. Keys are taken in the order i ^ ((i >> 1) & 1) so that lanes that differ
 // in their keys read different halves of the banks.
@@ -59,21 +61,13 @@ struct AttnLaunch {
   float2* part_ml;             // [B, heads, row_tiles, splits, 8 NT]
 };
 
-// Code pair k of a word (bits 4 k and 16 + 4 k) as two 16-bit floats offset by kOff[k].
-template <typename T> struct Codes16;
-template <> struct Codes16<__nv_bfloat16> {
-  static __device__ __forceinline__ uint32_t pair(uint32_t w, int k) { return ((w >> (4 * k)) & 0x000f000fu) | 0x43004300u; }
-  static __device__ __forceinline__ uint32_t off(int) { return 0x43004300u; }  // 128, 128
-  static constexpr uint32_t kOnes = 0x3f803f80u;
-};
-template <> struct Codes16<__half> {
-  static __device__ __forceinline__ uint32_t pair(uint32_t w, int k) {
-    const uint32_t x = k >= 2 ? w >> 8 : w;
-    return (k & 1) ? (x & 0x00f000f0u) | 0x54005400u : (x & 0x000f000fu) | 0x64006400u;
-  }
-  static __device__ __forceinline__ uint32_t off(int k) { return (k & 1) ? 0x54005400u : 0x64006400u; }  // 64 or 1024
-  static constexpr uint32_t kOnes = 0x3c003c00u;
-};
+// Code pair k of a word (bits 4 k and 16 + 4 k) in the f16 halves' bits 0 .. 3 (even k) or
+// 4 .. 7 (odd k); and with the exponent that makes them 1024 + n or 64 + n.
+__device__ __forceinline__ uint32_t code_bits(uint32_t w, int k) {
+  return (k >= 2 ? w >> 8 : w) & ((k & 1) ? 0x00f000f0u : 0x000f000fu);
+}
+__device__ __forceinline__ uint32_t code_off(int k) { return (k & 1) ? 0x54005400u : 0x64006400u; }
+constexpr float kOddUnit = 1.f / 1048576.f;  // 2^-20: a code in bits 4 .. 7
 
 __device__ __forceinline__ uint32_t half_sub(uint32_t a, uint32_t b) {
   const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
@@ -143,7 +137,7 @@ __device__ __forceinline__ long long out_index(const AttnLaunch& L, int b, int h
 }
 
 template <typename T, int D, int NT>
-__global__ void __launch_bounds__(kAtWarps * 32, NT == 1 ? 3 : 2) kv4_attn_kernel(const __grid_constant__ AttnLaunch L) {
+__global__ void __launch_bounds__(kAtWarps * 32, NT == 1 ? (D == 64 ? 5 : 3) : 2) kv4_attn_kernel(const __grid_constant__ AttnLaunch L) {
   constexpr int G = D / kKv4Group, HALF = D / 2;
   constexpr int kCode = kAtKeys * HALF, kParam = kAtKeys * G * 4;  // bytes of a stage
   constexpr int kStage = 2 * (kCode + kParam);
@@ -199,8 +193,8 @@ __global__ void __launch_bounds__(kAtWarps * 32, NT == 1 ? 3 : 2) kv4_attn_kerne
 
   // the query rows as the second operand: column g of tile j is row 8 j + g
   uint32_t qf[NT][G][4];
-  float qsum[NT][G][2], qoff[NT][G][2];  // of columns 2 c, 2 c + 1: sum q, -sum q OFF
-  int last[NT][2];  // of rows 8 j + 2 c, 2 c + 1
+  float qsum[NT][G][2], zscale[NT][2];  // of rows 8 j + 2 c, 2 c + 1
+  int last[NT][2];
 #pragma unroll
   for (int j = 0; j < NT; ++j) {
     const int row = tile * ROWS + 8 * j + g;
@@ -210,30 +204,38 @@ __global__ void __launch_bounds__(kAtWarps * 32, NT == 1 ? 3 : 2) kv4_attn_kerne
       const int t = row / L.group, head = h * L.group + row - t * L.group;
       q += b * a.qs[0] + t * a.qs[1] + head * a.qs[2];
     }
+    float x[G][8], most = 0.f;
+#pragma unroll
+    for (int i = 0; i < G; ++i)
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        x[i][k] = there ? Elem<T>::to_f(q[i * 32 + c * 8 + k]) : 0.f;
+        most = fmaxf(most, fabsf(x[i][k]));
+      }
+#pragma unroll
+    for (int s = 1; s < 4; s <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, s));
+    // 2^(10 - exponent of the largest element), from the exponent's bits; 1 for an infinity
+    const int exponent = __float_as_int(most) >> 23;
+    const float up = exponent == 255 ? 1.f : __int_as_float(min(264 - exponent, 250) << 23);
 #pragma unroll
     for (int i = 0; i < G; ++i) {
-      uint16_t e[8];
 #pragma unroll
-      for (int k = 0; k < 8; ++k)
-        e[k] = there ? reinterpret_cast<const uint16_t*>(q)[i * 32 + c * 8 + k] : static_cast<uint16_t>(0);
-#pragma unroll
-      for (int k = 0; k < 4; ++k) qf[j][i][k] = e[k] | (static_cast<uint32_t>(e[k + 4]) << 16);
-      float s[4] = {}, f[4] = {};
-      const uint32_t one = Codes16<T>::kOnes, o0 = Codes16<T>::off(0), o1 = Codes16<T>::off(1);
-      mma_16816<T>(s, one, one, one, one, qf[j][i][0], qf[j][i][1]);
-      mma_16816<T>(s, one, one, one, one, qf[j][i][2], qf[j][i][3]);
-      mma_16816<T>(f, o0, o0, o1, o1, qf[j][i][0], qf[j][i][1]);
-      mma_16816<T>(f, o0, o0, o1, o1, qf[j][i][2], qf[j][i][3]);
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        qsum[j][i][e] = s[e];
-        qoff[j][i][e] = -f[e];
+      for (int k = 0; k < 4; ++k) {
+        const float f = (k & 1) ? up : 16.f * up;
+        qf[j][i][k] = half_pack(x[i][k] * f, x[i][k + 4] * f);
       }
+      float s[4] = {};
+      const uint32_t one = 0x3c003c00u, sixteenth = 0x2c002c00u;
+      mma_16816<__half>(s, sixteenth, sixteenth, one, one, qf[j][i][0], qf[j][i][1]);
+      mma_16816<__half>(s, sixteenth, sixteenth, one, one, qf[j][i][2], qf[j][i][3]);
+#pragma unroll
+      for (int e = 0; e < 2; ++e) qsum[j][i][e] = s[e] * kOddUnit;
     }
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       const int r = tile * ROWS + 8 * j + 2 * c + e;
       last[j][e] = r < L.rows ? last_place(seq, r / L.group) : -1;
+      zscale[j][e] = a.scale * (kLog2e / kOddUnit) / __shfl_sync(0xffffffffu, up, 4 * (2 * c + e));
     }
   }
   int least = 0x7fffffff;  // places up to this one are seen by all rows that see any
@@ -248,7 +250,6 @@ __global__ void __launch_bounds__(kAtWarps * 32, NT == 1 ? 3 : 2) kv4_attn_kerne
   float o[NT][2 * G][4] = {}, m[NT][2], l[NT][2] = {};
 #pragma unroll
   for (int j = 0; j < NT; ++j) m[j][0] = m[j][1] = -INFINITY;
-  const float zscale = a.scale * kLog2e;
   const int swap = (g >> 1) & 1;          // keys in the order i ^ ((i >> 1) & 1)
   // One stage. MASKED: some of its 32 places may not be seen by some row; a copy of its own,
   // as the tests, predicated away, would still take a third of the common one's issue slots.
@@ -272,22 +273,20 @@ __global__ void __launch_bounds__(kAtWarps * 32, NT == 1 ? 3 : 2) kv4_attn_kerne
         uint32_t f0[4], f1[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          f0[k] = Codes16<T>::pair(w0[i], k);
-          f1[k] = Codes16<T>::pair(w1[i], k);
+          f0[k] = code_bits(w0[i], k);
+          f1[k] = code_bits(w1[i], k);
         }
         const float2 s0 = __half22float2(*reinterpret_cast<const __half2*>(&p0[i]));
         const float2 s1 = __half22float2(*reinterpret_cast<const __half2*>(&p1[i]));
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
           float acc[4];
-          mma_16816<T>(acc, f0[0], f1[0], f0[1], f1[1], qf[j][i][0], qf[j][i][1], qoff[j][i][0], qoff[j][i][1],
-                       qoff[j][i][0], qoff[j][i][1]);
-          mma_16816<T>(acc, f0[2], f1[2], f0[3], f1[3], qf[j][i][2], qf[j][i][3]);
+          mma_16816<__half>(acc, f0[0], f1[0], f0[1], f1[1], qf[j][i][0], qf[j][i][1], 0.f, 0.f, 0.f, 0.f);
+          mma_16816<__half>(acc, f0[2], f1[2], f0[3], f1[3], qf[j][i][2], qf[j][i][3]);
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const float2 s = e < 2 ? s0 : s1;
-            const float y = fmaf(s.x, acc[e], s.y * qsum[j][i][e & 1]);
-            z[mt][j][e] = i == 0 ? y : z[mt][j][e] + y;
+            z[mt][j][e] = fmaf(s.x, acc[e], i == 0 ? s.y * qsum[j][i][e & 1] : fmaf(s.y, qsum[j][i][e & 1], z[mt][j][e]));
           }
         }
       }
@@ -296,7 +295,7 @@ __global__ void __launch_bounds__(kAtWarps * 32, NT == 1 ? 3 : 2) kv4_attn_kerne
       for (int j = 0; j < NT; ++j)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          z[mt][j][e] *= zscale;
+          z[mt][j][e] *= zscale[j][e & 1];
           if constexpr (MASKED) {
             const int place = at + (e < 2 ? key0 : key1);
             if (!whole || place >= to || place > last[j][e & 1]) z[mt][j][e] = -INFINITY;
@@ -394,7 +393,7 @@ __global__ void __launch_bounds__(kAtWarps * 32, NT == 1 ? 3 : 2) kv4_attn_kerne
           const uint32_t low = __byte_perm(par[2 * e][i], par[2 * e + 1][i], 0x7632u);
 #pragma unroll
           for (int k = 0; k < 4; ++k)
-            f[e][k] = half_fma(half_sub(Codes16<__half>::pair(w, k), Codes16<__half>::off(k)), step, low);
+            f[e][k] = half_fma(half_sub(code_bits(w, k) | code_off(k), code_off(k)), step, low);
         }
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
