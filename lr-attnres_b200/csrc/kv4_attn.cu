@@ -22,13 +22,13 @@
 // by movmatrix. Keys are taken in the order i ^ ((i >> 1) & 1) so that lanes that differ
 // in their keys read different halves of the banks.
 //
-// A value that some rows may not see must not reach them as 0 * NaN: in the 32 places
+// A value that some rows may not see must not reach them as 0 * NaN: in the stage
 // around a sequence's end, values that nobody sees count as zero, and so do those with
 // an infinity or NaN, which turn the rows that do see them into NaN through their sum.
 //
 // A CTA takes a stretch of places of one (sequence, key head, 8 NT query rows); its four
-// warps walk through it 32 places at a time, each with a ring of its own that bulk
-// copies fill (codes and params of 16 or 32 places are contiguous in a page). Sums of
+// warps walk through it 32 or 64 places at a time, each with a ring of its own that bulk
+// copies fill (codes and params of 16 places are contiguous in a page). Sums of
 // the warps are joined in shared memory, those of the stretches by kv4_join_kernel.
 // Every mbarrier wait is bounded (~2 s, a status bit on timeout).
 #include <algorithm>
@@ -44,8 +44,10 @@ namespace attnres {
 static __device__ unsigned int g_kv4_attn_status = 0;
 
 constexpr int kAtWarps = 4;
-constexpr int kAtStages = 3;       // 32 places each, per warp
-constexpr int kAtKeys = 32;
+// Places of a stage, and stages of a warp's ring: what a stage costs besides its places
+// (the wait, the copies, the maximum's vote) is a third of 32 places' work at head_dim 64.
+constexpr int at_keys(int D) { return D == 64 ? 64 : 32; }
+constexpr int at_stages(int D) { return D == 64 ? 2 : 3; }
 constexpr int kAtMaxStretch = 4096;
 constexpr float kLog2e = 1.4426950408889634f;
 // The running maximum is raised only when a score passes it by this much (in powers of
@@ -56,6 +58,7 @@ constexpr float kSlack = 8.f;
 struct AttnLaunch {
   Kv4AttnArgs a;
   int group, rows, row_tiles;  // query heads a key head; rows = T * group; tiles of 8 NT rows
+  int q_packs;                 // q's rows start on 16-byte boundaries
   int stretch, splits;         // places of a CTA, stretches of the longest possible sequence
   float* part_o;               // [B, heads, row_tiles, splits, 8 NT, D]
   float2* part_ml;             // [B, heads, row_tiles, splits, 8 NT]
@@ -139,21 +142,29 @@ __device__ __forceinline__ long long out_index(const AttnLaunch& L, int b, int h
 template <typename T, int D, int NT>
 __global__ void __launch_bounds__(kAtWarps * 32, NT == 1 ? (D == 64 ? 5 : 3) : 2) kv4_attn_kernel(const __grid_constant__ AttnLaunch L) {
   constexpr int G = D / kKv4Group, HALF = D / 2;
-  constexpr int kCode = kAtKeys * HALF, kParam = kAtKeys * G * 4;  // bytes of a stage
+  constexpr int KEYS = at_keys(D), PIECES = KEYS / 16, STAGES = at_stages(D);
+  constexpr int kCode = KEYS * HALF, kParam = KEYS * G * 4;  // bytes of a stage
   constexpr int kStage = 2 * (kCode + kParam);
   constexpr int ROWS = 8 * NT;
   const Kv4AttnArgs& a = L.a;
   extern __shared__ __align__(128) unsigned char smem[];
-  __shared__ int rows16[kAtMaxStretch / 16];  // row of the pool / 16 of each 16 places, -1 where there is no page
-  __shared__ uint64_t bars[kAtWarps][kAtStages];
-  __shared__ float warp_m[kAtWarps][ROWS], warp_l[kAtWarps][ROWS];
+  __shared__ __align__(16) int rows16[kAtMaxStretch / 16];  // row of the pool / 16 of each 16 places, -1 where there is no page
+  __shared__ uint64_t bars[kAtWarps][STAGES];
+  __shared__ float warp_m[kAtWarps][ROWS], warp_l[kAtWarps][ROWS], row_top[ROWS], row_sum[ROWS];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
   const int split = blockIdx.x % L.splits, tile = blockIdx.x / L.splits, h = blockIdx.y, b = blockIdx.z;
   const SeqFacts seq = seq_facts(a, b);
   const int from = split * L.stretch, to = min(from + L.stretch, seq.length);
+  // the join may take up its place on the GPU; it waits for this grid's end before it reads
+  if (L.splits > 1) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (from >= to && L.splits > 1) return;  // the join knows how many stretches there are
 
-  for (int i = threadIdx.x; i * 16 < to - from; i += kAtWarps * 32) {
+  const int count = (to - from + KEYS - 1) / KEYS;  // a warp's stages: its number, + 4, ...
+  for (int i = threadIdx.x; i < count * PIECES; i += kAtWarps * 32) {
+    if (i * 16 >= to - from) {
+      rows16[i] = -1;
+      continue;
+    }
     const int at = from + i * 16, slot = at / a.c.page;
     const int p = a.table[b * a.table_stride + slot];
     const bool there = p >= 0 && p < a.c.pages;
@@ -162,34 +173,32 @@ __global__ void __launch_bounds__(kAtWarps * 32, NT == 1 ? (D == 64 ? 5 : 3) : 2
     rows16[i] = there ? static_cast<int>((static_cast<long long>(p) * a.c.heads + h) * (a.c.page >> 4)) + place16 : -1;
   }
   if (lane == 0)
-    for (int i = 0; i < kAtStages; ++i) mbar_init(&bars[warp][i], 1);
+    for (int i = 0; i < STAGES; ++i) mbar_init(&bars[warp][i], 1);
   fence_mbar_init();
   __syncthreads();
 
-  const int first = warp, count = (to - from + kAtKeys - 1) / kAtKeys;  // this warp's stages: first, first + 4, ...
-  unsigned char* ring = smem + warp * kAtStages * kStage;
-  // Lanes 0 .. 7 copy 16 places each: lane & 3 is keys, key params, values, value params.
+  unsigned char* ring = smem + warp * STAGES * kStage;
+  // Lanes copy 16 places each: lane & 3 is keys, key params, values, value params.
   const unsigned char* const my_src = static_cast<const unsigned char*>(
       (lane & 2) ? ((lane & 1) ? a.c.v_params : a.c.v_codes) : ((lane & 1) ? a.c.k_params : a.c.k_codes));
   const uint32_t my_bytes = 16 * ((lane & 1) ? G * 4 : HALF);
+  const int my_piece = lane >> 2;
   unsigned char* const my_dst = ring + ((lane & 1) ? 2 * kCode + ((lane >> 1) & 1) * kParam : ((lane >> 1) & 1) * kCode) +
-                                ((lane >> 2) & 1) * my_bytes;
+                                my_piece * my_bytes;
   auto fetch = [&](int stage, int slot) {
-    const int i = 2 * stage;
-    const int r0 = rows16[i], r1 = (i + 1) * 16 < to - from ? rows16[i + 1] : -1;
+    const int r = my_piece < PIECES ? rows16[stage * PIECES + my_piece] : -1;
+    const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, r >= 0)) * (kStage / PIECES / 4);
     if (lane == 0) {
-      const uint32_t bytes = (r0 >= 0 ? kStage / 2 : 0) + (r1 >= 0 ? kStage / 2 : 0);
       if (bytes) mbar_arrive_expect_tx(&bars[warp][slot], bytes);
       else mbar_arrive(&bars[warp][slot]);
     }
     __syncwarp();
-    const int r = lane < 4 ? r0 : r1;
-    if (lane < 8 && r >= 0)
+    if (r >= 0)
       bulk_g2s(my_dst + slot * kStage, my_src + static_cast<long long>(r) * my_bytes, my_bytes, &bars[warp][slot]);
   };
 #pragma unroll
-  for (int i = 0; i < kAtStages; ++i)
-    if (first + i * kAtWarps < count) fetch(first + i * kAtWarps, i);
+  for (int i = 0; i < STAGES; ++i)
+    if (warp + i * kAtWarps < count) fetch(warp + i * kAtWarps, i);
 
   // the query rows as the second operand: column g of tile j is row 8 j + g
   uint32_t qf[NT][G][4];
@@ -206,12 +215,20 @@ __global__ void __launch_bounds__(kAtWarps * 32, NT == 1 ? (D == 64 ? 5 : 3) : 2
     }
     float x[G][8], most = 0.f;
 #pragma unroll
-    for (int i = 0; i < G; ++i)
+    for (int i = 0; i < G; ++i) {
+      Pack<T, 8> v = {};
+      if (there && L.q_packs) {
+        v = load_pack<T, 8>(q + i * 32 + c * 8);
+      } else if (there) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v.e[k] = q[i * 32 + c * 8 + k];
+      }
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
-        x[i][k] = there ? Elem<T>::to_f(q[i * 32 + c * 8 + k]) : 0.f;
+        x[i][k] = Elem<T>::to_f(v.e[k]);
         most = fmaxf(most, fabsf(x[i][k]));
       }
+    }
 #pragma unroll
     for (int s = 1; s < 4; s <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, s));
     // 2^(10 - exponent of the largest element), from the exponent's bits; 1 for an infinity
@@ -251,17 +268,17 @@ __global__ void __launch_bounds__(kAtWarps * 32, NT == 1 ? (D == 64 ? 5 : 3) : 2
 #pragma unroll
   for (int j = 0; j < NT; ++j) m[j][0] = m[j][1] = -INFINITY;
   const int swap = (g >> 1) & 1;          // keys in the order i ^ ((i >> 1) & 1)
-  // One stage. MASKED: some of its 32 places may not be seen by some row; a copy of its own,
+  // One stage. MASKED: some of its places may not be seen by some row; a copy of its own,
   // as the tests, predicated away, would still take a third of the common one's issue slots.
-  auto attend = [&](const unsigned char* kc, int at, bool whole0, bool whole1, auto masked) {
+  auto attend = [&](const unsigned char* kc, int at, int stage, auto masked) {
     constexpr bool MASKED = decltype(masked)::value;
     const unsigned char* vc = kc + kCode;
     const unsigned char* kp = kc + 2 * kCode;
     const unsigned char* vp = kp + kParam;
     // ---- scores: accumulator row g (and g + 8) is a key, columns 2c, 2c + 1 rows
-    float z[2][NT][4];
+    float z[PIECES][NT][4];
 #pragma unroll
-    for (int mt = 0; mt < 2; ++mt) {
+    for (int mt = 0; mt < PIECES; ++mt) {
       const int key0 = mt * 16 + (g ^ swap), key1 = key0 + 8;
       uint32_t w0[G], w1[G], p0[G], p1[G];
       load_words<G>(kc + key0 * HALF + c * 4 * G, w0);
@@ -290,7 +307,6 @@ __global__ void __launch_bounds__(kAtWarps * 32, NT == 1 ? (D == 64 ? 5 : 3) : 2
           }
         }
       }
-      const bool whole = mt ? whole1 : whole0;
 #pragma unroll
       for (int j = 0; j < NT; ++j)
 #pragma unroll
@@ -298,7 +314,7 @@ __global__ void __launch_bounds__(kAtWarps * 32, NT == 1 ? (D == 64 ? 5 : 3) : 2
           z[mt][j][e] *= zscale[j][e & 1];
           if constexpr (MASKED) {
             const int place = at + (e < 2 ? key0 : key1);
-            if (!whole || place >= to || place > last[j][e & 1]) z[mt][j][e] = -INFINITY;
+            if (rows16[stage * PIECES + mt] < 0 || place >= to || place > last[j][e & 1]) z[mt][j][e] = -INFINITY;
           }
         }
     }
@@ -310,7 +326,9 @@ __global__ void __launch_bounds__(kAtWarps * 32, NT == 1 ? (D == 64 ? 5 : 3) : 2
     for (int j = 0; j < NT; ++j)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        top[j][e] = fmaxf(fmaxf(z[0][j][e], z[0][j][2 + e]), fmaxf(z[1][j][e], z[1][j][2 + e]));
+        top[j][e] = fmaxf(z[0][j][e], z[0][j][2 + e]);
+#pragma unroll
+        for (int mt = 1; mt < PIECES; ++mt) top[j][e] = fmaxf(top[j][e], fmaxf(z[mt][j][e], z[mt][j][2 + e]));
         passed |= top[j][e] > m[j][e] + kSlack;  // also the first score of a row: m is -inf
       }
     if (__any_sync(0xffffffffu, passed)) {
@@ -336,7 +354,7 @@ __global__ void __launch_bounds__(kAtWarps * 32, NT == 1 ? (D == 64 ? 5 : 3) : 2
     for (int j = 0; j < NT; ++j) {
       const float less[2] = {m[j][0] == -INFINITY ? 0.f : m[j][0], m[j][1] == -INFINITY ? 0.f : m[j][1]};
 #pragma unroll
-      for (int mt = 0; mt < 2; ++mt)
+      for (int mt = 0; mt < PIECES; ++mt)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           z[mt][j][e] = exp2_fast(z[mt][j][e] - less[e & 1]);
@@ -346,7 +364,7 @@ __global__ void __launch_bounds__(kAtWarps * 32, NT == 1 ? (D == 64 ? 5 : 3) : 2
 
     // ---- output: accumulator rows are elements of the value, columns query rows
 #pragma unroll
-    for (int mt = 0; mt < 2; ++mt) {
+    for (int mt = 0; mt < PIECES; ++mt) {
       uint32_t words[4][(G + 1) / 2], par[4][G];
 #pragma unroll
       for (int k = 0; k < 4; ++k) {  // MMA columns 2c, 2c + 1, 2c + 8, 2c + 9
@@ -354,7 +372,7 @@ __global__ void __launch_bounds__(kAtWarps * 32, NT == 1 ? (D == 64 ? 5 : 3) : 2
         load_words<(G + 1) / 2>(vc + key * HALF + g * 2 * G, words[k]);
         load_words<G>(vp + key * 4 * G, par[k]);
         if constexpr (MASKED) {
-          const bool there = (mt ? whole1 : whole0) && at + key < to;
+          const bool there = rows16[stage * PIECES + mt] >= 0 && at + key < to;
 #pragma unroll
           for (int i2 = 0; i2 < G; ++i2)
             if (!there || not_finite(par[k][i2])) par[k][i2] = 0;
@@ -407,22 +425,27 @@ __global__ void __launch_bounds__(kAtWarps * 32, NT == 1 ? (D == 64 ? 5 : 3) : 2
   bool ok = true;
   int slot = 0, n = 0;
   uint32_t phase = 0;
-  for (int stage = first; stage < count; stage += kAtWarps, ++n) {
+  for (int stage = warp; stage < count; stage += kAtWarps, ++n) {
     ok = mbar_wait_bounded(&bars[warp][slot], phase);
     if (!__all_sync(0xffffffffu, ok)) {
       ok = false;
       break;
     }
-    const int at = from + stage * kAtKeys;
-    const bool whole0 = rows16[2 * stage] >= 0, whole1 = at + 16 < to && rows16[2 * stage + 1] >= 0;
-    // nothing masked: 32 places that every row sees (least < to)
-    const bool open = whole0 && whole1 && at + kAtKeys - 1 <= least;
-
-    if (open) attend(ring + slot * kStage, at, true, true, std::false_type{});
-    else attend(ring + slot * kStage, at, whole0, whole1, std::true_type{});
+    const int at = from + stage * KEYS;
+    int rows = 0;  // negative if 16 places have no page
+    if constexpr (PIECES == 4) {
+      const int4 r = *reinterpret_cast<const int4*>(rows16 + stage * 4);
+      rows = r.x | r.y | r.z | r.w;
+    } else {
+      const int2 r = *reinterpret_cast<const int2*>(rows16 + stage * 2);
+      rows = r.x | r.y;
+    }
+    // nothing masked: places that are there and that every row sees (least < to)
+    if (rows >= 0 && at + KEYS - 1 <= least) attend(ring + slot * kStage, at, stage, std::false_type{});
+    else attend(ring + slot * kStage, at, stage, std::true_type{});
     __syncwarp();  // every lane has read the stage
-    if (stage + kAtStages * kAtWarps < count) fetch(stage + kAtStages * kAtWarps, slot);
-    if (++slot == kAtStages) {
+    if (stage + STAGES * kAtWarps < count) fetch(stage + STAGES * kAtWarps, slot);
+    if (++slot == STAGES) {
       slot = 0;
       phase ^= 1u;
     }
@@ -430,9 +453,9 @@ __global__ void __launch_bounds__(kAtWarps * 32, NT == 1 ? (D == 64 ? 5 : 3) : 2
   if (!ok) {
     if (lane == 0) atomicOr(&g_kv4_attn_status, kStatusFullWaitTimeout);
     // copies still in flight land before the CTA's shared memory is given away
-    for (int i = 0; i < kAtStages; ++i, ++n)
-      if (first + n * kAtWarps < count &&
-          !mbar_wait_bounded(&bars[warp][n % kAtStages], static_cast<uint32_t>((n / kAtStages) & 1)) && lane == 0)
+    for (int i = 0; i < STAGES; ++i, ++n)
+      if (warp + n * kAtWarps < count &&
+          !mbar_wait_bounded(&bars[warp][n % STAGES], static_cast<uint32_t>((n / STAGES) & 1)) && lane == 0)
         atomicOr(&g_kv4_attn_status, kStatusDrainTimeout);
   }
 
@@ -465,27 +488,42 @@ __global__ void __launch_bounds__(kAtWarps * 32, NT == 1 ? (D == 64 ? 5 : 3) : 2
         const int element = 32 * (i >> 1) + 4 * g + 2 * (i & 1) + (e >> 1);
         sums[(warp * ROWS + 8 * j + 2 * c + (e & 1)) * PITCH + element] = o[j][i][e];
       }
-  __syncthreads();
-  const long long unit = ((static_cast<long long>(b) * a.c.heads + h) * L.row_tiles + tile) * L.splits + split;
-  for (int i = threadIdx.x; i < ROWS * D; i += kAtWarps * 32) {
-    const int r = i / D, d = i - r * D, row = tile * ROWS + r;
-    if (row >= L.rows) break;
-    float top = warp_m[0][r];
+  // weights of the warps' sums, once a row (over the maxima they came from)
+  if (threadIdx.x < ROWS) {
+    const int r = threadIdx.x;
+    float top = warp_m[0][r], total = 0.f;
 #pragma unroll
     for (int w = 1; w < kAtWarps; ++w) top = fmaxf(top, warp_m[w][r]);
-    float total = 0.f, y = 0.f;
 #pragma unroll
     for (int w = 0; w < kAtWarps; ++w) {
       const float f = warp_m[w][r] == -INFINITY ? 0.f : exp2f(warp_m[w][r] - top);
       total += f * warp_l[w][r];
-      y += f * sums[(w * ROWS + r) * PITCH + d];
+      warp_m[w][r] = f;
     }
+    row_top[r] = top;
+    row_sum[r] = total;
+  }
+  __syncthreads();
+  const long long unit = ((static_cast<long long>(b) * a.c.heads + h) * L.row_tiles + tile) * L.splits + split;
+  for (int i = threadIdx.x * 4; i < ROWS * D; i += kAtWarps * 32 * 4) {
+    const int r = i / D, d = i - r * D, row = tile * ROWS + r;
+    if (row >= L.rows) break;
+    float y[4] = {};
+#pragma unroll
+    for (int w = 0; w < kAtWarps; ++w) {
+      const float4 x = *reinterpret_cast<const float4*>(&sums[(w * ROWS + r) * PITCH + d]);
+      const float f = warp_m[w][r];
+      y[0] += f * x.x, y[1] += f * x.y, y[2] += f * x.z, y[3] += f * x.w;
+    }
+    const float top = row_top[r], total = row_sum[r];
     if (L.splits == 1) {
       const long long to_row = out_index<T>(L, b, h, row);
-      static_cast<T*>(a.out)[to_row * D + d] = Elem<T>::from_f(top == -INFINITY ? 0.f : y / total);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) y[e] = top == -INFINITY ? 0.f : y[e] / total;
+      store_pack<T, 4>(static_cast<T*>(a.out) + to_row * D + d, y);
       if (a.lse && d == 0) a.lse[to_row] = top == -INFINITY ? -INFINITY : (top + log2f(total)) / kLog2e;
     } else {
-      L.part_o[(unit * ROWS + r) * D + d] = y;
+      store_pack<float, 4>(L.part_o + (unit * ROWS + r) * D + d, y);
       if (d == 0) L.part_ml[unit * ROWS + r] = make_float2(top, total);
     }
   }
@@ -501,6 +539,7 @@ __global__ void __launch_bounds__(128) kv4_join_kernel(const __grid_constant__ A
   const int row = static_cast<int>(index % L.rows);
   const long long bh = index / L.rows;
   const int h = static_cast<int>(bh % a.c.heads), b = static_cast<int>(bh / a.c.heads);
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   const SeqFacts seq = seq_facts(a, b);
   const int n = (seq.length + L.stretch - 1) / L.stretch;
   const long long unit = (bh * L.row_tiles + row / tile_rows) * L.splits;
@@ -531,10 +570,10 @@ namespace {
 
 int tiles_of_rows(int rows) { return rows <= 8 ? 1 : 2; }  // NT
 
-int stage_bytes(int D) { return 2 * kAtKeys * (D / 2 + D / kKv4Group * 4); }
+int stage_bytes(int D) { return 2 * at_keys(D) * (D / 2 + D / kKv4Group * 4); }
 
 size_t attn_smem(int D, int NT) {
-  const size_t ring = static_cast<size_t>(kAtWarps) * kAtStages * stage_bytes(D);
+  const size_t ring = static_cast<size_t>(kAtWarps) * at_stages(D) * stage_bytes(D);
   const size_t sums = static_cast<size_t>(kAtWarps) * 8 * NT * (D + 4) * sizeof(float);
   return std::max(ring, sums);
 }
@@ -556,6 +595,7 @@ AttnLaunch plan(const Kv4AttnArgs& a) {
   long long stretch = (std::min<long long>(wish, room) + 127) / 128 * 128;
   stretch = std::min<long long>(std::max<long long>(stretch, 128), kAtMaxStretch);
   L.stretch = static_cast<int>(stretch);
+  L.q_packs = (reinterpret_cast<uintptr_t>(a.q) & 15u) == 0 && a.qs[0] % 8 == 0 && a.qs[1] % 8 == 0 && a.qs[2] % 8 == 0;
   L.splits = static_cast<int>((room + stretch - 1) / stretch);
   return L;
 }
@@ -575,8 +615,17 @@ cudaError_t attn_t(const AttnLaunch& L, cudaStream_t st) {
   kv4_attn_kernel<T, D, NT><<<grid, kAtWarps * 32, smem, st>>>(L);
   if ((e = cudaGetLastError()) != cudaSuccess || L.splits == 1) return e;
   const long long rows = static_cast<long long>(L.a.B) * L.a.c.heads * L.rows;
-  kv4_join_kernel<T, D><<<static_cast<unsigned>((rows + 3) / 4), 128, 0, st>>>(L, 8 * NT);
-  return cudaGetLastError();
+  // a programmatic dependent: its launch overlaps the attention (3 us less a call)
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>((rows + 3) / 4));
+  cfg.blockDim = dim3(128);
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kv4_join_kernel<T, D>, L, 8 * NT);
 }
 
 template <typename T>
