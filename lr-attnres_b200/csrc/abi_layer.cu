@@ -137,9 +137,9 @@ attnres::Kv4Cache kv4_cache(const void* k_codes, const void* k_params, const voi
           const_cast<void*>(v_params), pages, heads, page, D};
 }
 
-// One thread for 8 elements of a key and its value in 32-bit block counts.
+// The kernels count groups of 32 elements in 32 bits.
 int check_kv4_rows(const attnres::Kv4RowsArgs& a) {
-  if (static_cast<double>(a.B) * a.T * a.c.heads * (a.c.D / 8) > 256.0 * 0x7fffffff)
+  if (static_cast<double>(a.B) * a.T * a.c.heads * (a.c.D / 32) > 0x7fffffff)
     return fail(ATTNRES_ERR_UNSUPPORTED, "kv4 cache: too many tokens for one launch");
   return ATTNRES_OK;
 }

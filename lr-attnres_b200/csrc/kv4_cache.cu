@@ -7,10 +7,13 @@
 // reads back as NaN.
 //
 // Four lanes share a group (8 elements each, two shuffles for its extremes), and a
-// thread does the same part of a key and of its value, so that both loads are in
-// flight. Bound by HBM and close behind it by issue slots: the quotient is formed with
-// the reciprocal and redone by division only within 2^-16 of a tie, which keeps the
-// codes those of the division.
+// thread does the same part of a key and of its value, of two groups next to each other
+// where a head has an even number: four loads in flight, and one look at the page table. HBM is the floor, issue slots are what it meets first (a thread has 20 bytes
+// for every 16 elements it forms), so the work per element is kept to a subtraction, a
+// product, a sum that rounds (adding 1.5 * 2^23 leaves the integer in the low bits), a
+// multiply-add into the packed word, and the distance to a tie: the quotient is formed
+// with the reciprocal, and the eight are redone by division if one of them comes within
+// 2^-16 of a tie, which keeps the codes those of the division.
 #include "common.cuh"
 #include "kv4.h"
 #include "tma.cuh"
@@ -19,29 +22,48 @@ namespace attnres {
 
 static __device__ unsigned int g_kv4_status = 0;
 
-// Row of the pool of token t of sequence b for head 0 (head h is h * page rows on),
-// -1 if the token takes no part, -2 if the page table has no page for it.
-__device__ __forceinline__ long long kv4_row(const Kv4RowsArgs& a, int b, int t) {
-  if (a.counts && t >= a.counts[b]) return -1;
-  const long long at = static_cast<long long>(a.start[b]) + t;
-  if (at < 0) return -2;
-  const long long slot = at / a.c.page;
-  if (slot >= a.max_pages) return -2;
-  const int page = a.table[b * a.table_stride + slot];
-  if (page < 0 || page >= a.c.pages) return -2;
-  return static_cast<long long>(page) * a.c.heads * a.c.page + (at - slot * a.c.page);
+// Which group of which token a thread's quad of lanes has. Everything is counted in 32
+// bits (the host refuses more groups than that): 64-bit divisions were most of the time.
+struct GroupRef {
+  unsigned g, h, t, b;  // g: the first of N groups
+};
+template <int N>
+__device__ __forceinline__ GroupRef group_ref(const Kv4RowsArgs& a, unsigned quad) {
+  const unsigned G = a.c.D / kKv4Group / N;
+  GroupRef r;
+  unsigned i = quad / G;
+  r.g = (quad - i * G) * N;
+  const unsigned j = i / a.c.heads;
+  r.h = i - j * a.c.heads;
+  r.b = j / a.T;
+  r.t = j - r.b * a.T;
+  return r;
 }
 
-// 8 consecutive elements as fp32, by 16-byte loads where the row allows.
-template <typename T>
-__device__ __forceinline__ void load8(const T* p, bool packs, float (&x)[8]) {
-  if (packs) {
+// Row of the pool of the group's token and head, -1 if the token takes no part, -2 if the
+// page table has no page for it.
+__device__ __forceinline__ long long kv4_row(const Kv4RowsArgs& a, const GroupRef& r) {
+  if (a.counts && static_cast<int>(r.t) >= a.counts[r.b]) return -1;
+  const int start = a.start[r.b];
+  const unsigned at = static_cast<unsigned>(start) + r.t;  // below 2^32: both are below 2^31
+  if (start < 0) return -2;
+  const unsigned slot = at / a.c.page;
+  if (slot >= static_cast<unsigned>(a.max_pages)) return -2;
+  const int page = a.table[r.b * a.table_stride + slot];
+  if (page < 0 || page >= a.c.pages) return -2;
+  return (static_cast<long long>(page) * a.c.heads + r.h) * a.c.page + (at - slot * a.c.page);
+}
+
+// 8 consecutive elements as fp32, PACKS: by 16-byte loads.
+template <typename T, bool PACKS>
+__device__ __forceinline__ void load8(const T* p, float (&x)[8]) {
+  if constexpr (PACKS) {
     constexpr int VEC = 16 / sizeof(T);
 #pragma unroll
     for (int i = 0; i < 8; i += VEC) {
       const Pack<T, VEC> v = load_stream<T, VEC>(p + i);
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) x[i + e] = Elem<T>::to_f(v.e[e]);
+      for (int e = 0; e < VEC / 2; ++e) unpack2<T, VEC>(v, e, x[i + 2 * e], x[i + 2 * e + 1]);
     }
   } else {
 #pragma unroll
@@ -49,128 +71,194 @@ __device__ __forceinline__ void load8(const T* p, bool packs, float (&x)[8]) {
   }
 }
 
+// The larger / smaller of the two, NaN if either is one.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float min_nan(float a, float b) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
 struct Quantised {
   uint32_t codes;  // element e in bits 4e .. 4e + 3
   __half2 params;  // step, low
 };
 
+constexpr float kRounder = 12582912.f;  // 1.5 * 2^23: x + kRounder holds rint(x) in its low bits
+
 // The four lanes of a group call this together.
 __device__ __forceinline__ Quantised quantise8(const float (&x)[8]) {
   float top = x[0], low = x[0];
-  bool odd = false;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    top = fmaxf(top, x[e]);
-    low = fminf(low, x[e]);
-    odd |= !(fabsf(x[e]) <= 3.402823466e38f);
+  for (int e = 1; e < 8; ++e) {
+    top = max_nan(top, x[e]);
+    low = min_nan(low, x[e]);
   }
 #pragma unroll
   for (int o = 1; o < 4; o <<= 1) {
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    low = fminf(low, __shfl_xor_sync(0xffffffffu, low, o));
-    odd |= __shfl_xor_sync(0xffffffffu, static_cast<int>(odd), o) != 0;
+    top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
+    low = min_nan(low, __shfl_xor_sync(0xffffffffu, low, o));
   }
+  const float range = __fsub_rn(top, low), nan = __int_as_float(0x7fffffff);
+  const bool odd = !(range <= 3.402823466e38f);  // an infinity or a NaN among them
   Quantised r;
-  const float nan = __int_as_float(0x7fffffff);
-  r.params = odd ? __floats2half2_rn(nan, nan)
-                 : __floats2half2_rn(__fmul_rn(__fsub_rn(top, low), 1.f / 15.f), low);
+  r.params = odd ? __floats2half2_rn(nan, nan) : __floats2half2_rn(__fmul_rn(range, 1.f / 15.f), low);
   const float step = __low2float(r.params), base = __high2float(r.params);
-  r.codes = 0;
-  if (step > 0.f) {
-    const float inv = __frcp_rn(step);
+  const float inv = step > 0.f ? __fdividef(1.f / 15.f, step) : 0.f;  // codes of 0 where there is no step
+  float worst = 0.f;
+  uint32_t word = 0, own = 0;  // own: the rounder's own bits, 0x4b400000 at every shift that keeps some
 #pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    // the quotient over 15, clamped to 0 .. 1 on the way
+    const float q = __saturatef(__fsub_rn(x[e], base) * inv), n = fmaf(q, 15.f, kRounder);
+    worst = fmaxf(worst, fabsf(fmaf(q, 15.f, -__fsub_rn(n, kRounder))));
+    word += __float_as_uint(n) << (4 * e);
+    own += 0x4b400000u << (4 * e);
+  }
+  r.codes = word - own;
+  if (worst > 0.5f - 1.f / 65536.f) {
+    r.codes = 0;
+#pragma unroll 1
     for (int e = 0; e < 8; ++e) {
-      const float d = __fsub_rn(x[e], base), quotient = d * inv;
-      float n = rintf(quotient);
-      if (fabsf(quotient - n) > 0.5f - 1.f / 65536.f) n = rintf(__fdiv_rn(d, step));
+      float y = x[0];  // x[e], without an array in memory
+#pragma unroll
+      for (int i = 1; i < 8; ++i) y = i == e ? x[i] : y;
+      const float n = rintf(__fdiv_rn(__fsub_rn(y, base), step));
       r.codes |= static_cast<uint32_t>(fminf(fmaxf(n, 0.f), 15.f)) << (4 * e);
     }
   }
   return r;
 }
 
-template <typename T>
-__global__ void __launch_bounds__(256) kv4_append_kernel(const __grid_constant__ Kv4RowsArgs a, bool packs) {
-  const int G = a.c.D / kKv4Group;
-  const long long quad = (static_cast<long long>(blockIdx.x) * 256 + threadIdx.x) >> 2;
-  const int c = threadIdx.x & 3;
-  const long long total = static_cast<long long>(a.B) * a.T * a.c.heads * G;
-  const bool live = quad < total;  // whole groups; the shuffles need every lane
-  long long i = live ? quad : 0;
-  const int g = static_cast<int>(i % G);
-  i /= G;
-  const int h = static_cast<int>(i % a.c.heads);
-  i /= a.c.heads;
-  const int t = static_cast<int>(i % a.T), b = static_cast<int>(i / a.T);
-  const long long base = live ? kv4_row(a, b, t) : -1;
-  float k[8] = {}, v[8] = {};
-  if (base >= 0) {
-    const int e = g * kKv4Group + c * 8;
-    load8<T>(static_cast<const T*>(a.k) + b * a.ks[0] + t * a.ks[1] + h * a.ks[2] + e, packs, k);
-    load8<T>(static_cast<const T*>(a.v) + b * a.vs[0] + t * a.vs[1] + h * a.vs[2] + e, packs, v);
-  }
-  const Quantised qk = quantise8(k), qv = quantise8(v);
-  if (base < 0) {
-    if (base == -2) atomicOr(&g_kv4_status, kStatusCacheRange);
-    return;
-  }
-  const long long row = base + static_cast<long long>(h) * a.c.page;
-  reinterpret_cast<uint32_t*>(static_cast<unsigned char*>(a.c.k_codes) + row * (a.c.D / 2))[c * G + g] = qk.codes;
-  uint16_t* vc = reinterpret_cast<uint16_t*>(static_cast<unsigned char*>(a.c.v_codes) + row * (a.c.D / 2));
-  vc[2 * c * G + g] = static_cast<uint16_t>(qv.codes);
-  vc[(2 * c + 1) * G + g] = static_cast<uint16_t>(qv.codes >> 16);
-  if (c == 0) static_cast<__half2*>(a.c.k_params)[row * G + g] = qk.params;
-  if (c == 1) static_cast<__half2*>(a.c.v_params)[row * G + g] = qv.params;
+// N 32-bit words next to each other.
+template <int N>
+__device__ __forceinline__ void put_words(uint32_t* p, const uint32_t (&w)[N]) {
+  if constexpr (N == 2) *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+  else *p = w[0];
 }
 
+template <typename T, bool PACKS, int N>
+__global__ void __launch_bounds__(256) kv4_append_kernel(const __grid_constant__ Kv4RowsArgs a) {
+  const int G = a.c.D / kKv4Group;
+  const unsigned quad = blockIdx.x * 64u + (threadIdx.x >> 2);
+  const int c = threadIdx.x & 3;
+  const unsigned total = static_cast<unsigned>(a.B) * a.T * a.c.heads * (G / N);
+  const bool live = quad < total;  // whole groups; the shuffles need every lane
+  const GroupRef at = group_ref<N>(a, live ? quad : 0);
+  const long long row = live ? kv4_row(a, at) : -1;
+  float k[N][8] = {}, v[N][8] = {};
+  if (row >= 0) {
+    const int e = at.g * kKv4Group + c * 8;
+    const T* kr = static_cast<const T*>(a.k) + at.b * a.ks[0] + at.t * a.ks[1] + at.h * a.ks[2] + e;
+    const T* vr = static_cast<const T*>(a.v) + at.b * a.vs[0] + at.t * a.vs[1] + at.h * a.vs[2] + e;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      load8<T, PACKS>(kr + i * kKv4Group, k[i]);
+      load8<T, PACKS>(vr + i * kKv4Group, v[i]);
+    }
+  }
+  Quantised qk[N], qv[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    qk[i] = quantise8(k[i]);
+    qv[i] = quantise8(v[i]);
+  }
+  if (row < 0) {
+    if (row == -2) atomicOr(&g_kv4_status, kStatusCacheRange);
+    return;
+  }
+  unsigned char* kc = static_cast<unsigned char*>(a.c.k_codes) + row * (a.c.D / 2);
+  uint16_t* vc = reinterpret_cast<uint16_t*>(static_cast<unsigned char*>(a.c.v_codes) + row * (a.c.D / 2));
+  uint32_t words[N], params[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    words[i] = qk[i].codes;
+    const __half2 p = c == 0 ? qk[i].params : qv[i].params;
+    params[i] = *reinterpret_cast<const uint32_t*>(&p);
+  }
+  put_words<N>(reinterpret_cast<uint32_t*>(kc) + c * G + at.g, words);
+  if constexpr (N == 2) {
+    *reinterpret_cast<uint32_t*>(vc + 2 * c * G + at.g) = __byte_perm(qv[0].codes, qv[1].codes, 0x5410);
+    *reinterpret_cast<uint32_t*>(vc + (2 * c + 1) * G + at.g) = __byte_perm(qv[0].codes, qv[1].codes, 0x7632);
+  } else {
+    vc[2 * c * G + at.g] = static_cast<uint16_t>(qv[0].codes);
+    vc[(2 * c + 1) * G + at.g] = static_cast<uint16_t>(qv[0].codes >> 16);
+  }
+  if (c < 2) put_words<N>(static_cast<uint32_t*>(c == 0 ? a.c.k_params : a.c.v_params) + row * G + at.g, params);
+}
+
+// Codes become floats by way of 2^23 + n (an exact difference; conversion instructions are
+// an eighth as fast).
 template <typename T>
 __device__ __forceinline__ void store_values(T* out, uint32_t codes, __half2 params, bool there) {
-  const float step = __low2float(params), low = __high2float(params);
+  const float step = there ? __low2float(params) : 0.f, low = there ? __high2float(params) : 0.f;
   constexpr int VEC = 16 / sizeof(T);
 #pragma unroll
   for (int i = 0; i < 8; i += VEC) {
-    float y[VEC];
+    Pack<T, VEC> y;
 #pragma unroll
-    for (int e = 0; e < VEC; ++e)
-      y[e] = there ? __fadd_rn(low, __fmul_rn(step, static_cast<float>((codes >> (4 * (i + e))) & 15u))) : 0.f;
-    store_pack<T, VEC>(out + i, y);
+    for (int e = 0; e < VEC; e += 2) {
+      float v[2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const uint32_t n = ((codes >> (4 * (i + e + j))) & 15u) | 0x4b000000u;
+        v[j] = fmaf(step, __uint_as_float(n) - 8388608.f, low);
+      }
+      if constexpr (std::is_same<T, float>::value) {
+        y.e[e] = v[0];
+        y.e[e + 1] = v[1];
+      } else if constexpr (std::is_same<T, __half>::value) {
+        *reinterpret_cast<__half2*>(&y.e[e]) = __floats2half2_rn(v[0], v[1]);
+      } else {
+        *reinterpret_cast<__nv_bfloat162*>(&y.e[e]) = __floats2bfloat162_rn(v[0], v[1]);
+      }
+    }
+    *reinterpret_cast<Pack<T, VEC>*>(out + i) = y;
   }
 }
 
-template <typename T>
+template <typename T, int N>
 __global__ void __launch_bounds__(256) kv4_read_kernel(const __grid_constant__ Kv4RowsArgs a) {
   const int G = a.c.D / kKv4Group;
-  const long long quad = (static_cast<long long>(blockIdx.x) * 256 + threadIdx.x) >> 2;
+  const unsigned quad = blockIdx.x * 64u + (threadIdx.x >> 2);
   const int c = threadIdx.x & 3;
-  if (quad >= static_cast<long long>(a.B) * a.T * a.c.heads * G) return;
-  long long i = quad;
-  const int g = static_cast<int>(i % G);
-  i /= G;
-  const int h = static_cast<int>(i % a.c.heads);
-  i /= a.c.heads;
-  const int t = static_cast<int>(i % a.T), b = static_cast<int>(i / a.T);
-  const long long base = kv4_row(a, b, t);
-  uint32_t kw = 0, vw = 0;
-  __half2 kp = __half2{}, vp = __half2{};
-  if (base >= 0) {
-    const long long row = base + static_cast<long long>(h) * a.c.page;
-    kw = reinterpret_cast<const uint32_t*>(static_cast<const unsigned char*>(a.c.k_codes) + row * (a.c.D / 2))[c * G + g];
+  if (quad >= static_cast<unsigned>(a.B) * a.T * a.c.heads * (G / N)) return;
+  const GroupRef at = group_ref<N>(a, quad);
+  const long long row = kv4_row(a, at);
+  uint32_t kw[N] = {}, vw[N] = {};
+  __half2 kp[N] = {}, vp[N] = {};
+  if (row >= 0) {
+    const uint32_t* kc = reinterpret_cast<const uint32_t*>(static_cast<const unsigned char*>(a.c.k_codes) + row * (a.c.D / 2));
     const uint16_t* vc = reinterpret_cast<const uint16_t*>(static_cast<const unsigned char*>(a.c.v_codes) + row * (a.c.D / 2));
-    vw = vc[2 * c * G + g] | (static_cast<uint32_t>(vc[(2 * c + 1) * G + g]) << 16);
-    kp = static_cast<const __half2*>(a.c.k_params)[row * G + g];
-    vp = static_cast<const __half2*>(a.c.v_params)[row * G + g];
-  } else if (base == -2) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      kw[i] = kc[c * G + at.g + i];
+      vw[i] = vc[2 * c * G + at.g + i] | (static_cast<uint32_t>(vc[(2 * c + 1) * G + at.g + i]) << 16);
+      kp[i] = static_cast<const __half2*>(a.c.k_params)[row * G + at.g + i];
+      vp[i] = static_cast<const __half2*>(a.c.v_params)[row * G + at.g + i];
+    }
+  } else if (row == -2) {
     atomicOr(&g_kv4_status, kStatusCacheRange);
   }
-  const long long to = quad * kKv4Group + c * 8;
-  store_values<T>(static_cast<T*>(a.k_out) + to, kw, kp, base >= 0);
-  store_values<T>(static_cast<T*>(a.v_out) + to, vw, vp, base >= 0);
+  const long long to = static_cast<long long>(quad) * (N * kKv4Group) + c * 8;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    store_values<T>(static_cast<T*>(a.k_out) + to + i * kKv4Group, kw[i], kp[i], row >= 0);
+    store_values<T>(static_cast<T*>(a.v_out) + to + i * kKv4Group, vw[i], vp[i], row >= 0);
+  }
 }
 
 namespace {
 
+// Two groups a thread where a head's groups come in pairs.
+int groups_a_thread(const Kv4RowsArgs& a) { return a.c.D / kKv4Group % 2 == 0 ? 2 : 1; }
+
 unsigned blocks_of(const Kv4RowsArgs& a) {
-  const long long threads = 4LL * a.B * a.T * a.c.heads * (a.c.D / kKv4Group);
+  const long long threads = 4LL * a.B * a.T * a.c.heads * (a.c.D / kKv4Group / groups_a_thread(a));
   return static_cast<unsigned>((threads + 255) / 256);
 }
 
@@ -178,7 +266,17 @@ template <typename T>
 cudaError_t append_t(const Kv4RowsArgs& a, cudaStream_t st) {
   bool packs = (reinterpret_cast<uintptr_t>(a.k) & 15u) == 0 && (reinterpret_cast<uintptr_t>(a.v) & 15u) == 0;
   for (int i = 0; i < 3; ++i) packs = packs && a.ks[i] * sizeof(T) % 16 == 0 && a.vs[i] * sizeof(T) % 16 == 0;
-  kv4_append_kernel<T><<<blocks_of(a), 256, 0, st>>>(a, packs);
+  const bool two = groups_a_thread(a) == 2;
+  const auto fn = packs ? (two ? kv4_append_kernel<T, true, 2> : kv4_append_kernel<T, true, 1>)
+                        : (two ? kv4_append_kernel<T, false, 2> : kv4_append_kernel<T, false, 1>);
+  fn<<<blocks_of(a), 256, 0, st>>>(a);
+  return cudaGetLastError();
+}
+
+template <typename T>
+cudaError_t read_t(const Kv4RowsArgs& a, cudaStream_t st) {
+  const auto fn = groups_a_thread(a) == 2 ? kv4_read_kernel<T, 2> : kv4_read_kernel<T, 1>;
+  fn<<<blocks_of(a), 256, 0, st>>>(a);
   return cudaGetLastError();
 }
 
@@ -193,13 +291,11 @@ cudaError_t kv4_append_launch(int dtype, const Kv4RowsArgs& a, cudaStream_t st) 
 }
 
 cudaError_t kv4_read_launch(int dtype, const Kv4RowsArgs& a, cudaStream_t st) {
-  const unsigned grid = blocks_of(a);
   switch (dtype) {
-    case ATTNRES_DTYPE_F32: kv4_read_kernel<float><<<grid, 256, 0, st>>>(a); break;
-    case ATTNRES_DTYPE_F16: kv4_read_kernel<__half><<<grid, 256, 0, st>>>(a); break;
-    default: kv4_read_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(a);
+    case ATTNRES_DTYPE_F32: return read_t<float>(a, st);
+    case ATTNRES_DTYPE_F16: return read_t<__half>(a, st);
+    default: return read_t<__nv_bfloat16>(a, st);
   }
-  return cudaGetLastError();
 }
 
 cudaError_t read_kv4_status(unsigned* status, bool reset) {
