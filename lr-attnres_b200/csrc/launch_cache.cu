@@ -21,6 +21,7 @@ std::mutex g_mu;
 DeviceFacts g_dev[kMaxDevices];
 std::map<std::pair<int, const void*>, int> g_smem;                            // (device, fn) -> bytes set
 std::map<std::tuple<int, const void*, int, size_t>, int> g_occupancy;         // -> blocks per SM
+std::map<std::tuple<int, const void*, int, int, size_t>, int> g_clusters;     // -> clusters resident at once
 
 cudaError_t facts(DeviceFacts** out, int* dev_out) {
   int dev = 0;
@@ -87,6 +88,37 @@ cudaError_t cached_occupancy(int* per_sm, const void* fn, int block, size_t smem
   if (e != cudaSuccess) return e;
   std::lock_guard<std::mutex> lock(g_mu);
   g_occupancy[key] = *per_sm;
+  return cudaSuccess;
+}
+
+cudaError_t cached_max_clusters(int* clusters, const void* fn, int ctas, int block, size_t smem) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const auto key = std::make_tuple(dev, fn, ctas, block, smem);
+  {
+    std::lock_guard<std::mutex> lock(g_mu);
+    auto it = g_clusters.find(key);
+    if (it != g_clusters.end()) {
+      *clusters = it->second;
+      return cudaSuccess;
+    }
+  }
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(ctas);
+  cfg.blockDim = dim3(block);
+  cfg.dynamicSmemBytes = smem;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = static_cast<unsigned>(ctas);
+  at[0].val.clusterDim.y = 1;
+  at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  e = cudaOccupancyMaxActiveClusters(clusters, fn, &cfg);
+  if (e != cudaSuccess) return e;
+  std::lock_guard<std::mutex> lock(g_mu);
+  g_clusters[key] = *clusters;
   return cudaSuccess;
 }
 

@@ -18,4 +18,7 @@ cudaError_t ensure_dynamic_smem(const void* fn, int bytes);
 // cudaOccupancyMaxActiveBlocksPerMultiprocessor, cached per (device, fn, block, smem)
 cudaError_t cached_occupancy(int* per_sm, const void* fn, int block, size_t smem);
 
+// cudaOccupancyMaxActiveClusters of clusters of `ctas` CTAs, cached per (device, fn, ctas, block, smem)
+cudaError_t cached_max_clusters(int* clusters, const void* fn, int ctas, int block, size_t smem);
+
 }  // namespace attnres

@@ -19,12 +19,17 @@
 //   dW             A = [du dg]^T, B = x, both MN-major.
 // Few tokens: swiglu_few_kernel streams W once past the registers of all SMs.
 //
-// Roles in a CTA: warp 0 one thread of TMA loads into a ring of stages, warp 1 one
-// thread of tcgen05.mma, 8 warps of epilogue on the other half of the accumulators.
-// Every mbarrier wait is bounded (~2 s, a status bit on timeout); tensor memory is
-// always released.
+// Two CTAs of a cluster share a tile (tcgen05 cta_group::2): each loads its own 128 rows
+// of A and half of B and holds its 128 rows of the sums, so an SM takes in 32 KB for 128 x
+// 256 x 64 products instead of 48. With one CTA a tile the products ran at 1185 TFLOP/s,
+// bound by that intake.
+// Roles: warp 0 one thread of TMA loads into a ring of stages, warp 1 of the even CTA one
+// thread of tcgen05.mma for both, 8 warps of epilogue on the other half of the
+// accumulators. Every mbarrier wait is bounded (~2 s, a status bit on timeout); tensor
+// memory is always released.
 #include <algorithm>
 
+#include "cluster.cuh"
 #include "common.cuh"
 #include "launch_cache.h"
 #include "mma.cuh"
@@ -36,35 +41,97 @@ namespace attnres {
 
 static __device__ unsigned int g_swiglu_status = 0;
 
-constexpr int kGmM = 128, kGmN = 256, kGmK = 64;  // tile, and columns of a stage
-constexpr int kGmStages = 4;
-constexpr uint32_t kGmABytes = kGmM * kGmK * 2, kGmBBytes = kGmN * kGmK * 2;
-constexpr uint32_t kGmStageBytes = kGmABytes + kGmBBytes;
+constexpr int kGmM = 256, kGmK = 64;  // rows of a pair's tile, columns of a stage
+constexpr int kGmRing = 6 * 32768;    // bytes of stages
 constexpr int kGmEpiWarps = 8;
 constexpr int kGmThreads = (2 + kGmEpiWarps) * 32;
-constexpr size_t kGmSmem = 1024 + kGmStages * kGmStageBytes + 256;
+constexpr size_t kGmSmem = 1024 + kGmRing + 256;
 
-enum GemmMode { kGateForward, kGateBackward, kGradInput, kGradWeight };
+enum GemmMode { kGateForward, kGateBackward, kGradients };
 
-struct GemmArgs {
+// One product: out [M, cols] = A B, in tiles of 256 x BN.
+struct GemmJob {
   CUtensorMap a, b, b2;  // b2: the gate rows of the two gate modes
-  void* out;             // h [N, F]; [du dg] [N, 2F]; dx [N, C]; dW [2F, C]
-  const void* dh;        // gate backward
-  long long out_stride, dh_stride;
-  long long M;           // rows of the output
+  void* out;             // h [N, F]; [du dg] [N, 2F]; dW [2F, C]; dx [N, C]
+  long long out_stride, M;
   int cols;              // columns of the output (gate modes: F)
   int tiles_m, tiles_n, ksteps;
   uint32_t idesc;
 };
+struct GemmArgs {
+  GemmJob job[2];  // kGradients: dW, then dx; else one
+  const void* dh;  // gate backward
+  long long dh_stride;
+  // dx tiles of a pair after its dW tiles: x each for the first `more` pairs (which have
+  // a dW tile more than the others), y each for the rest
+  int more, x, y;
+};
 
-// Tiles in bands of 16 row tiles, rows fastest inside a band: the CTAs running at one
+struct TileRef {
+  int job, m, n;
+};
+
+// Tiles in bands of 8 row tiles, rows fastest inside a band: the pairs running at one
 // time read few distinct row and column panels, which stay in L2.
-__device__ __forceinline__ void tile_at(const GemmArgs& a, int tile, int& m, int& n) {
-  constexpr int BAND = 16;
-  const int per_band = BAND * a.tiles_n, band = tile / per_band, in = tile - band * per_band;
-  const int rows = min(BAND, a.tiles_m - band * BAND);
-  n = in / rows;
-  m = band * BAND + in - n * rows;
+__device__ __forceinline__ TileRef tile_at(const GemmArgs& a, int job, int tile) {
+  constexpr int BAND = 8;
+  const GemmJob& g = a.job[job];
+  const int per_band = BAND * g.tiles_n, band = tile / per_band, in = tile - band * per_band;
+  const int rows = min(BAND, g.tiles_m - band * BAND), n = in / rows;
+  return {job, band * BAND + in - n * rows, n};
+}
+
+// The i-th tile of pair p of P, job -1 when there is none.
+template <int MODE>
+__device__ __forceinline__ TileRef tile_of(const GemmArgs& a, int p, int P, int i) {
+  const int first = a.job[0].tiles_m * a.job[0].tiles_n;
+  const int own = p < first ? (first - 1 - p) / P + 1 : 0;
+  if (i < own) return tile_at(a, 0, p + i * P);
+  if (MODE == kGradients) {
+    const int j = i - own, each = p < a.more ? a.x : a.y;
+    const int tile = p < a.more ? j * a.more + p : a.more * a.x + j * (P - a.more) + p - a.more;
+    if (j < each && tile < a.job[1].tiles_m * a.job[1].tiles_n) return tile_at(a, 1, tile);
+  }
+  return {-1, 0, 0};
+}
+
+// ---- the two-CTA forms of the tensor-core instructions
+// A TMA load into this CTA's shared memory that completes on an mbarrier of the cluster's
+// even CTA (its shared::cluster address).
+__device__ __forceinline__ void tma_load_2d_pair(void* dst, const CUtensorMap* map, int c0, int c1, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], "
+      "[%4];" ::"r"(smem_u32(dst)),
+      "l"(map), "r"(c0), "r"(c1), "r"(bar)
+      : "memory");
+}
+__device__ __forceinline__ void umma_f16_pair(uint32_t tmem_d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+      :
+      : "r"(tmem_d), "l"(a), "l"(b), "r"(idesc), "r"(acc));
+}
+// Arrives on the mbarrier at this address in both CTAs when the MMAs issued so far are done.
+__device__ __forceinline__ void umma_commit_pair(uint64_t* bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+          smem_u32(bar)),
+      "h"(static_cast<uint16_t>(3))
+      : "memory");
+}
+__device__ __forceinline__ void tmem_alloc_pair(uint32_t* slot, uint32_t cols) {
+  asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(slot)), "r"(cols)
+               : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_dealloc_pair(uint32_t base, uint32_t cols) {
+  asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(base), "r"(cols) : "memory");
+}
+// Arrives on an mbarrier of a CTA of the cluster (shared::cluster address).
+__device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 
 __device__ __forceinline__ float sigmoid_fast(float g) { return __fdividef(1.f, 1.f + __expf(-g)); }
@@ -82,213 +149,224 @@ __device__ __forceinline__ void store8(T* p, const float* v) {
   *reinterpret_cast<Pack<T, 8>*>(p) = r;
 }
 
-template <typename T, int MODE>
-__global__ void __launch_bounds__(kGmThreads, 1) swiglu_gemm_kernel(const __grid_constant__ GemmArgs a) {
-  constexpr bool GATE = MODE == kGateForward || MODE == kGateBackward;
+template <typename T, int MODE, int BN>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGmThreads, 1)
+    swiglu_gemm_kernel(const __grid_constant__ GemmArgs a) {
+  constexpr bool GATE = MODE != kGradients;
+  constexpr uint32_t kA = 128 * kGmK * 2, kB = BN / 2 * kGmK * 2, kStage = kA + kB;  // bytes, of each CTA
+  constexpr int STAGES = kGmRing / kStage, F = BN / 2;                               // F: outputs of a gate tile
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* stages =
       reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint64_t* full = reinterpret_cast<uint64_t*>(stages + kGmStages * kGmStageBytes);
-  uint64_t* empty = full + kGmStages;
-  uint64_t* acc_full = empty + kGmStages;
-  uint64_t* acc_empty = acc_full + 2;
+  uint64_t* full = reinterpret_cast<uint64_t*>(stages + kGmRing);  // the even CTA's are used
+  uint64_t* empty = full + STAGES;
+  uint64_t* acc_full = empty + STAGES;
+  uint64_t* acc_empty = acc_full + 2;  // the even CTA's are used
   uint64_t* done = acc_empty + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int ntiles = a.tiles_m * a.tiles_n, nk = a.ksteps;
+  const int rank = cluster_rank(), pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < kGmStages; ++i) {
+    for (int i = 0; i < STAGES; ++i) {
       mbar_init(&full[i], 1);
       mbar_init(&empty[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&acc_full[i], 1);
-      mbar_init(&acc_empty[i], kGmEpiWarps);
+      mbar_init(&acc_empty[i], 2 * kGmEpiWarps);
     }
     mbar_init(done, 1);
     *abort_flag = 0;
     fence_mbar_init();
   }
-  if (warp == 1) tmem_alloc(tmem_slot, 512);
+  if (warp == 1) tmem_alloc_pair(tmem_slot, 512);
   tc_fence_before();
   __syncthreads();
+  cluster_sync_all();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
   if (warp == 0) {
-    // ---------------- TMA producer -------------------------------------------
+    // ---------------- TMA producer: this CTA's half of each stage ------------------
     if (lane == 0) {
       long long it = 0;
       bool ok = true;
-      for (int tile = blockIdx.x; tile < ntiles && ok; tile += gridDim.x) {
-        int m, n;
-        tile_at(a, tile, m, n);
-        for (int kc = 0; kc < nk; ++kc, ++it) {
-          const int st = static_cast<int>(it % kGmStages);
-          if (*abort_flag || !mbar_wait_bounded(&empty[st], static_cast<uint32_t>((it / kGmStages) & 1) ^ 1u)) {
+      for (int i = 0; ok; ++i) {
+        const TileRef t = tile_of<MODE>(a, pair, pairs, i);
+        if (t.job < 0) break;
+        const GemmJob& g = a.job[t.job];
+        const int m0 = t.m * kGmM + rank * 128;
+        for (int kc = 0; kc < g.ksteps; ++kc, ++it) {
+          const int st = static_cast<int>(it % STAGES);
+          if (*abort_flag || !mbar_wait_bounded(&empty[st], static_cast<uint32_t>((it / STAGES) & 1) ^ 1u)) {
             atomicOr(&g_swiglu_status, kStatusEmptyWaitTimeout);
             *abort_flag = 1;
             ok = false;
             break;
           }
-          unsigned char* sa = stages + st * kGmStageBytes;
-          unsigned char* sb = sa + kGmABytes;
-          mbar_arrive_expect_tx(&full[st], kGmStageBytes);
-          if (MODE == kGradWeight) {
-            for (int i = 0; i < kGmM / 64; ++i)
-              tma_load_2d(sa + i * 64 * 128, &a.a, m * kGmM + i * 64, kc * kGmK, &full[st]);
-          } else {
-            tma_load_2d(sa, &a.a, kc * kGmK, m * kGmM, &full[st]);
-          }
+          unsigned char* sa = stages + st * kStage;
+          unsigned char* sb = sa + kA;
+          if (rank == 0) mbar_arrive_expect_tx(&full[st], 2 * kStage);
+          const uint32_t bar = map_to_rank(smem_u32(&full[st]), 0);
           if (GATE) {
-            tma_load_2d(sb, &a.b, kc * kGmK, n * 128, &full[st]);
-            tma_load_2d(sb + 128 * 128, &a.b2, kc * kGmK, n * 128, &full[st]);
+            tma_load_2d_pair(sa, &g.a, kc * kGmK, m0, bar);
+            tma_load_2d_pair(sb, rank == 0 ? &g.b : &g.b2, kc * kGmK, t.n * F, bar);
           } else {
-            for (int i = 0; i < kGmN / 64; ++i)
-              tma_load_2d(sb + i * 64 * 128, &a.b, n * kGmN + i * 64, kc * kGmK, &full[st]);
+            if (t.job == 0) {  // dW: rows of A are columns of [du dg]
+              tma_load_2d_pair(sa, &g.a, m0, kc * kGmK, bar);
+              tma_load_2d_pair(sa + 64 * 128, &g.a, m0 + 64, kc * kGmK, bar);
+            } else {
+              tma_load_2d_pair(sa, &g.a, kc * kGmK, m0, bar);
+            }
+#pragma unroll
+            for (int j = 0; j < BN / 128; ++j)
+              tma_load_2d_pair(sb + j * 64 * 128, &g.b, t.n * BN + rank * (BN / 2) + j * 64, kc * kGmK, bar);
           }
         }
       }
-      if (!ok) {
-        for (long long j = (it > kGmStages ? it - kGmStages : 0); j < it; ++j)
-          if (!mbar_wait_bounded(&full[j % kGmStages], static_cast<uint32_t>((j / kGmStages) & 1)))
+      if (!ok && rank == 0) {
+        // stages that were posted land in both CTAs before either goes on to exit
+        for (long long j = (it > STAGES ? it - STAGES : 0); j < it; ++j)
+          if (!mbar_wait_bounded(&full[j % STAGES], static_cast<uint32_t>((j / STAGES) & 1)))
             atomicOr(&g_swiglu_status, kStatusDrainTimeout);
       }
     }
   } else if (warp == 1) {
-    // ---------------- MMA issuer -----------------------------------------------
-    if (lane == 0) {
+    // ---------------- MMA issuer of the pair ---------------------------------------
+    if (lane == 0 && rank == 0) {
       long long it = 0;
-      int count = 0;
-      bool issued_any = false;
-      for (int tile = blockIdx.x; tile < ntiles; tile += gridDim.x, ++count) {
-        const int ab = count & 1;
-        if (*abort_flag || !mbar_wait_bounded(&acc_empty[ab], static_cast<uint32_t>((count >> 1) & 1) ^ 1u)) {
+      bool issued_any = false, ok = true;
+      for (int i = 0; ok; ++i) {
+        const TileRef t = tile_of<MODE>(a, pair, pairs, i);
+        if (t.job < 0) break;
+        const GemmJob& g = a.job[t.job];
+        const int ab = i & 1;
+        if (*abort_flag || !mbar_wait_cluster(&acc_empty[ab], static_cast<uint32_t>((i >> 1) & 1) ^ 1u)) {
           atomicOr(&g_swiglu_status, kStatusEmptyWaitTimeout);
           *abort_flag = 1;
           break;
         }
         tc_fence_after();
-        const uint32_t acc = tmem + ab * kGmN;
-        bool ok = true;
-        for (int kc = 0; kc < nk; ++kc, ++it) {
-          const int st = static_cast<int>(it % kGmStages);
-          if (*abort_flag || !mbar_wait_bounded(&full[st], static_cast<uint32_t>((it / kGmStages) & 1))) {
+        const uint32_t acc = tmem + ab * BN;
+        const bool a_mn = !GATE && t.job == 0;
+        for (int kc = 0; kc < g.ksteps; ++kc, ++it) {
+          const int st = static_cast<int>(it % STAGES);
+          if (*abort_flag || !mbar_wait_bounded(&full[st], static_cast<uint32_t>((it / STAGES) & 1))) {
             atomicOr(&g_swiglu_status, kStatusFullWaitTimeout);
             *abort_flag = 1;
             ok = false;
             break;
           }
           tc_fence_after();
-          const unsigned char* sa = stages + st * kGmStageBytes;
-          const unsigned char* sb = sa + kGmABytes;
+          const unsigned char* sa = stages + st * kStage;
+          const unsigned char* sb = sa + kA;
           // K = 16 an instruction: 32 bytes on in a K-major tile, two groups of 8
           // rows (2048 bytes) in an MN-major one
-          const uint64_t da = MODE == kGradWeight ? umma_desc_sw128_mn(sa, 64 * 128) : umma_desc_sw128(sa);
+          const uint64_t da = a_mn ? umma_desc_sw128_mn(sa, 64 * 128) : umma_desc_sw128(sa);
           const uint64_t db = GATE ? umma_desc_sw128(sb) : umma_desc_sw128_mn(sb, 64 * 128);
+          const uint64_t da_step = a_mn ? 128 : 2, db_step = GATE ? 2 : 128;
 #pragma unroll
           for (int k = 0; k < kGmK / 16; ++k)
-            umma_f16(acc, da + (MODE == kGradWeight ? 128 : 2) * k, db + (GATE ? 2 : 128) * k, a.idesc,
-                     (kc > 0 || k > 0) ? 1u : 0u);
-          umma_commit(&empty[st]);
+            umma_f16_pair(acc, da + da_step * k, db + db_step * k, g.idesc, (kc > 0 || k > 0) ? 1u : 0u);
+          umma_commit_pair(&empty[st]);
           issued_any = true;
         }
-        if (!ok) break;
-        umma_commit(&acc_full[ab]);
+        if (ok) umma_commit_pair(&acc_full[ab]);
       }
-      umma_commit(done);  // all MMAs of this CTA retired before the accumulators are freed
+      umma_commit_pair(done);  // all MMAs retired before the accumulators are freed
       if (issued_any && !mbar_wait_bounded(done, 0)) atomicOr(&g_swiglu_status, kStatusDrainTimeout);
     }
   } else {
     // ---------------- epilogue: one accumulator row a thread, half the columns a warp
     const int q = warp & 3, half = (warp - 2) >> 2;
     const uint32_t lane_off = static_cast<uint32_t>(q * 32) << 16;
-    T* out = static_cast<T*>(a.out);
-    int count = 0;
-    for (int tile = blockIdx.x; tile < ntiles; tile += gridDim.x, ++count) {
-      int m, n;
-      tile_at(a, tile, m, n);
-      const int ab = count & 1;
-      if (*abort_flag || !mbar_wait_bounded(&acc_full[ab], static_cast<uint32_t>((count >> 1) & 1))) {
+    const uint32_t freed[2] = {map_to_rank(smem_u32(&acc_empty[0]), 0), map_to_rank(smem_u32(&acc_empty[1]), 0)};
+    for (int i = 0;; ++i) {
+      const TileRef t = tile_of<MODE>(a, pair, pairs, i);
+      if (t.job < 0) break;
+      const GemmJob& g = a.job[t.job];
+      const int ab = i & 1;
+      if (*abort_flag || !mbar_wait_bounded(&acc_full[ab], static_cast<uint32_t>((i >> 1) & 1))) {
         *abort_flag = 1;
         break;
       }
       tc_fence_after();
-      const long long row = static_cast<long long>(m) * kGmM + q * 32 + lane;
-      const uint32_t acc = tmem + lane_off + ab * kGmN;
+      const long long row = static_cast<long long>(t.m) * kGmM + rank * 128 + q * 32 + lane;
+      const uint32_t acc = tmem + lane_off + ab * BN;
+      T* out = static_cast<T*>(g.out) + row * g.out_stride;
       if constexpr (GATE) {
-        const int f0 = n * 128 + half * 64;
-        T* o = out + row * a.out_stride + f0;
+        const int f0 = t.n * F + half * (F / 2);
+        T* o = out + f0;
         const T* dh = MODE == kGateBackward ? static_cast<const T*>(a.dh) + row * a.dh_stride + f0 : nullptr;
 #pragma unroll 1
-        for (int c = 0; c < 64; c += 16) {
+        for (int c = 0; c < F / 2; c += 16) {
           uint32_t ur[16], gr[16];
-          tmem_ld16_nowait(acc + half * 64 + c, ur);
-          tmem_ld16_nowait(acc + 128 + half * 64 + c, gr);
+          tmem_ld16_nowait(acc + half * (F / 2) + c, ur);
+          tmem_ld16_nowait(acc + F + half * (F / 2) + c, gr);
           Pack<T, 8> d[2];
           if (MODE == kGateBackward) {
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
-              if (row < a.M && f0 + c + i * 8 < a.cols) d[i] = load_stream<T, 8>(dh + c + i * 8);
-              else d[i] = Pack<T, 8>{};
+            for (int j = 0; j < 2; ++j)
+              if (row < g.M && f0 + c + j * 8 < g.cols) d[j] = load_stream<T, 8>(dh + c + j * 8);
+              else d[j] = Pack<T, 8>{};
           }
           tmem_ld_wait();
           tmem_regs_ready(ur);
           tmem_regs_ready(gr);
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
+          for (int j = 0; j < 2; ++j) {
             float y[8], z[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-              const float u = __uint_as_float(ur[i * 8 + e]), g = __uint_as_float(gr[i * 8 + e]);
-              const float s = sigmoid_fast(g), silu = g * s;
+              const float u = __uint_as_float(ur[j * 8 + e]), gt = __uint_as_float(gr[j * 8 + e]);
+              const float s = sigmoid_fast(gt), silu = gt * s;
               if (MODE == kGateForward) {
                 y[e] = u * silu;
               } else {
-                const float dhe = Elem<T>::to_f(d[i].e[e]);
+                const float dhe = Elem<T>::to_f(d[j].e[e]);
                 y[e] = dhe * silu;
                 z[e] = dhe * u * (s + silu * (1.f - s));
               }
             }
-            if (row < a.M && f0 + c + i * 8 < a.cols) {
-              store8<T>(o + c + i * 8, y);
-              if (MODE == kGateBackward) store8<T>(o + a.cols + c + i * 8, z);
+            if (row < g.M && f0 + c + j * 8 < g.cols) {
+              store8<T>(o + c + j * 8, y);
+              if (MODE == kGateBackward) store8<T>(o + g.cols + c + j * 8, z);
             }
           }
         }
       } else {
-        const int c0 = n * kGmN + half * 128;
-        T* o = out + row * a.out_stride + c0;
+        const int c0 = t.n * BN + half * (BN / 2);
 #pragma unroll 1
-        for (int c = 0; c < 128; c += 32) {
+        for (int c = 0; c < BN / 2; c += 32) {
           uint32_t r0[16], r1[16];
-          tmem_ld16_nowait(acc + half * 128 + c, r0);
-          tmem_ld16_nowait(acc + half * 128 + c + 16, r1);
+          tmem_ld16_nowait(acc + half * (BN / 2) + c, r0);
+          tmem_ld16_nowait(acc + half * (BN / 2) + c + 16, r1);
           tmem_ld_wait();
           tmem_regs_ready(r0);
           tmem_regs_ready(r1);
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (row < a.M && c0 + c + i * 8 < a.cols) {
+          for (int j = 0; j < 4; ++j)
+            if (row < g.M && c0 + c + j * 8 < g.cols) {
               float y[8];
 #pragma unroll
-              for (int e = 0; e < 8; ++e) y[e] = __uint_as_float(i < 2 ? r0[i * 8 + e] : r1[(i - 2) * 8 + e]);
-              store8<T>(o + c + i * 8, y);
+              for (int e = 0; e < 8; ++e) y[e] = __uint_as_float(j < 2 ? r0[j * 8 + e] : r1[(j - 2) * 8 + e]);
+              store8<T>(out + c0 + c + j * 8, y);
             }
         }
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&acc_empty[ab]);
+      if (lane == 0) mbar_arrive_cluster(freed[ab]);
     }
   }
   tc_fence_before();
   __syncthreads();
+  cluster_sync_all();  // neither CTA leaves while the other's MMAs or arrivals may reach it
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc(tmem, 512);
+    tmem_dealloc_pair(tmem, 512);
   }
 }
 
@@ -380,20 +458,58 @@ cudaError_t few_t(const SwigluArgs& s, cudaStream_t st) {
   return cudaGetLastError();
 }
 
-template <typename T, int MODE>
-cudaError_t gemm_t(GemmArgs& a, int dtype, cudaStream_t st) {
-  constexpr bool GATE = MODE == kGateForward || MODE == kGateBackward;
-  a.tiles_m = static_cast<int>((a.M + kGmM - 1) / kGmM);
-  a.tiles_n = GATE ? ceil_div_i(a.cols, 128) : ceil_div_i(a.cols, kGmN);
-  a.idesc = umma_idesc_f16(dtype == ATTNRES_DTYPE_BF16, MODE == kGradWeight, !GATE, kGmM, kGmN);
-  const void* fn = reinterpret_cast<const void*>(&swiglu_gemm_kernel<T, MODE>);
-  cudaError_t e = ensure_dynamic_smem(fn, static_cast<int>(kGmSmem));
-  int nsm = 0;
-  if (e == cudaSuccess) e = cached_sm_count(&nsm);
+// Time of a list of tiles on P pairs, in units of 512 cycles: a step of 64 columns of a
+// 256 x 256 tile is 1, of a 256 x 128 tile (half the products, 3/4 of the loads) 0.75, and
+// a tile's start and end that no other tile hides about 8.
+double tiles_cost(const GemmJob& g, int BN, bool gate, int P) {
+  const int n = gate ? ceil_div_i(g.cols, BN / 2) : ceil_div_i(g.cols, BN);
+  const long long tiles = static_cast<long long>((g.M + kGmM - 1) / kGmM) * n;
+  return static_cast<double>((tiles + P - 1) / P) * g.ksteps * (BN == 256 ? 1.0 : 0.75) + 8.0;
+}
+
+template <typename T, int MODE, int BN>
+cudaError_t gemm_bn(GemmArgs& a, int dtype, int pairs, cudaStream_t st) {
+  constexpr bool GATE = MODE != kGradients;
+  long long tiles = 0;
+  int count[2] = {0, 0};
+  for (int i = 0; i < 2; ++i) {
+    GemmJob& g = a.job[i];
+    if (!g.out) continue;  // not wanted: no tiles
+    g.tiles_m = static_cast<int>((g.M + kGmM - 1) / kGmM);
+    g.tiles_n = GATE ? ceil_div_i(g.cols, BN / 2) : ceil_div_i(g.cols, BN);
+    g.idesc = umma_idesc_f16(dtype == ATTNRES_DTYPE_BF16, !GATE && i == 0, !GATE, kGmM, BN);
+    count[i] = g.tiles_m * g.tiles_n;
+    tiles += count[i];
+  }
+  const int P = static_cast<int>(std::min<long long>(tiles, pairs));
+  if (MODE == kGradients && count[1] > 0) {
+    // the split of the dx tiles that ends soonest
+    a.more = count[0] % P;
+    const double k0 = a.job[0].ksteps, k1 = a.job[1].ksteps, base = count[0] / P * k0;
+    double best = -1.0;
+    const int most = a.more > 0 ? (count[1] + a.more - 1) / a.more : 0;
+    for (int x = 0; x <= most; ++x) {
+      const int left = std::max(0, count[1] - a.more * x), y = (left + P - a.more - 1) / (P - a.more);
+      const double end = std::max(a.more > 0 ? base + k0 + x * k1 : 0.0, base + y * k1);
+      if (best < 0.0 || end < best) {
+        best = end;
+        a.x = x;
+        a.y = y;
+      }
+    }
+  }
+  const void* fn = reinterpret_cast<const void*>(&swiglu_gemm_kernel<T, MODE, BN>);
+  const cudaError_t e = ensure_dynamic_smem(fn, static_cast<int>(kGmSmem));
   if (e != cudaSuccess) return e;
-  const int grid = std::min(a.tiles_m * a.tiles_n, nsm);
-  swiglu_gemm_kernel<T, MODE><<<grid, kGmThreads, kGmSmem, st>>>(a);
+  swiglu_gemm_kernel<T, MODE, BN><<<2 * P, kGmThreads, kGmSmem, st>>>(a);
   return cudaGetLastError();
+}
+
+// Operand tiles of both widths read boxes of 64 rows or columns of B, so the maps do not
+// depend on the width; the gate modes' boxes are BN / 2 rows.
+template <typename T, int MODE>
+cudaError_t gemm_t(GemmArgs& a, int dtype, int pairs, bool wide, cudaStream_t st) {
+  return wide ? gemm_bn<T, MODE, 256>(a, dtype, pairs, st) : gemm_bn<T, MODE, 128>(a, dtype, pairs, st);
 }
 
 constexpr cudaError_t kNoTensorMap = cudaErrorInvalidValue;
@@ -408,56 +524,77 @@ bool map(CUtensorMap* m, int dtype, const void* p, long long rows, int cols, lon
   return encode_2d(m, dtype, p, rows, cols, stride, box_rows);
 }
 
+// Pairs of CTAs that are resident at once (one CTA an SM; a group of SMs with an odd one
+// leaves it out): a persistent launch of more would queue the rest behind all the work.
+cudaError_t pair_count(int* pairs) {
+  const void* fn = reinterpret_cast<const void*>(&swiglu_gemm_kernel<__nv_bfloat16, kGateForward, 256>);
+  cudaError_t e = ensure_dynamic_smem(fn, static_cast<int>(kGmSmem));
+  if (e == cudaSuccess) e = cached_max_clusters(pairs, fn, 2, kGmThreads, kGmSmem);
+  if (e == cudaSuccess && *pairs < 1) e = cudaErrorInvalidConfiguration;
+  return e;
+}
+
 template <typename T>
 cudaError_t gate_t(const SwigluArgs& s, bool backward, int dtype, cudaStream_t st) {
+  int pairs = 0;
+  const cudaError_t e = pair_count(&pairs);
+  if (e != cudaSuccess) return e;
   GemmArgs a{};
+  GemmJob& g = a.job[0];
+  g.M = s.N;
+  g.cols = s.F;
+  g.ksteps = ceil_div_i(s.C, kGmK);
+  const bool wide = tiles_cost(g, 256, true, pairs) <= tiles_cost(g, 128, true, pairs);
   const T* w = static_cast<const T*>(s.w);
-  if (!map(&a.a, dtype, s.x, s.N, s.C, s.x_stride, kGmM) || !map(&a.b, dtype, w, s.F, s.C, s.w_stride, 128) ||
-      !map(&a.b2, dtype, w + s.F * s.w_stride, s.F, s.C, s.w_stride, 128))
+  if (!map(&g.a, dtype, s.x, s.N, s.C, s.x_stride, 128) || !map(&g.b, dtype, w, s.F, s.C, s.w_stride, wide ? 128 : 64) ||
+      !map(&g.b2, dtype, w + s.F * s.w_stride, s.F, s.C, s.w_stride, wide ? 128 : 64))
     return kNoTensorMap;
-  a.M = s.N;
-  a.cols = s.F;
-  a.ksteps = ceil_div_i(s.C, kGmK);
   if (!backward) {
-    a.out = s.out;
-    a.out_stride = s.F;
-    return gemm_t<T, kGateForward>(a, dtype, st);
+    g.out = s.out;
+    g.out_stride = s.F;
+    return gemm_t<T, kGateForward>(a, dtype, pairs, wide, st);
   }
-  a.out = s.workspace;
-  a.out_stride = 2LL * s.F;
+  g.out = s.workspace;
+  g.out_stride = 2LL * s.F;
   a.dh = s.dh;
   a.dh_stride = s.dh_stride;
-  return gemm_t<T, kGateBackward>(a, dtype, st);
+  return gemm_t<T, kGateBackward>(a, dtype, pairs, wide, st);
 }
 
 template <typename T>
 cudaError_t backward_t(const SwigluArgs& s, int dtype, cudaStream_t st) {
   cudaError_t e = gate_t<T>(s, true, dtype, st);
   if (e != cudaSuccess) return e;
+  int pairs = 0;
+  if ((e = pair_count(&pairs)) != cudaSuccess) return e;
   const int F2 = 2 * s.F;
-  if (s.dx) {
-    GemmArgs a{};
-    if (!map(&a.a, dtype, s.workspace, s.N, F2, F2, kGmM) || !map(&a.b, dtype, s.w, F2, s.C, s.w_stride, kGmK))
-      return kNoTensorMap;
-    a.out = s.dx;
-    a.out_stride = s.C;
-    a.M = s.N;
-    a.cols = s.C;
-    a.ksteps = ceil_div_i(F2, kGmK);
-    if ((e = gemm_t<T, kGradInput>(a, dtype, st)) != cudaSuccess) return e;
-  }
+  GemmArgs a{};
+  double cost[2] = {0.0, 0.0};  // of wide and narrow tiles
   if (s.dw) {
-    GemmArgs a{};
-    if (!map(&a.a, dtype, s.workspace, s.N, F2, F2, kGmK) || !map(&a.b, dtype, s.x, s.N, s.C, s.x_stride, kGmK))
+    GemmJob& g = a.job[0];
+    if (!map(&g.a, dtype, s.workspace, s.N, F2, F2, kGmK) || !map(&g.b, dtype, s.x, s.N, s.C, s.x_stride, kGmK))
       return kNoTensorMap;
-    a.out = s.dw;
-    a.out_stride = s.C;
-    a.M = F2;
-    a.cols = s.C;
-    a.ksteps = static_cast<int>((s.N + kGmK - 1) / kGmK);
-    if ((e = gemm_t<T, kGradWeight>(a, dtype, st)) != cudaSuccess) return e;
+    g.out = s.dw;
+    g.out_stride = s.C;
+    g.M = F2;
+    g.cols = s.C;
+    g.ksteps = static_cast<int>((s.N + kGmK - 1) / kGmK);
+    cost[0] += tiles_cost(g, 256, false, pairs);
+    cost[1] += tiles_cost(g, 128, false, pairs);
   }
-  return cudaSuccess;
+  if (s.dx) {
+    GemmJob& g = a.job[1];
+    if (!map(&g.a, dtype, s.workspace, s.N, F2, F2, 128) || !map(&g.b, dtype, s.w, F2, s.C, s.w_stride, kGmK))
+      return kNoTensorMap;
+    g.out = s.dx;
+    g.out_stride = s.C;
+    g.M = s.N;
+    g.cols = s.C;
+    g.ksteps = ceil_div_i(F2, kGmK);
+    cost[0] += tiles_cost(g, 256, false, pairs);
+    cost[1] += tiles_cost(g, 128, false, pairs);
+  }
+  return gemm_t<T, kGradients>(a, dtype, pairs, cost[0] <= cost[1], st);
 }
 
 }  // namespace
