@@ -42,26 +42,27 @@ namespace attnres {
 static __device__ unsigned int g_swiglu_status = 0;
 
 constexpr int kGmM = 256, kGmK = 64;  // rows of a pair's tile, columns of a stage
-constexpr int kGmRing = 6 * 32768;    // bytes of stages
+constexpr int kGmRing = 5 * 32768;    // bytes of stages
+constexpr int kGmBuf = 32 * 128;      // 32 rows x 64 outputs of an epilogue warp; two each
 constexpr int kGmEpiWarps = 8;
 constexpr int kGmThreads = (2 + kGmEpiWarps) * 32;
-constexpr size_t kGmSmem = 1024 + kGmRing + 256;
+constexpr size_t kGmSmem = 1024 + kGmRing + kGmEpiWarps * 2 * kGmBuf + 512;
 
 enum GemmMode { kGateForward, kGateBackward, kGradients };
 
 // One product: out [M, cols] = A B, in tiles of 256 x BN.
 struct GemmJob {
   CUtensorMap a, b, b2;  // b2: the gate rows of the two gate modes
-  void* out;             // h [N, F]; [du dg] [N, 2F]; dW [2F, C]; dx [N, C]
-  long long out_stride, M;
+  CUtensorMap out, out2;  // h [N, F], or du and dg as [N, F] inside [N, 2F]; dW [2F, C]; dx [N, C]
+  bool wanted;
+  long long M;
   int cols;              // columns of the output (gate modes: F)
   int tiles_m, tiles_n, ksteps;
   uint32_t idesc;
 };
 struct GemmArgs {
   GemmJob job[2];  // kGradients: dW, then dx; else one
-  const void* dh;  // gate backward
-  long long dh_stride;
+  CUtensorMap dh;  // gate backward: [N, F]
   // dx tiles of a pair after its dW tiles: x each for the first `more` pairs (which have
   // a dW tile more than the others), y each for the rest
   int more, x, y;
@@ -136,6 +137,11 @@ __device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
 
 __device__ __forceinline__ float sigmoid_fast(float g) { return __fdividef(1.f, 1.f + __expf(-g)); }
 
+// Where 16-byte piece `piece` of row `row` lies in a 128-byte-swizzled buffer.
+__device__ __forceinline__ unsigned char* piece_at(unsigned char* buf, int row, int piece) {
+  return buf + row * 128 + ((piece ^ (row & 7)) << 4);
+}
+
 template <typename T>
 __device__ __forceinline__ void store8(T* p, const float* v) {
   Pack<T, 8> r;
@@ -155,15 +161,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGmThreads, 1)
   constexpr bool GATE = MODE != kGradients;
   constexpr uint32_t kA = 128 * kGmK * 2, kB = BN / 2 * kGmK * 2, kStage = kA + kB;  // bytes, of each CTA
   constexpr int STAGES = kGmRing / kStage, F = BN / 2;                               // F: outputs of a gate tile
+  // 64 columns a chunk; a gate tile of one chunk goes to either half of the epilogue warps in turn
+  constexpr int CHUNKS = GATE ? F / 64 : BN / 64;
+  constexpr bool ALTERNATE = CHUNKS == 1;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* stages =
       reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint64_t* full = reinterpret_cast<uint64_t*>(stages + kGmRing);  // the even CTA's are used
+  unsigned char* bufs = stages + kGmRing;  // [epilogue warps][2] output buffers
+  uint64_t* full = reinterpret_cast<uint64_t*>(bufs + kGmEpiWarps * 2 * kGmBuf);  // the even CTA's are used
   uint64_t* empty = full + STAGES;
   uint64_t* acc_full = empty + STAGES;
   uint64_t* acc_empty = acc_full + 2;  // the even CTA's are used
   uint64_t* done = acc_empty + 2;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
+  uint64_t* dh_full = done + 1;  // [epilogue warps]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(dh_full + kGmEpiWarps);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = cluster_rank(), pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
@@ -175,9 +186,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGmThreads, 1)
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&acc_full[i], 1);
-      mbar_init(&acc_empty[i], 2 * kGmEpiWarps);
+      mbar_init(&acc_empty[i], 2 * (ALTERNATE ? kGmEpiWarps / 2 : kGmEpiWarps));
     }
     mbar_init(done, 1);
+    for (int i = 0; i < kGmEpiWarps; ++i) mbar_init(&dh_full[i], 1);
     *abort_flag = 0;
     fence_mbar_init();
   }
@@ -279,44 +291,59 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGmThreads, 1)
       if (issued_any && !mbar_wait_bounded(done, 0)) atomicOr(&g_swiglu_status, kStatusDrainTimeout);
     }
   } else {
-    // ---------------- epilogue: one accumulator row a thread, half the columns a warp
+    // ---------------- epilogue: one accumulator row a thread, 64 columns at a time ----
+    // into the warp's swizzled buffers, which TMA stores from (rows and columns past the
+    // end are dropped there); dh comes the same way, a tile ahead.
     const int q = warp & 3, half = (warp - 2) >> 2;
     const uint32_t lane_off = static_cast<uint32_t>(q * 32) << 16;
     const uint32_t freed[2] = {map_to_rank(smem_u32(&acc_empty[0]), 0), map_to_rank(smem_u32(&acc_empty[1]), 0)};
-    for (int i = 0;; ++i) {
-      const TileRef t = tile_of<MODE>(a, pair, pairs, i);
-      if (t.job < 0) break;
+    unsigned char* buf0 = bufs + (warp - 2) * 2 * kGmBuf;
+    unsigned char* buf1 = buf0 + kGmBuf;
+    uint64_t* dh_bar = &dh_full[warp - 2];
+    const int row0 = rank * 128 + q * 32, step = ALTERNATE ? 2 : 1;
+    auto fetch_dh = [&](const TileRef& t) {  // lane 0, once buf0 is free
+      mbar_arrive_expect_tx(dh_bar, kGmBuf);
+      tma_load_2d(buf0, &a.dh, t.n * F + (ALTERNATE ? 0 : half * 64), t.m * kGmM + row0, dh_bar);
+    };
+    TileRef t = tile_of<MODE>(a, pair, pairs, ALTERNATE ? half : 0);
+    if (MODE == kGateBackward && t.job >= 0 && lane == 0) fetch_dh(t);
+    uint32_t dh_phase = 0;
+    bool dh_pending = MODE == kGateBackward && t.job >= 0;
+    for (int i = ALTERNATE ? half : 0; t.job >= 0; i += step) {
       const GemmJob& g = a.job[t.job];
       const int ab = i & 1;
-      if (*abort_flag || !mbar_wait_bounded(&acc_full[ab], static_cast<uint32_t>((i >> 1) & 1))) {
+      bool ok = !*abort_flag && mbar_wait_bounded(&acc_full[ab], static_cast<uint32_t>((i >> 1) & 1));
+      if (MODE == kGateBackward && ok) {
+        ok = mbar_wait_bounded(dh_bar, dh_phase);
+        if (ok) {
+          dh_pending = false;
+          dh_phase ^= 1u;
+        }
+      }
+      if (!__all_sync(0xffffffffu, ok)) {
+        if (lane == 0) atomicOr(&g_swiglu_status, kStatusFullWaitTimeout);
         *abort_flag = 1;
         break;
       }
       tc_fence_after();
-      const long long row = static_cast<long long>(t.m) * kGmM + rank * 128 + q * 32 + lane;
       const uint32_t acc = tmem + lane_off + ab * BN;
-      T* out = static_cast<T*>(g.out) + row * g.out_stride;
+      const int r0 = t.m * kGmM + row0;
+      const TileRef next = tile_of<MODE>(a, pair, pairs, i + step);
       if constexpr (GATE) {
-        const int f0 = t.n * F + half * (F / 2);
-        T* o = out + f0;
-        const T* dh = MODE == kGateBackward ? static_cast<const T*>(a.dh) + row * a.dh_stride + f0 : nullptr;
+        const int chunk = ALTERNATE ? 0 : half;
 #pragma unroll 1
-        for (int c = 0; c < F / 2; c += 16) {
+        for (int c = 0; c < 64; c += 16) {
           uint32_t ur[16], gr[16];
-          tmem_ld16_nowait(acc + half * (F / 2) + c, ur);
-          tmem_ld16_nowait(acc + F + half * (F / 2) + c, gr);
-          Pack<T, 8> d[2];
-          if (MODE == kGateBackward) {
-#pragma unroll
-            for (int j = 0; j < 2; ++j)
-              if (row < g.M && f0 + c + j * 8 < g.cols) d[j] = load_stream<T, 8>(dh + c + j * 8);
-              else d[j] = Pack<T, 8>{};
-          }
+          tmem_ld16_nowait(acc + chunk * 64 + c, ur);
+          tmem_ld16_nowait(acc + F + chunk * 64 + c, gr);
           tmem_ld_wait();
           tmem_regs_ready(ur);
           tmem_regs_ready(gr);
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
+            unsigned char* at = piece_at(buf0, lane, c / 8 + j);
+            Pack<T, 8> d = {};
+            if (MODE == kGateBackward) d = *reinterpret_cast<const Pack<T, 8>*>(at);
             float y[8], z[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
@@ -325,41 +352,73 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGmThreads, 1)
               if (MODE == kGateForward) {
                 y[e] = u * silu;
               } else {
-                const float dhe = Elem<T>::to_f(d[j].e[e]);
+                const float dhe = Elem<T>::to_f(d.e[e]);
                 y[e] = dhe * silu;
                 z[e] = dhe * u * (s + silu * (1.f - s));
               }
             }
-            if (row < g.M && f0 + c + j * 8 < g.cols) {
-              store8<T>(o + c + j * 8, y);
-              if (MODE == kGateBackward) store8<T>(o + g.cols + c + j * 8, z);
-            }
+            store8<T>(reinterpret_cast<T*>(at), y);
+            if (MODE == kGateBackward) store8<T>(reinterpret_cast<T*>(piece_at(buf1, lane, c / 8 + j)), z);
           }
         }
+        tc_fence_before();
+        fence_async_shared();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive_cluster(freed[ab]);
+          const int c0 = t.n * F + chunk * 64;
+          if (c0 < g.cols && r0 < g.M) {
+            tma_store_2d(&g.out, c0, r0, buf0);
+            if (MODE == kGateBackward) tma_store_2d(&g.out2, c0, r0, buf1);
+          }
+          bulk_commit_group();
+          bulk_wait_group_read0();
+          if (MODE == kGateBackward && next.job >= 0) fetch_dh(next);
+        }
+        if (MODE == kGateBackward) dh_pending = next.job >= 0;
+        __syncwarp();
       } else {
-        const int c0 = t.n * BN + half * (BN / 2);
 #pragma unroll 1
-        for (int c = 0; c < BN / 2; c += 32) {
-          uint32_t r0[16], r1[16];
-          tmem_ld16_nowait(acc + half * (BN / 2) + c, r0);
-          tmem_ld16_nowait(acc + half * (BN / 2) + c + 16, r1);
-          tmem_ld_wait();
-          tmem_regs_ready(r0);
-          tmem_regs_ready(r1);
+        for (int k = 0; k < CHUNKS / 2; ++k) {
+          const int chunk = half * (CHUNKS / 2) + k;
+          unsigned char* buf = k & 1 ? buf1 : buf0;
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
-            if (row < g.M && c0 + c + j * 8 < g.cols) {
+          for (int c = 0; c < 64; c += 32) {
+            uint32_t r[2][16];
+            tmem_ld16_nowait(acc + chunk * 64 + c, r[0]);
+            tmem_ld16_nowait(acc + chunk * 64 + c + 16, r[1]);
+            tmem_ld_wait();
+            tmem_regs_ready(r[0]);
+            tmem_regs_ready(r[1]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
               float y[8];
 #pragma unroll
-              for (int e = 0; e < 8; ++e) y[e] = __uint_as_float(j < 2 ? r0[j * 8 + e] : r1[(j - 2) * 8 + e]);
-              store8<T>(out + c0 + c + j * 8, y);
+              for (int e = 0; e < 8; ++e) y[e] = __uint_as_float(r[j >> 1][(j & 1) * 8 + e]);
+              store8<T>(reinterpret_cast<T*>(piece_at(buf, lane, c / 8 + j)), y);
             }
+          }
+          if (k == CHUNKS / 2 - 1) tc_fence_before();
+          fence_async_shared();
+          __syncwarp();
+          if (lane == 0) {
+            if (k == CHUNKS / 2 - 1) mbar_arrive_cluster(freed[ab]);
+            const int c0 = t.n * BN + chunk * 64;
+            if (c0 < g.cols && r0 < g.M) tma_store_2d(&g.out, c0, r0, buf);
+            bulk_commit_group();
+            if (k == CHUNKS / 2 - 1) bulk_wait_group_read0();  // both buffers free for the next tile
+          }
+          __syncwarp();
         }
       }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive_cluster(freed[ab]);
+      t = next;
     }
+    if (lane == 0) {
+      // a load of dh still in flight lands before the CTA's shared memory is given away
+      if (dh_pending && !mbar_wait_bounded(dh_bar, dh_phase)) atomicOr(&g_swiglu_status, kStatusDrainTimeout);
+      bulk_wait_group0();
+    }
+    __syncwarp();
   }
   tc_fence_before();
   __syncthreads();
@@ -474,7 +533,7 @@ cudaError_t gemm_bn(GemmArgs& a, int dtype, int pairs, cudaStream_t st) {
   int count[2] = {0, 0};
   for (int i = 0; i < 2; ++i) {
     GemmJob& g = a.job[i];
-    if (!g.out) continue;  // not wanted: no tiles
+    if (!g.wanted) continue;  // no tiles
     g.tiles_m = static_cast<int>((g.M + kGmM - 1) / kGmM);
     g.tiles_n = GATE ? ceil_div_i(g.cols, BN / 2) : ceil_div_i(g.cols, BN);
     g.idesc = umma_idesc_f16(dtype == ATTNRES_DTYPE_BF16, !GATE && i == 0, !GATE, kGmM, BN);
@@ -549,15 +608,15 @@ cudaError_t gate_t(const SwigluArgs& s, bool backward, int dtype, cudaStream_t s
   if (!map(&g.a, dtype, s.x, s.N, s.C, s.x_stride, 128) || !map(&g.b, dtype, w, s.F, s.C, s.w_stride, wide ? 128 : 64) ||
       !map(&g.b2, dtype, w + s.F * s.w_stride, s.F, s.C, s.w_stride, wide ? 128 : 64))
     return kNoTensorMap;
+  g.wanted = true;
   if (!backward) {
-    g.out = s.out;
-    g.out_stride = s.F;
+    if (!map(&g.out, dtype, s.out, s.N, s.F, s.F, 32)) return kNoTensorMap;
     return gemm_t<T, kGateForward>(a, dtype, pairs, wide, st);
   }
-  g.out = s.workspace;
-  g.out_stride = 2LL * s.F;
-  a.dh = s.dh;
-  a.dh_stride = s.dh_stride;
+  T* d = static_cast<T*>(s.workspace);
+  if (!map(&g.out, dtype, d, s.N, s.F, 2LL * s.F, 32) || !map(&g.out2, dtype, d + s.F, s.N, s.F, 2LL * s.F, 32) ||
+      !map(&a.dh, dtype, s.dh, s.N, s.F, s.dh_stride, 32))
+    return kNoTensorMap;
   return gemm_t<T, kGateBackward>(a, dtype, pairs, wide, st);
 }
 
@@ -572,10 +631,10 @@ cudaError_t backward_t(const SwigluArgs& s, int dtype, cudaStream_t st) {
   double cost[2] = {0.0, 0.0};  // of wide and narrow tiles
   if (s.dw) {
     GemmJob& g = a.job[0];
-    if (!map(&g.a, dtype, s.workspace, s.N, F2, F2, kGmK) || !map(&g.b, dtype, s.x, s.N, s.C, s.x_stride, kGmK))
+    if (!map(&g.a, dtype, s.workspace, s.N, F2, F2, kGmK) || !map(&g.b, dtype, s.x, s.N, s.C, s.x_stride, kGmK) ||
+        !map(&g.out, dtype, s.dw, F2, s.C, s.C, 32))
       return kNoTensorMap;
-    g.out = s.dw;
-    g.out_stride = s.C;
+    g.wanted = true;
     g.M = F2;
     g.cols = s.C;
     g.ksteps = static_cast<int>((s.N + kGmK - 1) / kGmK);
@@ -584,10 +643,10 @@ cudaError_t backward_t(const SwigluArgs& s, int dtype, cudaStream_t st) {
   }
   if (s.dx) {
     GemmJob& g = a.job[1];
-    if (!map(&g.a, dtype, s.workspace, s.N, F2, F2, 128) || !map(&g.b, dtype, s.w, F2, s.C, s.w_stride, kGmK))
+    if (!map(&g.a, dtype, s.workspace, s.N, F2, F2, 128) || !map(&g.b, dtype, s.w, F2, s.C, s.w_stride, kGmK) ||
+        !map(&g.out, dtype, s.dx, s.N, s.C, s.C, 32))
       return kNoTensorMap;
-    g.out = s.dx;
-    g.out_stride = s.C;
+    g.wanted = true;
     g.M = s.N;
     g.cols = s.C;
     g.ksteps = ceil_div_i(F2, kGmK);
