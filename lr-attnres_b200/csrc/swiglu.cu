@@ -155,6 +155,29 @@ __device__ __forceinline__ void store8(T* p, const float* v) {
   *reinterpret_cast<Pack<T, 8>*>(p) = r;
 }
 
+// The ring's waits. The producer and the issuer are one thread each and every cycle of
+// their loops counts (a stage of a narrow tile is 256 cycles of products), so the usual
+// case is one test and nothing else; only a wait that has to go on looks at the abort
+// flag and the clock.
+__device__ __forceinline__ bool ring_test(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.acquire.cta.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+__device__ __forceinline__ bool ring_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+  if (ring_test(bar, parity)) return true;
+  const unsigned long long t0 = global_timer_ns();
+  while (!ring_test(bar, parity))
+    if (*abort_flag || global_timer_ns() - t0 > kWaitLimitNs) return ring_test(bar, parity);
+  return true;
+}
+
 template <typename T, int MODE, int BN>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGmThreads, 1)
     swiglu_gemm_kernel(const __grid_constant__ GemmArgs a) {
@@ -203,16 +226,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGmThreads, 1)
   if (warp == 0) {
     // ---------------- TMA producer: this CTA's half of each stage ------------------
     if (lane == 0) {
-      long long it = 0;
+      const uint32_t full0 = map_to_rank(smem_u32(full), 0), empty0 = smem_u32(empty);
+      int st = 0;
+      long long posted = 0;
+      uint32_t phase = 1;  // an untouched barrier's previous phase counts as done
       bool ok = true;
       for (int i = 0; ok; ++i) {
         const TileRef t = tile_of<MODE>(a, pair, pairs, i);
         if (t.job < 0) break;
         const GemmJob& g = a.job[t.job];
-        const int m0 = t.m * kGmM + rank * 128;
-        for (int kc = 0; kc < g.ksteps; ++kc, ++it) {
-          const int st = static_cast<int>(it % STAGES);
-          if (*abort_flag || !mbar_wait_bounded(&empty[st], static_cast<uint32_t>((it / STAGES) & 1) ^ 1u)) {
+        const int m0 = t.m * kGmM + rank * 128, n0 = GATE ? t.n * F : t.n * BN + rank * (BN / 2);
+        const CUtensorMap* const bmap = GATE && rank ? &g.b2 : &g.b;
+        const int k_end = g.ksteps * kGmK;
+        for (int k = 0; k < k_end; k += kGmK) {
+          if (!ring_wait(empty0 + 8 * st, phase, abort_flag)) {
             atomicOr(&g_swiglu_status, kStatusEmptyWaitTimeout);
             *abort_flag = 1;
             ok = false;
@@ -221,26 +248,30 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGmThreads, 1)
           unsigned char* sa = stages + st * kStage;
           unsigned char* sb = sa + kA;
           if (rank == 0) mbar_arrive_expect_tx(&full[st], 2 * kStage);
-          const uint32_t bar = map_to_rank(smem_u32(&full[st]), 0);
+          const uint32_t bar = full0 + 8 * st;
           if (GATE) {
-            tma_load_2d_pair(sa, &g.a, kc * kGmK, m0, bar);
-            tma_load_2d_pair(sb, rank == 0 ? &g.b : &g.b2, kc * kGmK, t.n * F, bar);
+            tma_load_2d_pair(sa, &g.a, k, m0, bar);
+            tma_load_2d_pair(sb, bmap, k, n0, bar);
           } else {
             if (t.job == 0) {  // dW: rows of A are columns of [du dg]
-              tma_load_2d_pair(sa, &g.a, m0, kc * kGmK, bar);
-              tma_load_2d_pair(sa + 64 * 128, &g.a, m0 + 64, kc * kGmK, bar);
+              tma_load_2d_pair(sa, &g.a, m0, k, bar);
+              tma_load_2d_pair(sa + 64 * 128, &g.a, m0 + 64, k, bar);
             } else {
-              tma_load_2d_pair(sa, &g.a, kc * kGmK, m0, bar);
+              tma_load_2d_pair(sa, &g.a, k, m0, bar);
             }
 #pragma unroll
-            for (int j = 0; j < BN / 128; ++j)
-              tma_load_2d_pair(sb + j * 64 * 128, &g.b, t.n * BN + rank * (BN / 2) + j * 64, kc * kGmK, bar);
+            for (int j = 0; j < BN / 128; ++j) tma_load_2d_pair(sb + j * 64 * 128, bmap, n0 + j * 64, k, bar);
+          }
+          ++posted;
+          if (++st == STAGES) {
+            st = 0;
+            phase ^= 1u;
           }
         }
       }
       if (!ok && rank == 0) {
         // stages that were posted land in both CTAs before either goes on to exit
-        for (long long j = (it > STAGES ? it - STAGES : 0); j < it; ++j)
+        for (long long j = (posted > STAGES ? posted - STAGES : 0); j < posted; ++j)
           if (!mbar_wait_bounded(&full[j % STAGES], static_cast<uint32_t>((j / STAGES) & 1)))
             atomicOr(&g_swiglu_status, kStatusDrainTimeout);
       }
@@ -248,7 +279,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGmThreads, 1)
   } else if (warp == 1) {
     // ---------------- MMA issuer of the pair ---------------------------------------
     if (lane == 0 && rank == 0) {
-      long long it = 0;
+      const uint32_t full0 = smem_u32(full);
+      // K = 16 an instruction: 32 bytes on in a K-major tile, two groups of 8 rows (2048
+      // bytes) in an MN-major one
+      const uint64_t k_major = umma_desc_sw128(stages), mn_major = umma_desc_sw128_mn(stages, 64 * 128);
+      constexpr uint64_t kStageStep = kStage >> 4;
+      const uint64_t b0 = (GATE ? k_major : mn_major) + (kA >> 4);
+      constexpr uint64_t b_step = GATE ? 2 : 128;
+      int st = 0;
+      uint32_t phase = 0;
       bool issued_any = false, ok = true;
       for (int i = 0; ok; ++i) {
         const TileRef t = tile_of<MODE>(a, pair, pairs, i);
@@ -261,29 +300,27 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGmThreads, 1)
           break;
         }
         tc_fence_after();
-        const uint32_t acc = tmem + ab * BN;
+        const uint32_t acc = tmem + ab * BN, idesc = g.idesc;
         const bool a_mn = !GATE && t.job == 0;
-        for (int kc = 0; kc < g.ksteps; ++kc, ++it) {
-          const int st = static_cast<int>(it % STAGES);
-          if (*abort_flag || !mbar_wait_bounded(&full[st], static_cast<uint32_t>((it / STAGES) & 1))) {
+        const uint64_t a0 = a_mn ? mn_major : k_major, a_step = a_mn ? 128 : 2;
+        for (int k = 0; k < g.ksteps; ++k) {
+          if (!ring_wait(full0 + 8 * st, phase, abort_flag)) {
             atomicOr(&g_swiglu_status, kStatusFullWaitTimeout);
             *abort_flag = 1;
             ok = false;
             break;
           }
           tc_fence_after();
-          const unsigned char* sa = stages + st * kStage;
-          const unsigned char* sb = sa + kA;
-          // K = 16 an instruction: 32 bytes on in a K-major tile, two groups of 8
-          // rows (2048 bytes) in an MN-major one
-          const uint64_t da = a_mn ? umma_desc_sw128_mn(sa, 64 * 128) : umma_desc_sw128(sa);
-          const uint64_t db = GATE ? umma_desc_sw128(sb) : umma_desc_sw128_mn(sb, 64 * 128);
-          const uint64_t da_step = a_mn ? 128 : 2, db_step = GATE ? 2 : 128;
+          const uint64_t da = a0 + st * kStageStep, db = b0 + st * kStageStep;
 #pragma unroll
-          for (int k = 0; k < kGmK / 16; ++k)
-            umma_f16_pair(acc, da + da_step * k, db + db_step * k, g.idesc, (kc > 0 || k > 0) ? 1u : 0u);
+          for (int j = 0; j < kGmK / 16; ++j)
+            umma_f16_pair(acc, da + a_step * j, db + b_step * j, idesc, (k > 0 || j > 0) ? 1u : 0u);
           umma_commit_pair(&empty[st]);
           issued_any = true;
+          if (++st == STAGES) {
+            st = 0;
+            phase ^= 1u;
+          }
         }
         if (ok) umma_commit_pair(&acc_full[ab]);
       }
