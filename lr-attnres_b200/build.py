@@ -85,7 +85,7 @@ def build(verbose=False, force=False):
     os.replace(tmp, OUT)
     tmp = BINDING + ".tmp"
     subprocess.run(["g++", "-shared", "-o", tmp, binding, "-L" + os.path.dirname(OUT), "-l:" + os.path.basename(OUT),
-                    "-Wl,-rpath,$ORIGIN", *("-L" + p for p in torch_paths()[1]), "-lc10", "-lc10_cuda", "-ltorch_cpu",
+                    "-Wl,-rpath,$ORIGIN", *("-L" + p for p in torch_paths()[1]), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda",
                     "-ltorch_python"], check=True)
     os.replace(tmp, BINDING)
     return OUT

@@ -3,6 +3,7 @@
 // step's sizes the same steps in Python and ctypes take several times the kernels'
 // own time (split + norm + rotation of four tokens: 26 us in Python, 3 us on the
 // GPU). Errors are C++ exceptions that pybind11 turns into RuntimeError.
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -43,6 +44,13 @@ void check_device(const char* what, const Tensor& first, const Tensor& t) {
 Tensor or_undefined(const OptTensor& t) { return t.has_value() ? *t : Tensor(); }
 const void* ptr(const Tensor& t) { return t.defined() ? t.const_data_ptr() : nullptr; }
 void* mut(const Tensor& t) { return t.defined() ? t.mutable_data_ptr() : nullptr; }
+
+// An uninitialised tensor on `like`'s device, without the trip through the dispatcher
+// (half the cost of at::empty, and a call makes up to three).
+Tensor fresh(const Tensor& like, at::IntArrayRef shape, at::ScalarType dtype) {
+  return at::detail::empty_cuda(shape, dtype, like.device(), std::nullopt);
+}
+Tensor fresh(const Tensor& like, at::IntArrayRef shape) { return fresh(like, shape, like.scalar_type()); }
 
 // Makes the tensor's device current and hands out its current stream.
 struct Launch {
@@ -126,9 +134,9 @@ struct RopeCall {
 std::vector<Tensor> rope_forward(const Tensor& qkv, const Tensor& cos, const Tensor& sin, const Tensor& positions,
                                  const Tensor& wq, const Tensor& wk, const RopeHow& how) {
   const RopeCall c(qkv, cos, sin, positions, wq, wk, how);
-  const Tensor q = at::empty({c.B, c.T, how.q_heads, c.D}, qkv.options());
-  const Tensor k = at::empty({c.B, c.T, how.kv_heads, c.D}, qkv.options());
-  const Tensor v = at::empty({c.B, c.T, how.kv_heads, c.D}, qkv.options());
+  const Tensor q = fresh(qkv, {c.B, c.T, how.q_heads, c.D});
+  const Tensor k = fresh(qkv, {c.B, c.T, how.kv_heads, c.D});
+  const Tensor v = fresh(qkv, {c.B, c.T, how.kv_heads, c.D});
   const Launch on(c.qkv);
   check_status(attnres_qk_norm_rope_forward(
                    c.tokens(), c.seq(), how.q_heads, how.kv_heads, c.D, 2 * c.cos.size(1), c.code, ptr(c.qkv), c.stride,
@@ -159,15 +167,15 @@ std::vector<Tensor> rope_backward(const std::array<Tensor, 3>& grads, const Tens
     if (g[i].scalar_type() != qkv.scalar_type() || g[i].stride(3) != 1) g[i] = g[i].to(qkv.scalar_type()).contiguous();
     for (int j = 0; j < 3; ++j) strides[3 * i + j] = g[i].stride(j);
   }
-  const Tensor dqkv = at::empty({c.B, c.T, (how.q_heads + 2 * how.kv_heads) * c.D}, qkv.options());
+  const Tensor dqkv = fresh(qkv, {c.B, c.T, (how.q_heads + 2 * how.kv_heads) * c.D});
   Tensor dwq, dwk, workspace;
   size_t bytes = 0;
   if (want_wq || want_wk) {
     const Launch on(c.qkv);
     bytes = attnres_qk_norm_rope_backward_workspace_bytes(c.D);
-    workspace = at::empty({static_cast<int64_t>(bytes)}, qkv.options().dtype(at::kByte));
-    if (want_wq) dwq = at::empty({c.D}, qkv.options());
-    if (want_wk) dwk = at::empty({c.D}, qkv.options());
+    workspace = fresh(qkv, {static_cast<int64_t>(bytes)}, at::kByte);
+    if (want_wq) dwq = fresh(qkv, {c.D});
+    if (want_wk) dwk = fresh(qkv, {c.D});
   }
   const Launch on(c.qkv);
   check_status(attnres_qk_norm_rope_backward(
@@ -238,19 +246,31 @@ py::tuple py_qk_norm_rope_backward(const Tensor& gq, const Tensor& gk, const Ten
 // ---------------------------------------------------------------------------
 // swiglu_projection
 // ---------------------------------------------------------------------------
-// t as [rows, width] with 16-byte aligned rows that do not overlap, copied only if
-// it is not.
-Tensor packed_rows(const Tensor& t, int64_t rows, int64_t width) {
-  Tensor m = t.reshape({rows, width});
-  const int64_t stride = m.size(0) > 1 ? m.stride(0) : width;
-  const bool aligned = reinterpret_cast<uintptr_t>(m.const_data_ptr()) % 16 == 0;
-  if (m.stride(1) == 1 && stride >= width && stride % 8 == 0 && aligned) return m;
-  return m.is_contiguous() ? m.clone() : m.contiguous();
-}
-int64_t row_stride(const Tensor& m) { return m.size(0) > 1 ? m.stride(0) : m.size(1); }
+// t as `rows` rows of `width` elements, 16-byte aligned and one stride apart without
+// overlap; a copy only where it does not lie like that.
+struct Rows {
+  Tensor t;
+  int64_t stride;
+
+  Rows() = default;
+  Rows(const Tensor& from, int64_t rows, int64_t width) : t(from), stride(width) {
+    if (!t.is_contiguous()) {
+      if (t.dim() != 2) t = t.reshape({rows, width});
+      if (rows > 1) stride = t.stride(0);
+      if (t.stride(1) != 1 || stride < width || stride % 8 != 0) {
+        t = t.contiguous();
+        stride = width;
+      }
+    }
+    if (reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 != 0) {
+      t = t.clone(at::MemoryFormat::Contiguous);
+      stride = width;
+    }
+  }
+};
 
 struct SwigluCall {
-  Tensor x, w;
+  Rows x, w;
   int64_t N, C, F;
   int code;
 
@@ -269,8 +289,8 @@ struct SwigluCall {
                 "attnres_b200: swiglu_projection takes widths that are multiples of 8, got in ", C, " and hidden ", F);
     N = x_.numel() / C;
     code = dtype_code(x_);
-    x = packed_rows(x_, N, C);
-    w = packed_rows(w_.to(x_.scalar_type()), 2 * F, C);
+    x = Rows(x_, N, C);
+    w = Rows(w_.to(x_.scalar_type()), 2 * F, C);
   }
 };
 
@@ -282,9 +302,9 @@ std::vector<int64_t> with_last(const Tensor& x, int64_t last) {
 
 Tensor swiglu_forward(const Tensor& x, const Tensor& w) {
   const SwigluCall c(x, w);
-  const Tensor h = at::empty(with_last(x, c.F), x.options());
-  const Launch on(c.x);
-  check_status(attnres_swiglu_forward(c.N, c.C, c.F, c.code, ptr(c.x), row_stride(c.x), ptr(c.w), row_stride(c.w), mut(h),
+  const Tensor h = fresh(x, with_last(x, c.F));
+  const Launch on(c.x.t);
+  check_status(attnres_swiglu_forward(c.N, c.C, c.F, c.code, ptr(c.x.t), c.x.stride, ptr(c.w.t), c.w.stride, mut(h),
                                       on.stream),
                "attnres_swiglu_forward");
   return h;
@@ -296,15 +316,15 @@ std::vector<Tensor> swiglu_backward(const Tensor& grad_h, const Tensor& x, const
   check_device("swiglu_projection", x, grad_h);
   TORCH_CHECK(grad_h.dim() == x.dim() && grad_h.numel() == c.N * c.F && (x.dim() == 0 || grad_h.size(-1) == c.F),
               "attnres_b200: swiglu_projection backward takes a gradient of its output's shape");
-  const Tensor g = packed_rows(grad_h.to(x.scalar_type()), c.N, c.F);
+  const Rows g(grad_h.to(x.scalar_type()), c.N, c.F);
   Tensor dx, dw;
-  if (want_x) dx = at::empty(x.sizes(), x.options());
-  if (want_w) dw = at::empty({2 * c.F, c.C}, x.options());
+  if (want_x) dx = fresh(x, x.sizes());
+  if (want_w) dw = fresh(x, {2 * c.F, c.C});
   const int64_t bytes = attnres_swiglu_backward_workspace_bytes(c.N, c.F);
-  const Tensor workspace = at::empty({bytes}, x.options().dtype(at::kByte));
-  const Launch on(c.x);
-  check_status(attnres_swiglu_backward(c.N, c.C, c.F, c.code, ptr(c.x), row_stride(c.x), ptr(c.w), row_stride(c.w), ptr(g),
-                                       row_stride(g), mut(dx), mut(dw), mut(workspace), bytes, on.stream),
+  const Tensor workspace = fresh(x, {bytes}, at::kByte);
+  const Launch on(c.x.t);
+  check_status(attnres_swiglu_backward(c.N, c.C, c.F, c.code, ptr(c.x.t), c.x.stride, ptr(c.w.t), c.w.stride, ptr(g.t),
+                                       g.stride, mut(dx), mut(dw), mut(workspace), bytes, on.stream),
                "attnres_swiglu_backward");
   if (want_w) dw = dw.to(w.scalar_type());
   return {dx, dw};
@@ -412,8 +432,8 @@ py::tuple py_kv4_read(const Tensor& kc, const Tensor& kp, const Tensor& vc, cons
                       const Tensor& start, int64_t tokens, const OptTensor& counts, at::ScalarType dtype) {
   const PoolCall c("kv4_read", kc, kp, vc, vp, table, start, counts);
   TORCH_CHECK(tokens >= 0 && tokens < (1 << 30), "attnres_b200: kv4_read takes a number of tokens, got ", tokens);
-  const Tensor k = at::empty({c.B, tokens, c.heads, c.D}, kc.options().dtype(dtype));
-  const Tensor v = at::empty({c.B, tokens, c.heads, c.D}, kc.options().dtype(dtype));
+  const Tensor k = fresh(kc, {c.B, tokens, c.heads, c.D}, dtype);
+  const Tensor v = fresh(kc, {c.B, tokens, c.heads, c.D}, dtype);
   const Launch on(kc);
   check_status(attnres_kv4_read(ptr(kc), ptr(kp), ptr(vc), ptr(vp), c.pages, c.heads, c.page, c.D, c.ints(c.table),
                                 c.max_pages, c.max_pages, c.ints(c.per_sequence), c.ints(c.counts), c.B, tokens,
@@ -437,13 +457,13 @@ py::tuple py_kv4_attention(const Tensor& q, const Tensor& kc, const Tensor& kp, 
   const int64_t T = q.size(1), Hq = q.size(2);
   int64_t qs[3];
   const Tensor qr = rows4(what, "q", q, c.B, Hq, c.D, qs);
-  const Tensor out = at::empty({c.B, T, Hq, c.D}, q.options());
+  const Tensor out = fresh(q, {c.B, T, Hq, c.D});
   Tensor lse, workspace;
-  if (want_lse) lse = at::empty({c.B, T, Hq}, q.options().dtype(at::kFloat));
+  if (want_lse) lse = fresh(q, {c.B, T, Hq}, at::kFloat);
   const Launch on(kc);
   const int64_t bytes =
       c.B && T ? attnres_kv4_attention_workspace_bytes(c.heads, c.page, c.D, c.max_pages, c.B, T, Hq) : 0;
-  if (bytes) workspace = at::empty({bytes}, kc.options());
+  if (bytes) workspace = fresh(kc, {bytes}, at::kByte);
   check_status(attnres_kv4_attention(ptr(kc), ptr(kp), ptr(vc), ptr(vp), c.pages, c.heads, c.page, c.D, c.ints(c.table),
                                      c.max_pages, c.max_pages, c.ints(c.per_sequence), c.ints(c.counts), c.B, T, Hq,
                                      dtype_code(qr), ptr(qr), qs, scale, mut(out), static_cast<float*>(mut(lse)),
