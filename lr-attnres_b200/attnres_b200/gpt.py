@@ -17,6 +17,16 @@ kernels (`lrid_attention_residual_read`, `attention_residual_block_summary`,
 `lrid_fused_projection_forward`); `fused=False` uses the reference's PyTorch
 read (model.py:2130-2159) -- the model's unfused path. Everything else
 (attention, GEMMs) is PyTorch.
+
+`fused_layer=True` (16-bit models) also runs the layer around the reads on this
+package's operators: the q/k norm with the rotation and the split into heads as
+one kernel (`qk_norm_rope`) and the MLP up to its output projection as another
+(`swiglu_projection`), in training and inference.
+
+`GPT.generate` continues prompts greedily over a `GPTCache`: keys and values of
+every layer in 4-bit pages (`kv4_append`), attended to by the new tokens
+(`kv4_attention`). A prompt itself is attended to in full precision while it is
+written.
 """
 import math
 from dataclasses import dataclass
@@ -51,6 +61,7 @@ class GPTConfig:
     pad_vocab_to: int = 64
     attn_res_query_init: str = "zero"
     fused: bool = True
+    fused_layer: bool = False
 
     @property
     def hidden_dim(self) -> int:
@@ -79,6 +90,13 @@ class RotaryEmbedding(nn.Module):
         freq = torch.outer(torch.arange(cfg.block_size), inv_freq)
         self.register_buffer("sin", freq.sin()[None, None])
         self.register_buffer("cos", freq.cos()[None, None])
+        # [block_size, head_dim / 2] float32 whatever the module is cast to: what qk_norm_rope takes
+        self.tables = (freq.cos().contiguous(), freq.sin().contiguous())
+
+    def _apply(self, fn, recurse=True):
+        super()._apply(fn, recurse)
+        self.tables = tuple(t.to(self.sin.device) for t in self.tables)  # follow the module's device, not its type
+        return self
 
     def rotate(self, x: Tensor) -> Tensor:
         T = x.size(-2)
@@ -146,24 +164,76 @@ class MultiHeadAttention(nn.Module):
         self.c_attn = nn.Linear(cfg.n_embd, 3 * cfg.n_embd, bias=False)
         self.c_proj = LRIDFusedProjection(cfg, cfg.n_embd, cfg.n_embd)
 
-    def forward(self, x: Tensor):
+    def _heads(self, x: Tensor, positions: Optional[Tensor]):
+        """Queries, keys and values [B, T, heads, head_dim], q and k normed and rotated."""
+        from .layer import qk_norm_rope
+
+        H = self.cfg.n_head
+        return qk_norm_rope(self.c_attn(x), H, H, *self.rope.tables, positions=positions,
+                            normalize=self.cfg.qk_norm)
+
+    def forward(self, x: Tensor, past: Optional["LayerPast"] = None):
         B, T, C = x.shape
-        q, k, v = self.c_attn(x).split(C, dim=2)
-        q, k, v = (t.view(B, T, self.cfg.n_head, self.head_dim).transpose(1, 2) for t in (q, k, v))
-        if self.cfg.qk_norm:
-            q, k = norm(q), norm(k)
-        q, k = self.rope.rotate(q), self.rope.rotate(k)
+        if past is not None:
+            return self.c_proj(past.attend(*self._heads(x, past.positions)).reshape(B, T, C))
+        if self.cfg.fused_layer:
+            q, k, v = (t.transpose(1, 2) for t in self._heads(x, None))
+        else:
+            q, k, v = self.c_attn(x).split(C, dim=2)
+            q, k, v = (t.view(B, T, self.cfg.n_head, self.head_dim).transpose(1, 2) for t in (q, k, v))
+            if self.cfg.qk_norm:
+                q, k = norm(q), norm(k)
+            q, k = self.rope.rotate(q), self.rope.rotate(k)
         y = F.scaled_dot_product_attention(q, k, v, is_causal=True)
         return self.c_proj(y.transpose(1, 2).contiguous().view(B, T, C))
+
+
+class GPTCache:
+    """Keys and values of `batch` sequences of up to `max_tokens` tokens for every layer of a GPT, in
+    4 bits: one pool of pages a layer, one page table for all."""
+
+    def __init__(self, cfg: GPTConfig, batch: int, max_tokens: int, page_size: int = 64, device="cuda"):
+        from .layer import KV4Cache
+
+        if max_tokens > cfg.block_size:
+            raise RuntimeError(f"attnres_b200: GPTCache of {max_tokens} tokens, the model has {cfg.block_size} positions")
+        per = -(-max_tokens // page_size)
+        self.max_tokens, self.used = max_tokens, 0
+        self.pools = [KV4Cache.empty(batch * per, page_size, cfg.n_head, cfg.n_embd // cfg.n_head, device)
+                      for _ in range(cfg.n_layer)]
+        self.page_table = torch.arange(batch * per, device=device, dtype=torch.int32).view(batch, per)
+        self.lengths = torch.zeros(batch, device=device, dtype=torch.int32)
+
+
+class LayerPast:
+    """What a layer's attention takes of a GPTCache for one call: new tokens are written behind the
+    sequences' and attend to all of them (to each other alone, in full precision, while the cache is empty)."""
+
+    def __init__(self, cache: GPTCache, layer: int, positions: Tensor, lengths: Tensor):
+        self.cache, self.pool, self.positions, self.lengths = cache, cache.pools[layer], positions, lengths
+
+    def attend(self, q: Tensor, k: Tensor, v: Tensor) -> Tensor:
+        from .layer import kv4_append, kv4_attention
+
+        kv4_append(self.pool, k, v, self.cache.page_table, self.cache.lengths)
+        if self.cache.used == 0:
+            q, k, v = (t.transpose(1, 2) for t in (q, k, v))
+            return F.scaled_dot_product_attention(q, k, v, is_causal=True).transpose(1, 2)
+        return kv4_attention(q, self.pool, self.cache.page_table, self.lengths)
 
 
 class MLP(nn.Module):
     def __init__(self, cfg: GPTConfig):
         super().__init__()
+        self.cfg = cfg
         self.fc1 = nn.Linear(cfg.n_embd, cfg.hidden_dim * 2, bias=False)
         self.fc2 = LRIDFusedProjection(cfg, cfg.hidden_dim, cfg.n_embd)
 
     def forward(self, x: Tensor):
+        if self.cfg.fused_layer:
+            from .layer import swiglu_projection
+
+            return self.fc2(swiglu_projection(x, self.fc1.weight))
         x, gate = self.fc1(x).chunk(2, dim=-1)
         return self.fc2(F.silu(gate) * x)
 
@@ -175,16 +245,16 @@ class Block(nn.Module):
         self.attn = MultiHeadAttention(cfg)
         self.mlp = MLP(cfg)
 
-    def _sublayer(self, f, x: Tensor, x_is_normalized: bool):
+    def _sublayer(self, f, x: Tensor, x_is_normalized: bool, *args):
         if self.cfg.norm_pos == "before" and not x_is_normalized:
             x = norm(x)
-        out, key = f(x)
+        out, key = f(x, *args)
         if self.cfg.norm_pos == "after":
             out = norm(out)
         return out, key
 
-    def forward_attention(self, x, x_is_normalized=False):
-        return self._sublayer(self.attn, x, x_is_normalized)
+    def forward_attention(self, x, x_is_normalized=False, past=None):
+        return self._sublayer(self.attn, x, x_is_normalized, past)
 
     def forward_mlp(self, x, x_is_normalized=False):
         return self._sublayer(self.mlp, x, x_is_normalized)
@@ -256,9 +326,19 @@ class GPT(nn.Module):
                                                  c.attnres_key_norm, source_logit_biases=biases)
         return norm(out) if normalize_output else out
 
-    def forward(self, idx: Tensor, return_hidden: bool = False) -> Tensor:
+    def forward(self, idx: Tensor, return_hidden: bool = False, cache: Optional[GPTCache] = None) -> Tensor:
+        """Logits [B, T, vocab] (or the normed hidden states). With a cache the tokens are the next
+        ones of its sequences, and are in it afterwards (no gradient)."""
         c = self.cfg
         x = self.transformer.wte(idx)
+        pasts = [None] * c.n_layer
+        if cache is not None:
+            T = idx.size(1)
+            if cache.used + T > cache.max_tokens:
+                raise RuntimeError(f"attnres_b200: the cache holds {cache.used} of {cache.max_tokens} tokens, {T} more do not fit")
+            positions = cache.lengths[:, None] + torch.arange(T, device=idx.device, dtype=torch.int32)
+            lengths = cache.lengths + T
+            pasts = [LayerPast(cache, li, positions, lengths) for li in range(c.n_layer)]
         fused_read_norm = (c.fused and c.norm_pos == "before" and c.attnres_fuse_read_norm
                            and c.lrid_num_heads == 1)  # model.py:2237-2243
         # completed block sources (value, key) and their counts; the live block
@@ -275,10 +355,13 @@ class GPT(nn.Module):
             return self._read(site, v, k, self._biases(n), fused_read_norm)
 
         for li, block in enumerate(self.transformer.layers):
-            for sub, f in ((0, block.forward_attention), (1, block.forward_mlp)):
+            for sub in (0, 1):
                 site = 2 * li + sub
                 x = read(site) if site > 0 else (norm(x) if fused_read_norm else x)
-                out, key = f(x, x_is_normalized=fused_read_norm)
+                if sub == 0:
+                    out, key = block.forward_attention(x, x_is_normalized=fused_read_norm, past=pasts[li])
+                else:
+                    out, key = block.forward_mlp(x, x_is_normalized=fused_read_norm)
                 part_n += 1
                 part, part_src = self._summary(part, out, part_n)
                 part_key = key if part_n == 1 else part_key + key
@@ -290,7 +373,24 @@ class GPT(nn.Module):
         x = read(2 * c.n_layer)
         if not fused_read_norm:
             x = norm(x)
+        if cache is not None:
+            cache.lengths = lengths
+            cache.used += T
         return x if return_hidden else self.logits(x)
+
+    @torch.no_grad()
+    def generate(self, idx: Tensor, new_tokens: int, cache: Optional[GPTCache] = None) -> Tensor:
+        """The prompts idx [B, T] with `new_tokens` tokens appended to each, the likeliest at every
+        step. Pass a cache to go on from it later; the last token chosen is not in it yet."""
+        if new_tokens < 1:
+            return idx
+        if cache is None:
+            cache = GPTCache(self.cfg, idx.size(0), idx.size(1) + new_tokens - 1, device=idx.device)
+        out, step = [idx], idx
+        for _ in range(new_tokens):
+            step = self.logits(self(step, return_hidden=True, cache=cache)[:, -1:]).argmax(-1)
+            out.append(step)
+        return torch.cat(out, dim=1)
 
     def logits(self, x: Tensor) -> Tensor:
         """lm_head(x). With a vocabulary that is not a multiple of
