@@ -17,7 +17,8 @@
 //           2^-24 of the largest. z = step * sum_d q_d n_d + low Q, Q the sum of the
 //           group's q: exact products, fp32 sums
 //   output  0x6400 | n is 1024 + n and 0x5400 | n << 4 is 64 + n; the difference to 1024 or
-//           64 is exact, step n + low is rounded once, weights (0 to 1) are too
+//           64 is exact, step n + low is rounded once, weights are too (f16 outputs: to twice
+//           the bits)
 // The row of a key is an accumulator's row and a value's column: weights change sides
 // by movmatrix. Keys are taken in the order i ^ ((i >> 1) & 1) so that lanes that differ
 // in their keys read different halves of the banks.
@@ -394,11 +395,21 @@ __global__ void __launch_bounds__(kAtWarps * 32, NT == 1 ? (D == 64 ? 5 : 3) : 2
               if (odd && z[mt][j][2 * e + r] > 0.f) l[j][r] = __int_as_float(0x7fffffff);
         }
       }
-      uint32_t pa[NT], pb[NT];
+      // the weights in f16; for f16 outputs also what that rounding left, as a second product:
+      // the value's and the output's own roundings are of the same size there
+      constexpr int PARTS = std::is_same<T, __half>::value ? 2 : 1;
+      uint32_t pa[PARTS][NT], pb[PARTS][NT];
 #pragma unroll
       for (int j = 0; j < NT; ++j) {
-        pa[j] = transposed(half_pack(z[mt][j][0], z[mt][j][1]));
-        pb[j] = transposed(half_pack(z[mt][j][2], z[mt][j][3]));
+        const uint32_t a0 = half_pack(z[mt][j][0], z[mt][j][1]), b0 = half_pack(z[mt][j][2], z[mt][j][3]);
+        pa[0][j] = transposed(a0);
+        pb[0][j] = transposed(b0);
+        if constexpr (PARTS == 2) {
+          const float2 a1 = __half22float2(*reinterpret_cast<const __half2*>(&a0));
+          const float2 b1 = __half22float2(*reinterpret_cast<const __half2*>(&b0));
+          pa[1][j] = transposed(half_pack(z[mt][j][0] - a1.x, z[mt][j][1] - a1.y));
+          pb[1][j] = transposed(half_pack(z[mt][j][2] - b1.x, z[mt][j][3] - b1.y));
+        }
       }
 #pragma unroll
       for (int i = 0; i < G; ++i) {
@@ -414,10 +425,12 @@ __global__ void __launch_bounds__(kAtWarps * 32, NT == 1 ? (D == 64 ? 5 : 3) : 2
             f[e][k] = half_fma(half_sub(code_bits(w, k) | code_off(k), code_off(k)), step, low);
         }
 #pragma unroll
-        for (int j = 0; j < NT; ++j) {
-          mma_16816<__half>(o[j][2 * i], f[0][0], f[0][1], f[1][0], f[1][1], pa[j], pb[j]);
-          mma_16816<__half>(o[j][2 * i + 1], f[0][2], f[0][3], f[1][2], f[1][3], pa[j], pb[j]);
-        }
+        for (int part = 0; part < PARTS; ++part)
+#pragma unroll
+          for (int j = 0; j < NT; ++j) {
+            mma_16816<__half>(o[j][2 * i], f[0][0], f[0][1], f[1][0], f[1][1], pa[part][j], pb[part][j]);
+            mma_16816<__half>(o[j][2 * i + 1], f[0][2], f[0][3], f[1][2], f[1][3], pa[part][j], pb[part][j]);
+          }
       }
     }
   };
