@@ -174,7 +174,7 @@ __global__ void __launch_bounds__(kRopeWarps * 32) qkrope_bwd_any_kernel(const _
 // ---------------------------------------------------------------------------
 // rows of 16-byte packs: a group of G lanes holds a head row, one pack a lane
 // ---------------------------------------------------------------------------
-// Unit of work of a warp: kRopeIter rounds of 32 / G consecutive heads of one
+// Unit of work of a warp: rope_rounds() rounds of 32 / G consecutive heads of one
 // token, so that a round is one contiguous stretch of the projection's row, the
 // loads of all rounds are in flight at once and the token's cosines and sines
 // are read once per unit. Element pairs: interleaved pairs lie in one lane's
@@ -182,7 +182,10 @@ __global__ void __launch_bounds__(kRopeWarps * 32) qkrope_bwd_any_kernel(const _
 // elements and lane l + h the second, exchanged by a shuffle. Units are counted in
 // 32 bits (64-bit divisions took half the backward's time); the host sends
 // launches with more of them to the kernels above.
-constexpr int kRopeIter = 4;
+// Rounds of a unit. The weight gradients' sums take registers that four rounds' loads
+// need: 1237 x 3 tokens of 20 + 4 heads of 128, backward: 42.7 us with 4, 34.1 with 2
+// (without weights 16384 tokens of 16 heads of 64: 60.6 us with 4, 75.6 with 2).
+constexpr int rope_rounds(bool backward, bool weighted) { return backward && weighted ? 2 : 4; }
 constexpr int kRopeVecThreads = 256;
 
 // Left as single loads, divisions and conversions this was bound by issue slots,
@@ -276,6 +279,13 @@ __device__ __forceinline__ Pack<T, VEC> narrow(const float (&v)[VEC]) {
   return r;
 }
 
+// The outputs do not displace the rows still to be read from L2 (98 -> 91 us, forward
+// and backward of 16384 tokens of 16 heads of 64).
+template <typename T, int VEC>
+__device__ __forceinline__ void store_streaming(T* p, const Pack<T, VEC>& x) {
+  __stcs(reinterpret_cast<uint4*>(p), *reinterpret_cast<const uint4*>(&x));
+}
+
 template <int VEC>
 __device__ __forceinline__ float dot(const float (&x)[VEC], const float (&y)[VEC]) {
   float a0 = 0.f, a1 = 0.f;
@@ -292,20 +302,20 @@ __device__ __forceinline__ void scale(float (&x)[VEC], float w) {
 template <typename T, int G, bool INTERLEAVED, bool WEIGHTED>
 __global__ void __launch_bounds__(kRopeVecThreads, sizeof(T) == 2 ? 4 : 3)
     qkrope_fwd_kernel(const __grid_constant__ QkRopeArgs a) {
-  constexpr int VEC = 16 / sizeof(T), ROUND = 32 / G;
+  constexpr int VEC = 16 / sizeof(T), ROUND = 32 / G, ROUNDS = rope_rounds(false, WEIGHTED);
   const int lane = threadIdx.x & 31, l = lane % G;
   const int H = a.Hq + 2 * a.Hkv, Hqk = a.Hq + a.Hkv;
-  const unsigned units = (H + kRopeIter * ROUND - 1) / (kRopeIter * ROUND);
+  const unsigned units = (H + ROUNDS * ROUND - 1) / (ROUNDS * ROUND);
   const unsigned unit = blockIdx.x * (kRopeVecThreads / 32) + (threadIdx.x >> 5);
   if (unit >= static_cast<unsigned>(a.N) * units) return;
   const unsigned n = unit / units;
-  const int first = static_cast<int>(unit - n * units) * kRopeIter * ROUND, r0 = first + lane / G;
+  const int first = static_cast<int>(unit - n * units) * ROUNDS * ROUND, r0 = first + lane / G;
   const bool mine = l * VEC < a.D;  // lanes beyond the head carry zeros
   const long long p = first < Hqk ? rope_position(a, n, n % static_cast<unsigned>(a.T)) : 0;
   const T* x0 = static_cast<const T*>(a.qkv) + n * a.qkv_stride + l * VEC;
-  Pack<T, VEC> x[kRopeIter];
+  Pack<T, VEC> x[ROUNDS];
 #pragma unroll
-  for (int i = 0; i < kRopeIter; ++i) {
+  for (int i = 0; i < ROUNDS; ++i) {
     const int r = r0 + i * ROUND;
     if (mine && r < H) x[i] = load_stream<T, VEC>(x0 + r * a.D);
     else x[i] = Pack<T, VEC>{};
@@ -329,7 +339,7 @@ __global__ void __launch_bounds__(kRopeVecThreads, sizeof(T) == 2 ? 4 : 3)
     }
   }
 #pragma unroll
-  for (int i = 0; i < kRopeIter; ++i) {
+  for (int i = 0; i < ROUNDS; ++i) {
     const int r = r0 + i * ROUND;
     if (first + i * ROUND < Hqk) {  // some head of the round turns (the same for the whole warp)
       float v[VEC];
@@ -342,7 +352,7 @@ __global__ void __launch_bounds__(kRopeVecThreads, sizeof(T) == 2 ? 4 : 3)
       rope_turn<VEC, INTERLEAVED>(turn, from, v);
       if (r < Hqk) x[i] = narrow<T, VEC>(v);
     }
-    if (mine && r < H) *reinterpret_cast<Pack<T, VEC>*>((r < a.Hq ? yq : (r < Hqk ? yk : yv)) + r * a.D) = x[i];
+    if (mine && r < H) store_streaming<T, VEC>((r < a.Hq ? yq : (r < Hqk ? yk : yv)) + r * a.D, x[i]);
   }
 }
 
@@ -351,10 +361,10 @@ __global__ void __launch_bounds__(kRopeVecThreads, sizeof(T) == 2 ? 4 : 3)
 template <typename T, int G, bool INTERLEAVED, bool WEIGHTED>
 __global__ void __launch_bounds__(kRopeVecThreads, WEIGHTED ? 2 : 3)
     qkrope_bwd_kernel(const __grid_constant__ QkRopeArgs a) {
-  constexpr int VEC = 16 / sizeof(T), ROUND = 32 / G;
+  constexpr int VEC = 16 / sizeof(T), ROUND = 32 / G, ROUNDS = rope_rounds(true, WEIGHTED);
   const int lane = threadIdx.x & 31, l = lane % G;
   const int H = a.Hq + 2 * a.Hkv, Hqk = a.Hq + a.Hkv;
-  const unsigned units = (H + kRopeIter * ROUND - 1) / (kRopeIter * ROUND);
+  const unsigned units = (H + ROUNDS * ROUND - 1) / (ROUNDS * ROUND);
   const bool mine = l * VEC < a.D;
   float wq[VEC], wk[VEC], acc[2][VEC];
   if (WEIGHTED) {
@@ -368,7 +378,7 @@ __global__ void __launch_bounds__(kRopeVecThreads, WEIGHTED ? 2 : 3)
   const unsigned step = gridDim.x * (kRopeVecThreads / 32), total = static_cast<unsigned>(a.N) * units;
   for (unsigned unit = blockIdx.x * (kRopeVecThreads / 32) + (threadIdx.x >> 5); unit < total; unit += step) {
     const unsigned n = unit / units, b = n / static_cast<unsigned>(a.T), t = n - b * static_cast<unsigned>(a.T);
-    const int first = static_cast<int>(unit - n * units) * kRopeIter * ROUND, r0 = first + lane / G;
+    const int first = static_cast<int>(unit - n * units) * ROUNDS * ROUND, r0 = first + lane / G;
     const long long p = first < Hqk ? rope_position(a, n, t) : 0;
     const T* x0 = static_cast<const T*>(a.qkv) + n * a.qkv_stride + l * VEC;
     const T* g0[3];
@@ -376,9 +386,9 @@ __global__ void __launch_bounds__(kRopeVecThreads, WEIGHTED ? 2 : 3)
 #pragma unroll
     for (int i = 0; i < 3; ++i)
       g0[i] = static_cast<const T*>(a.g[i]) + b * a.gs[i][0] + t * a.gs[i][1] - skip[i] * a.gs[i][2] + l * VEC;
-    Pack<T, VEC> x[kRopeIter], g[kRopeIter];
+    Pack<T, VEC> x[ROUNDS], g[ROUNDS];
 #pragma unroll
-    for (int i = 0; i < kRopeIter; ++i) {
+    for (int i = 0; i < ROUNDS; ++i) {
       const int r = r0 + i * ROUND, part = r < a.Hq ? 0 : (r < Hqk ? 1 : 2);
       x[i] = g[i] = Pack<T, VEC>{};
       if (mine && r < H) {
@@ -395,7 +405,7 @@ __global__ void __launch_bounds__(kRopeVecThreads, WEIGHTED ? 2 : 3)
     }
     T* const dx = static_cast<T*>(a.dqkv) + static_cast<long long>(n) * H * a.D + l * VEC;
 #pragma unroll
-    for (int i = 0; i < kRopeIter; ++i) {
+    for (int i = 0; i < ROUNDS; ++i) {
       const int r = r0 + i * ROUND;
       if (first + i * ROUND < Hqk) {
         float e[VEC], v[VEC];
@@ -418,7 +428,7 @@ __global__ void __launch_bounds__(kRopeVecThreads, WEIGHTED ? 2 : 3)
         scale<VEC>(e, inv);
         if (r < Hqk) g[i] = narrow<T, VEC>(e);
       }
-      if (mine && r < H) *reinterpret_cast<Pack<T, VEC>*>(dx + r * a.D) = g[i];
+      if (mine && r < H) store_streaming<T, VEC>(dx + r * a.D, g[i]);
     }
   }
   if constexpr (WEIGHTED) {
@@ -503,7 +513,8 @@ cudaError_t run_t(bool backward, const QkRopeArgs& a, cudaStream_t st) {
   if (e != cudaSuccess) return e;
   const int H = a.Hq + 2 * a.Hkv, G = pack_lanes<T>(a, backward);
   const int warps = G ? kRopeVecThreads / 32 : kRopeWarps;
-  const long long units = G ? a.N * ((H + kRopeIter * (32 / G) - 1) / (kRopeIter * (32 / G))) : a.N * H;
+  const int per_unit = G ? rope_rounds(backward, a.w[0] || a.w[1]) * (32 / G) : 1;
+  const long long units = a.N * ((H + per_unit - 1) / per_unit);
   long long blocks = (units + warps - 1) / warps;
   if (a.partials) blocks = std::min<long long>(blocks, static_cast<long long>(nsm) * kRopePartialBlocksPerSm);
   const unsigned grid = static_cast<unsigned>(blocks);
