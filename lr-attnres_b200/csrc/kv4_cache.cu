@@ -12,8 +12,8 @@
 // for every 16 elements it forms), so the work per element is kept to a subtraction, a
 // product, a sum that rounds (adding 1.5 * 2^23 leaves the integer in the low bits), a
 // multiply-add into the packed word, and the distance to a tie: the quotient is formed
-// with the reciprocal, and the eight are redone by division if one of them comes within
-// 2^-16 of a tie, which keeps the codes those of the division.
+// with the reciprocal, and elements within 2^-16 of a tie are redone by division, which
+// keeps the codes those of the division.
 #include "common.cuh"
 #include "kv4.h"
 #include "tma.cuh"
@@ -109,26 +109,34 @@ __device__ __forceinline__ Quantised quantise8(const float (&x)[8]) {
   r.params = odd ? __floats2half2_rn(nan, nan) : __floats2half2_rn(__fmul_rn(range, 1.f / 15.f), low);
   const float step = __low2float(r.params), base = __high2float(r.params);
   const float inv = step > 0.f ? __fdividef(1.f / 15.f, step) : 0.f;  // codes of 0 where there is no step
-  float worst = 0.f;
+  float worst = 0.f, off[8];
   uint32_t word = 0, own = 0;  // own: the rounder's own bits, 0x4b400000 at every shift that keeps some
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
     // the quotient over 15, clamped to 0 .. 1 on the way
     const float q = __saturatef(__fsub_rn(x[e], base) * inv), n = fmaf(q, 15.f, kRounder);
-    worst = fmaxf(worst, fabsf(fmaf(q, 15.f, -__fsub_rn(n, kRounder))));
+    off[e] = fabsf(fmaf(q, 15.f, -__fsub_rn(n, kRounder)));
+    worst = fmaxf(worst, off[e]);
     word += __float_as_uint(n) << (4 * e);
     own += 0x4b400000u << (4 * e);
   }
   r.codes = word - own;
-  if (worst > 0.5f - 1.f / 65536.f) {
-    r.codes = 0;
+  constexpr float kTie = 0.5f - 1.f / 65536.f;
+  if (worst > kTie) {
+    // Exact ties are common in 16-bit data (one element in a thousand), so only those
+    // close to one are done again.
+    unsigned close = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) close |= off[e] > kTie ? 1u << e : 0u;
 #pragma unroll 1
-    for (int e = 0; e < 8; ++e) {
+    while (close) {
+      const int e = __ffs(close) - 1;
+      close &= close - 1;
       float y = x[0];  // x[e], without an array in memory
 #pragma unroll
       for (int i = 1; i < 8; ++i) y = i == e ? x[i] : y;
-      const float n = rintf(__fdiv_rn(__fsub_rn(y, base), step));
-      r.codes |= static_cast<uint32_t>(fminf(fmaxf(n, 0.f), 15.f)) << (4 * e);
+      const float n = fminf(fmaxf(rintf(__fdiv_rn(__fsub_rn(y, base), step)), 0.f), 15.f);
+      r.codes = (r.codes & ~(15u << (4 * e))) | (static_cast<uint32_t>(n) << (4 * e));
     }
   }
   return r;
@@ -217,7 +225,7 @@ __device__ __forceinline__ void store_values(T* out, uint32_t codes, __half2 par
         *reinterpret_cast<__nv_bfloat162*>(&y.e[e]) = __floats2bfloat162_rn(v[0], v[1]);
       }
     }
-    *reinterpret_cast<Pack<T, VEC>*>(out + i) = y;
+    __stcs(reinterpret_cast<uint4*>(out + i), *reinterpret_cast<const uint4*>(&y));
   }
 }
 
