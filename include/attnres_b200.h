@@ -497,7 +497,7 @@ int attnres_base_backward(int num_sources, int64_t num_tokens, int value_dim, in
  * of seq_len; row n is token n % seq_len of sequence n / seq_len. cos / sin float
  * [table_rows, rotary_dim / 2] dense; positions int32 (int64 with
  * positions_are_64) [num_tokens], NULL for n % seq_len. A position outside
- * [0, table_rows) makes the token's q and k rows NaN. interleaved: pairs
+ * [0, table_rows) makes the rotated elements of the token's q and k NaN. interleaved: pairs
  * (2i, 2i+1), else (i, i + rotary_dim/2). normalize 0 leaves the norm out.
  * q_weight / k_weight dtype [head_dim] or NULL. q [num_tokens, q_heads, head_dim],
  * k, v [num_tokens, kv_heads, head_dim], dense. head_dim up to 512.

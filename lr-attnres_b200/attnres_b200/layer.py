@@ -117,7 +117,7 @@ def qk_norm_rope(qkv: Tensor, num_heads: int, num_kv_heads: int, cos: Tensor, si
     q [B, T, num_heads, head_dim] and k, v [B, T, num_kv_heads, head_dim], dense. cos, sin float32
     [positions, rotary_dim / 2], rotary_dim <= head_dim; the remaining elements pass unrotated.
     positions [B, T] int32 or int64 (default: the token's index in its sequence); a token whose
-    position lies outside the tables gets NaN queries and keys. interleaved pairs elements
+    position lies outside the tables gets NaN in the rotated elements of its queries and keys. interleaved pairs elements
     (2i, 2i + 1), otherwise (i, i + rotary_dim / 2). q_weight, k_weight [head_dim] multiply the normed
     heads. normalize=False leaves the norm out; eps defaults to float32's, as the model's norms have it.
     Differentiable in qkv and the weights."""

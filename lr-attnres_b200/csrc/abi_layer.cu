@@ -94,7 +94,9 @@ int check_swiglu(int64_t n, int in_dim, int hidden, int dtype, const void* x, in
   if (dtype == ATTNRES_DTYPE_F32) return fail(ATTNRES_ERR_UNSUPPORTED, "swiglu: float16 and bfloat16 only");
   if (in_dim % 8 || hidden % 8 || hidden > (1 << 28))
     return fail(ATTNRES_ERR_UNSUPPORTED, "swiglu: in_dim=%d and hidden=%d must be multiples of 8", in_dim, hidden);
-  if (n > 0x7fffffffLL || (n / 128 + 1) * (hidden / 128 + 1) > 0x7fffffffLL)
+  // tiles of 256 rows x 64 or 128 columns of h, dx and dW are counted in 32 bits
+  if (n > 0x7fffffffLL || in_dim > (1 << 28) || (n / 128 + 1) * (hidden / 128 + 1) > 0x7fffffffLL ||
+      (n / 128 + 1) * (in_dim / 128 + 1) > 0x7fffffffLL || (hidden / 128LL + 1) * (in_dim / 128 + 1) > 0x7fffffffLL)
     return fail(ATTNRES_ERR_UNSUPPORTED, "swiglu: num_tokens=%lld is too many for one launch", (long long)n);
   if (xs < in_dim || ws < in_dim) return fail(ATTNRES_ERR_INVALID_ARGUMENT, "swiglu: a row stride below in_dim");
   if (!w || (n > 0 && !x)) return fail(ATTNRES_ERR_INVALID_ARGUMENT, "swiglu: x or weight is NULL");

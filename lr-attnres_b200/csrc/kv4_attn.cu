@@ -658,6 +658,7 @@ size_t kv4_attention_workspace_bytes(const Kv4AttnArgs& a) {
 
 cudaError_t kv4_attention_launch(int dtype, const Kv4AttnArgs& a, cudaStream_t st) {
   AttnLaunch L = plan(a);
+  if (static_cast<long long>(L.splits) * L.row_tiles > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
   L.part_o = static_cast<float*>(a.workspace);
   L.part_ml = reinterpret_cast<float2*>(L.part_o + parts(L) * a.c.D);
   return dtype == ATTNRES_DTYPE_BF16 ? attn_dt<__nv_bfloat16>(L, st) : attn_dt<__half>(L, st);
