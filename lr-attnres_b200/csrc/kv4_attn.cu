@@ -154,8 +154,11 @@ __global__ void __launch_bounds__(kAtWarps * 32, NT == 1 ? (D == 64 ? 5 : 3) : 2
   __shared__ float warp_m[kAtWarps][ROWS], warp_l[kAtWarps][ROWS], row_top[ROWS], row_sum[ROWS];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
   const int split = blockIdx.x % L.splits, tile = blockIdx.x / L.splits, h = blockIdx.y, b = blockIdx.z;
+  // this thread's first entry of the page table, on its way while the length is read
+  const int from = split * L.stretch, first_slot = (from + static_cast<int>(threadIdx.x) * 16) / a.c.page;
+  const int first_page = first_slot < a.max_pages ? a.table[b * a.table_stride + first_slot] : -1;
   const SeqFacts seq = seq_facts(a, b);
-  const int from = split * L.stretch, to = min(from + L.stretch, seq.length);
+  const int to = min(from + L.stretch, seq.length);
   // the join may take up its place on the GPU; it waits for this grid's end before it reads
   if (L.splits > 1) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (from >= to && L.splits > 1) return;  // the join knows how many stretches there are
@@ -167,7 +170,7 @@ __global__ void __launch_bounds__(kAtWarps * 32, NT == 1 ? (D == 64 ? 5 : 3) : 2
       continue;
     }
     const int at = from + i * 16, slot = at / a.c.page;
-    const int p = a.table[b * a.table_stride + slot];
+    const int p = i < kAtWarps * 32 ? first_page : a.table[b * a.table_stride + slot];
     const bool there = p >= 0 && p < a.c.pages;
     if (!there) atomicOr(&g_kv4_attn_status, kStatusCacheRange);
     const int place16 = (at - slot * a.c.page) >> 4;
@@ -542,41 +545,53 @@ __global__ void __launch_bounds__(kAtWarps * 32, NT == 1 ? (D == 64 ? 5 : 3) : 2
   }
 }
 
-// One warp a row: adds the stretches of its sequence in order.
+// One CTA a row adds the stretches of its sequence: its warps take every fourth, and are
+// added in order. (With a warp a row, one sequence of 100000 keys spent 60 of 103 us here,
+// waiting for 196 loads one after the other.)
 template <typename T, int D>
 __global__ void __launch_bounds__(128) kv4_join_kernel(const __grid_constant__ AttnLaunch L, int tile_rows) {
+  constexpr int VEC = D / 32;
+  __shared__ float warp_top[4], warp_total[4], warp_sum_of[4][D];
   const Kv4AttnArgs& a = L.a;
-  const long long index = static_cast<long long>(blockIdx.x) * 4 + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
-  if (index >= static_cast<long long>(a.B) * a.c.heads * L.rows) return;
-  const int row = static_cast<int>(index % L.rows);
-  const long long bh = index / L.rows;
-  const int h = static_cast<int>(bh % a.c.heads), b = static_cast<int>(bh / a.c.heads);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int row = static_cast<int>(blockIdx.x % L.rows), bh = static_cast<int>(blockIdx.x / L.rows);
+  const int h = bh % a.c.heads, b = bh / a.c.heads;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const SeqFacts seq = seq_facts(a, b);
   const int n = (seq.length + L.stretch - 1) / L.stretch;
-  const long long unit = (bh * L.row_tiles + row / tile_rows) * L.splits;
-  const int r = row % tile_rows;
+  const long long first = (static_cast<long long>(bh) * L.row_tiles + row / tile_rows) * L.splits * tile_rows + row % tile_rows;
+  const float2* ml = L.part_ml + first;  // of stretch s: s * tile_rows on
+  const float* part = L.part_o + first * D + lane * VEC;
   float top = -INFINITY;
-  for (int s = lane; s < n; s += 32) top = fmaxf(top, L.part_ml[(unit + s) * tile_rows + r].x);
+  for (int s = threadIdx.x; s < n; s += 128) top = fmaxf(top, ml[static_cast<long long>(s) * tile_rows].x);
   top = warp_max(top);
-  constexpr int VEC = D / 32;
+  if (lane == 0) warp_top[warp] = top;
+  __syncthreads();
+  top = fmaxf(fmaxf(warp_top[0], warp_top[1]), fmaxf(warp_top[2], warp_top[3]));
   float y[VEC] = {}, total = 0.f;
   if (top != -INFINITY) {
-    for (int s = 0; s < n; ++s) {
-      const float2 ml = L.part_ml[(unit + s) * tile_rows + r];
-      const float f = ml.x == -INFINITY ? 0.f : exp2f(ml.x - top);
-      total += f * ml.y;
-      const Pack<float, VEC> p = load_pack<float, VEC>(L.part_o + ((unit + s) * tile_rows + r) * D + lane * VEC);
+#pragma unroll 4
+    for (int s = warp; s < n; s += 4) {
+      const float2 x = ml[static_cast<long long>(s) * tile_rows];
+      const Pack<float, VEC> p = load_pack<float, VEC>(part + static_cast<long long>(s) * tile_rows * D);
+      const float f = x.x == -INFINITY ? 0.f : exp2f(x.x - top);
+      total += f * x.y;
 #pragma unroll
       for (int e = 0; e < VEC; ++e) y[e] += f * p.e[e];
     }
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) y[e] /= total;
   }
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) warp_sum_of[warp][lane * VEC + e] = y[e];
+  if (lane == 0) warp_total[warp] = total;
+  __syncthreads();
+  total = (warp_total[0] + warp_total[1]) + (warp_total[2] + warp_total[3]);
   const long long to_row = out_index<T>(L, b, h, row);
-  store_pack<T, VEC>(static_cast<T*>(a.out) + to_row * D + lane * VEC, y);
-  if (a.lse && lane == 0) a.lse[to_row] = top == -INFINITY ? -INFINITY : (top + log2f(total)) / kLog2e;
+  if (threadIdx.x < D) {
+    const int d = threadIdx.x;
+    const float v = (warp_sum_of[0][d] + warp_sum_of[1][d]) + (warp_sum_of[2][d] + warp_sum_of[3][d]);
+    static_cast<T*>(a.out)[to_row * D + d] = Elem<T>::from_f(top == -INFINITY ? 0.f : v / total);
+  }
+  if (a.lse && threadIdx.x == 0) a.lse[to_row] = top == -INFINITY ? -INFINITY : (top + log2f(total)) / kLog2e;
 }
 
 namespace {
@@ -630,7 +645,7 @@ cudaError_t attn_t(const AttnLaunch& L, cudaStream_t st) {
   const long long rows = static_cast<long long>(L.a.B) * L.a.c.heads * L.rows;
   // a programmatic dependent: its launch overlaps the attention (3 us less a call)
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>((rows + 3) / 4));
+  cfg.gridDim = dim3(static_cast<unsigned>(rows));
   cfg.blockDim = dim3(128);
   cfg.stream = st;
   cudaLaunchAttribute at[1];
