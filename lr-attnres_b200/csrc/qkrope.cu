@@ -13,7 +13,9 @@
 // again in the backward: x is read there anyway, so nothing is saved.
 //
 // Bound by HBM: forward 2, backward (with x of q and k read again) 2 2/3 times
-// the projection's bytes when query and key heads are as many.
+// the projection's bytes when query and key heads are as many. 16384 tokens of 16
+// query and key heads of 64, bf16: forward 34.4 us for 201 MB (5.9 TB/s, 91 % of the
+// measured copy rate), backward 56.8 us for 277 MB (4.9 TB/s, 76 %).
 #include <algorithm>
 
 #include "common.cuh"

@@ -27,6 +27,9 @@
 // thread of tcgen05.mma for both, 8 warps of epilogue on the other half of the
 // accumulators. Every mbarrier wait is bounded (~2 s, a status bit on timeout); tensor
 // memory is always released.
+// 16384 tokens, 1024 -> 4096, bf16: gate forward 188 us (1465 TFLOP/s), gate backward 222
+// (1240; its epilogue moves 400 MB), dx and dW 365 (1505). The tensor cores are busy 80 to
+// 85 % of the cycles and the power limit holds the clock at 1.6 GHz.
 #include <algorithm>
 
 #include "cluster.cuh"
@@ -476,6 +479,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGmThreads, 1)
 // same from x: which of the 16 k a lane holds does not matter as long as A and B
 // agree. Bound by reading W once; the tensor cores of this kernel idle most of the
 // time, so the older instruction, whose operands come from registers, suffices.
+// 1024 -> 4096 in bf16, 16.8 MB: 5.1 us at 1 token, 6.6 at 12, 8.2 at 27.
 constexpr int kFewWarps = 8;
 
 struct FewArgs {
