@@ -55,7 +55,8 @@ constexpr int kAtWarps = 4;
 // Places of a stage, and stages of a warp's ring: what a stage costs besides its places
 // (the wait, the copies, the maximum's vote) is a third of 32 places' work at head_dim 64.
 constexpr int at_keys(int D) { return D == 64 ? 64 : 32; }
-constexpr int at_stages(int D) { return D == 64 ? 2 : 3; }
+constexpr int at_stages(int) { return 2; }
+template <int D, int NT> struct SharedQ { static constexpr bool value = D == 128; };
 constexpr int kAtMaxStretch = 4096;
 constexpr float kLog2e = 1.4426950408889634f;
 // The running maximum is raised only when a score passes it by this much (in powers of
@@ -148,7 +149,7 @@ __device__ __forceinline__ long long out_index(const AttnLaunch& L, int b, int h
 }
 
 template <typename T, int D, int NT>
-__global__ void __launch_bounds__(kAtWarps * 32, NT == 1 ? (D == 64 ? 5 : 3) : 2) kv4_attn_kernel(const __grid_constant__ AttnLaunch L) {
+__global__ void __launch_bounds__(kAtWarps * 32, NT == 1 ? (D == 64 ? 5 : 4) : 2) kv4_attn_kernel(const __grid_constant__ AttnLaunch L) {
   constexpr int G = D / kKv4Group, HALF = D / 2;
   constexpr int KEYS = at_keys(D), PIECES = KEYS / 16, STAGES = at_stages(D);
   constexpr int kCode = KEYS * HALF, kParam = KEYS * G * 4;  // bytes of a stage
@@ -211,8 +212,12 @@ __global__ void __launch_bounds__(kAtWarps * 32, NT == 1 ? (D == 64 ? 5 : 3) : 2
   for (int i = 0; i < STAGES; ++i)
     if (warp + i * kAtWarps < count) fetch(warp + i * kAtWarps, i);
 
-  // the query rows as the second operand: column g of tile j is row 8 j + g
-  uint32_t qf[NT][G][4];
+  // the query rows as the second operand: column g of tile j is row 8 j + g. At head_dim
+  // 128 they lie in shared memory, where the four warps share them: with them in registers
+  // three CTAs fit on an SM, and the kernel waits for its own latencies.
+  constexpr bool SHARED_Q = SharedQ<D, NT>::value;
+  __shared__ uint4 q_shared[SHARED_Q ? NT * G * 32 : 1];
+  uint32_t qf[SHARED_Q ? 1 : NT][SHARED_Q ? 1 : G][4];
   float qsum[NT][G][2], zscale[NT][2];  // of rows 8 j + 2 c, 2 c + 1
   int last[NT][2];
 #pragma unroll
@@ -247,15 +252,22 @@ __global__ void __launch_bounds__(kAtWarps * 32, NT == 1 ? (D == 64 ? 5 : 3) : 2
     const float up = exponent == 255 ? 1.f : __int_as_float(min(264 - exponent, 250) << 23);
 #pragma unroll
     for (int i = 0; i < G; ++i) {
+      uint32_t w[4];
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         const float f = (k & 1) ? up : 16.f * up;
-        qf[j][i][k] = half_pack(x[i][k] * f, x[i][k + 4] * f);
+        w[k] = half_pack(x[i][k] * f, x[i][k + 4] * f);
+      }
+      if constexpr (SHARED_Q) {
+        if (warp == i % kAtWarps) q_shared[(j * G + i) * 32 + lane] = make_uint4(w[0], w[1], w[2], w[3]);
+      } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) qf[j][i][k] = w[k];
       }
       float s[4] = {};
       const uint32_t one = 0x3c003c00u, sixteenth = 0x2c002c00u;
-      mma_16816<__half>(s, sixteenth, sixteenth, one, one, qf[j][i][0], qf[j][i][1]);
-      mma_16816<__half>(s, sixteenth, sixteenth, one, one, qf[j][i][2], qf[j][i][3]);
+      mma_16816<__half>(s, sixteenth, sixteenth, one, one, w[0], w[1]);
+      mma_16816<__half>(s, sixteenth, sixteenth, one, one, w[2], w[3]);
 #pragma unroll
       for (int e = 0; e < 2; ++e) qsum[j][i][e] = s[e] * kOddUnit;
     }
@@ -266,6 +278,7 @@ __global__ void __launch_bounds__(kAtWarps * 32, NT == 1 ? (D == 64 ? 5 : 3) : 2
       zscale[j][e] = a.scale * (kLog2e / kOddUnit) / __shfl_sync(0xffffffffu, up, 4 * (2 * c + e));
     }
   }
+  if constexpr (SHARED_Q) __syncthreads();
   int least = 0x7fffffff;  // places up to this one are seen by all rows that see any
 #pragma unroll
   for (int j = 0; j < NT; ++j)
@@ -308,9 +321,12 @@ __global__ void __launch_bounds__(kAtWarps * 32, NT == 1 ? (D == 64 ? 5 : 3) : 2
         const float2 s1 = __half22float2(*reinterpret_cast<const __half2*>(&p1[i]));
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
+          uint4 w;
+          if constexpr (SHARED_Q) w = q_shared[(j * G + i) * 32 + lane];
+          else w = make_uint4(qf[j][i][0], qf[j][i][1], qf[j][i][2], qf[j][i][3]);
           float acc[4];
-          mma_16816<__half>(acc, f0[0], f1[0], f0[1], f1[1], qf[j][i][0], qf[j][i][1], 0.f, 0.f, 0.f, 0.f);
-          mma_16816<__half>(acc, f0[2], f1[2], f0[3], f1[3], qf[j][i][2], qf[j][i][3]);
+          mma_16816<__half>(acc, f0[0], f1[0], f0[1], f1[1], w.x, w.y, 0.f, 0.f, 0.f, 0.f);
+          mma_16816<__half>(acc, f0[2], f1[2], f0[3], f1[3], w.z, w.w);
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const float2 s = e < 2 ? s0 : s1;
@@ -613,8 +629,10 @@ size_t attn_smem(int D, int NT) {
   return std::max(ring, sums);
 }
 
-// Stretches: about four CTAs for every one that fits on the GPU, so that ragged
-// lengths even out, of at least 128 places (one stage a warp).
+// Stretches: about two CTAs for every one that fits on the GPU (24 x 6000 places of 8
+// heads of 128: 62 us; with three CTAs for every two that fit 70, with four for one 69),
+// of at least 128 places. Sequences of up to 512 places stay whole: one launch instead of
+// two (one sequence of 300: 8.8 -> 7.6 us on the GPU).
 AttnLaunch plan(const Kv4AttnArgs& a) {
   AttnLaunch L{};
   L.a = a;
@@ -626,7 +644,7 @@ AttnLaunch plan(const Kv4AttnArgs& a) {
   if (cached_sm_count(&nsm) != cudaSuccess) nsm = 148;
   const long long room = std::max(1LL, static_cast<long long>(a.max_pages) * a.c.page);
   const long long all = room * a.B * a.c.heads * L.row_tiles;
-  const long long wish = all / (4LL * nsm * 3) + 1;
+  const long long wish = room <= 512 ? room : all / (8LL * nsm) + 1;
   long long stretch = (std::min<long long>(wish, room) + 127) / 128 * 128;
   stretch = std::min<long long>(std::max<long long>(stretch, 128), kAtMaxStretch);
   L.stretch = static_cast<int>(stretch);
