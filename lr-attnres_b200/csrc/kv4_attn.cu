@@ -36,9 +36,9 @@
 // HBM is the floor (40 bytes a place of 64 elements, keys and values each), the ALU what
 // it meets: 8 sequences of 50000 places, 16 heads of 64, 3 tokens: 154 us for 512 MB
 // (3.3 TB/s; the logic pipe is busy 60 % of the time, DRAM 36 %, the tensor cores 15 %);
-// 8 x 50000 places, 8 heads of 128, 4 query heads each: 147 us (3.5 TB/s). At head_dim 128
-// the accumulators leave room for 12 warps an SM, and a stretch of a few stages is mostly
-// its start and end: 24 ragged sequences up to 6000 places 34 us for 72 MB.
+// 8 x 50000 places, 8 heads of 128, 4 query heads each: 136 us (3.75 TB/s). A stretch of a
+// few stages is mostly its start and end: 24 ragged sequences up to 6000 places of 8 heads
+// of 128 32 us for 72 MB.
 #include <algorithm>
 
 #include "common.cuh"
@@ -56,7 +56,7 @@ constexpr int kAtWarps = 4;
 // (the wait, the copies, the maximum's vote) is a third of 32 places' work at head_dim 64.
 constexpr int at_keys(int D) { return D == 64 ? 64 : 32; }
 constexpr int at_stages(int) { return 2; }
-template <int D, int NT> struct SharedQ { static constexpr bool value = D == 128; };
+constexpr bool at_shared_q(int D) { return D == 128; }
 constexpr int kAtMaxStretch = 4096;
 constexpr float kLog2e = 1.4426950408889634f;
 // The running maximum is raised only when a score passes it by this much (in powers of
@@ -141,8 +141,7 @@ __device__ __forceinline__ int last_place(const SeqFacts& s, int t) {
   return t < s.count ? s.length - s.count + t : -1;
 }
 
-// Writes one finished row.
-template <typename T>
+// Where a row's outputs lie, in rows of head_dim.
 __device__ __forceinline__ long long out_index(const AttnLaunch& L, int b, int h, int row) {
   const int t = row / L.group, head = h * L.group + row - t * L.group;
   return (static_cast<long long>(b) * L.a.T + t) * L.a.Hq + head;
@@ -215,7 +214,7 @@ __global__ void __launch_bounds__(kAtWarps * 32, NT == 1 ? (D == 64 ? 5 : 4) : 2
   // the query rows as the second operand: column g of tile j is row 8 j + g. At head_dim
   // 128 they lie in shared memory, where the four warps share them: with them in registers
   // three CTAs fit on an SM, and the kernel waits for its own latencies.
-  constexpr bool SHARED_Q = SharedQ<D, NT>::value;
+  constexpr bool SHARED_Q = at_shared_q(D);
   __shared__ uint4 q_shared[SHARED_Q ? NT * G * 32 : 1];
   uint32_t qf[SHARED_Q ? 1 : NT][SHARED_Q ? 1 : G][4];
   float qsum[NT][G][2], zscale[NT][2];  // of rows 8 j + 2 c, 2 c + 1
@@ -556,7 +555,7 @@ __global__ void __launch_bounds__(kAtWarps * 32, NT == 1 ? (D == 64 ? 5 : 4) : 2
     }
     const float top = row_top[r], total = row_sum[r];
     if (L.splits == 1) {
-      const long long to_row = out_index<T>(L, b, h, row);
+      const long long to_row = out_index(L, b, h, row);
 #pragma unroll
       for (int e = 0; e < 4; ++e) y[e] = top == -INFINITY ? 0.f : y[e] / total;
       store_pack<T, 4>(static_cast<T*>(a.out) + to_row * D + d, y);
@@ -608,7 +607,7 @@ __global__ void __launch_bounds__(128) kv4_join_kernel(const __grid_constant__ A
   if (lane == 0) warp_total[warp] = total;
   __syncthreads();
   total = (warp_total[0] + warp_total[1]) + (warp_total[2] + warp_total[3]);
-  const long long to_row = out_index<T>(L, b, h, row);
+  const long long to_row = out_index(L, b, h, row);
   if (threadIdx.x < D) {
     const int d = threadIdx.x;
     const float v = (warp_sum_of[0][d] + warp_sum_of[1][d]) + (warp_sum_of[2][d] + warp_sum_of[3][d]);
