@@ -111,6 +111,20 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return y;
 }
 
+// (a0, a1) += (b0, b1) and (a0, a1) *= (b0, b1) in packed fp32.
+__device__ __forceinline__ void add_pair(float& a0, float& a1, float b0, float b1) {
+  asm("{\n\t.reg .b64 a, b;\n\tmov.b64 a, {%0, %1};\n\tmov.b64 b, {%2, %3};\n\t"
+      "add.rn.f32x2 a, a, b;\n\tmov.b64 {%0, %1}, a;\n\t}"
+      : "+f"(a0), "+f"(a1)
+      : "f"(b0), "f"(b1));
+}
+__device__ __forceinline__ void mul_pair(float& a0, float& a1, float b0, float b1) {
+  asm("{\n\t.reg .b64 a, b;\n\tmov.b64 a, {%0, %1};\n\tmov.b64 b, {%2, %3};\n\t"
+      "mul.rn.f32x2 a, a, b;\n\tmov.b64 {%0, %1}, a;\n\t}"
+      : "+f"(a0), "+f"(a1)
+      : "f"(b0), "f"(b1));
+}
+
 // G words at p, as one load where the size allows.
 template <int G>
 __device__ __forceinline__ void load_words(const unsigned char* p, uint32_t (&w)[G]) {
@@ -327,9 +341,13 @@ __global__ void __launch_bounds__(kAtWarps * 32, NT == 1 ? (D == 64 ? 5 : 4) : 2
           mma_16816<__half>(acc, f0[0], f1[0], f0[1], f1[1], w.x, w.y, 0.f, 0.f, 0.f, 0.f);
           mma_16816<__half>(acc, f0[2], f1[2], f0[3], f1[3], w.z, w.w);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float2 s = e < 2 ? s0 : s1;
-            z[mt][j][e] = fmaf(s.x, acc[e], i == 0 ? s.y * qsum[j][i][e & 1] : fmaf(s.y, qsum[j][i][e & 1], z[mt][j][e]));
+          for (int e = 0; e < 4; e += 2) {  // two rows at a time, in packed fp32
+            const float2 s = e == 0 ? s0 : s1;
+            float& z0 = z[mt][j][e];
+            float& z1 = z[mt][j][e + 1];
+            if (i == 0) mul2(z0, z1, s.y, qsum[j][i][0], qsum[j][i][1]);
+            else fma2(z0, z1, s.y, qsum[j][i][0], qsum[j][i][1]);
+            fma2(z0, z1, s.x, acc[e], acc[e + 1]);
           }
         }
       }
@@ -337,7 +355,7 @@ __global__ void __launch_bounds__(kAtWarps * 32, NT == 1 ? (D == 64 ? 5 : 4) : 2
       for (int j = 0; j < NT; ++j)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          z[mt][j][e] *= zscale[j][e & 1];
+          if (e % 2 == 0) mul_pair(z[mt][j][e], z[mt][j][e + 1], zscale[j][0], zscale[j][1]);
           if constexpr (MASKED) {
             const int place = at + (e < 2 ? key0 : key1);
             if (rows16[stage * PIECES + mt] < 0 || place >= to || place > last[j][e & 1]) z[mt][j][e] = -INFINITY;
@@ -378,13 +396,15 @@ __global__ void __launch_bounds__(kAtWarps * 32, NT == 1 ? (D == 64 ? 5 : 4) : 2
     }
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
-      const float less[2] = {m[j][0] == -INFINITY ? 0.f : m[j][0], m[j][1] == -INFINITY ? 0.f : m[j][1]};
+      const float less[2] = {m[j][0] == -INFINITY ? 0.f : -m[j][0], m[j][1] == -INFINITY ? 0.f : -m[j][1]};
 #pragma unroll
       for (int mt = 0; mt < PIECES; ++mt)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          z[mt][j][e] = exp2_fast(z[mt][j][e] - less[e & 1]);
-          l[j][e & 1] += z[mt][j][e];
+        for (int e = 0; e < 4; e += 2) {
+          add_pair(z[mt][j][e], z[mt][j][e + 1], less[0], less[1]);
+          z[mt][j][e] = exp2_fast(z[mt][j][e]);
+          z[mt][j][e + 1] = exp2_fast(z[mt][j][e + 1]);
+          add_pair(l[j][0], l[j][1], z[mt][j][e], z[mt][j][e + 1]);
         }
     }
 
