@@ -66,9 +66,10 @@ struct GemmJob {
 struct GemmArgs {
   GemmJob job[2];  // kGradients: dW, then dx; else one
   CUtensorMap dh;  // gate backward: [N, F]
-  // dx tiles of a pair after its dW tiles: x each for the first `more` pairs (which have
-  // a dW tile more than the others), y each for the rest
-  int more, x, y;
+  // kGradients: the tiles of job `first` (the one with the longer sums) are dealt out in
+  // turn; then come the other job's, x each for the first `more` pairs (which have one of
+  // the long ones more than the others), y each for the rest
+  int first, more, x, y;
 };
 
 struct TileRef {
@@ -88,13 +89,15 @@ __device__ __forceinline__ TileRef tile_at(const GemmArgs& a, int job, int tile)
 // The i-th tile of pair p of P, job -1 when there is none.
 template <int MODE>
 __device__ __forceinline__ TileRef tile_of(const GemmArgs& a, int p, int P, int i) {
-  const int first = a.job[0].tiles_m * a.job[0].tiles_n;
-  const int own = p < first ? (first - 1 - p) / P + 1 : 0;
-  if (i < own) return tile_at(a, 0, p + i * P);
+  const int first = MODE == kGradients ? a.first : 0;
+  const int count = a.job[first].tiles_m * a.job[first].tiles_n;
+  const int own = p < count ? (count - 1 - p) / P + 1 : 0;
+  if (i < own) return tile_at(a, first, p + i * P);
   if (MODE == kGradients) {
+    const GemmJob& other = a.job[1 - first];
     const int j = i - own, each = p < a.more ? a.x : a.y;
     const int tile = p < a.more ? j * a.more + p : a.more * a.x + j * (P - a.more) + p - a.more;
-    if (j < each && tile < a.job[1].tiles_m * a.job[1].tiles_n) return tile_at(a, 1, tile);
+    if (j < each && tile < other.tiles_m * other.tiles_n) return tile_at(a, 1 - first, tile);
   }
   return {-1, 0, 0};
 }
@@ -595,21 +598,25 @@ cudaError_t gemm_bn(GemmArgs& a, int dtype, int pairs, cudaStream_t st) {
     tiles += count[i];
   }
   const int P = static_cast<int>(std::min<long long>(tiles, pairs));
-  if (MODE == kGradients && count[1] > 0) {
-    // the split of the dx tiles that ends soonest: near the even share of all the work
-    a.more = count[0] % P;
-    const double k0 = a.job[0].ksteps, k1 = a.job[1].ksteps, base = count[0] / P * k0;
-    const double even = (count[0] * k0 + count[1] * k1) / P;
-    const int guess = std::max(0, static_cast<int>((even - base - k0) / k1));
-    double best = -1.0;
-    for (int x = std::max(0, guess - 2); x <= guess + 2; ++x) {
-      const long long left = std::max<long long>(0, count[1] - static_cast<long long>(a.more) * x);
-      const int y = static_cast<int>((left + P - a.more - 1) / (P - a.more));
-      const double end = std::max(a.more > 0 ? base + k0 + x * k1 : 0.0, base + y * k1);
-      if (best < 0.0 || end < best) {
-        best = end;
-        a.x = x;
-        a.y = y;
+  if (MODE == kGradients) {
+    // the split of the shorter tiles that ends soonest: near the even share of all the work
+    a.first = a.job[0].wanted && (!a.job[1].wanted || a.job[0].ksteps >= a.job[1].ksteps) ? 0 : 1;
+    const int n0 = count[a.first], n1 = count[1 - a.first];
+    a.more = n0 % P;
+    if (n1 > 0) {
+      const double k0 = a.job[a.first].ksteps, k1 = a.job[1 - a.first].ksteps, base = n0 / P * k0;
+      const double even = (n0 * k0 + n1 * k1) / P;
+      const int guess = std::max(0, static_cast<int>((even - base - k0) / k1));
+      double best = -1.0;
+      for (int x = std::max(0, guess - 2); x <= guess + 2; ++x) {
+        const long long left = std::max<long long>(0, n1 - static_cast<long long>(a.more) * x);
+        const int y = static_cast<int>((left + P - a.more - 1) / (P - a.more));
+        const double end = std::max(a.more > 0 ? base + k0 + x * k1 : 0.0, base + y * k1);
+        if (best < 0.0 || end < best) {
+          best = end;
+          a.x = x;
+          a.y = y;
+        }
       }
     }
   }
