@@ -188,7 +188,10 @@ template <typename T, int MODE, int BN>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGmThreads, 1)
     swiglu_gemm_kernel(const __grid_constant__ GemmArgs a) {
   constexpr bool GATE = MODE != kGradients;
-  constexpr uint32_t kA = 128 * kGmK * 2, kB = BN / 2 * kGmK * 2, kStage = kA + kB;  // bytes, of each CTA
+  // Bytes of each CTA: 64 columns of A and of B, and SUB of those a stage: a stage costs its
+  // issuer 0.16 us besides the products, as much as those of 64 columns of a narrow tile.
+  constexpr int SUB = BN == 128 ? 2 : 1;
+  constexpr uint32_t kA = 128 * kGmK * 2, kB = BN / 2 * kGmK * 2, kSub = kA + kB, kStage = SUB * kSub;
   constexpr int STAGES = kGmRing / kStage, F = BN / 2;                               // F: outputs of a gate tile
   // 64 columns a chunk; a gate tile of one chunk goes to either half of the epilogue warps in turn
   constexpr int CHUNKS = GATE ? F / 64 : BN / 64;
@@ -244,29 +247,33 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGmThreads, 1)
         const int m0 = t.m * kGmM + rank * 128, n0 = GATE ? t.n * F : t.n * BN + rank * (BN / 2);
         const CUtensorMap* const bmap = GATE && rank ? &g.b2 : &g.b;
         const int k_end = g.ksteps * kGmK;
-        for (int k = 0; k < k_end; k += kGmK) {
+        for (int k0 = 0; k0 < k_end; k0 += SUB * kGmK) {
           if (!ring_wait(empty0 + 8 * st, phase, abort_flag)) {
             atomicOr(&g_swiglu_status, kStatusEmptyWaitTimeout);
             *abort_flag = 1;
             ok = false;
             break;
           }
-          unsigned char* sa = stages + st * kStage;
-          unsigned char* sb = sa + kA;
           if (rank == 0) mbar_arrive_expect_tx(&full[st], 2 * kStage);
           const uint32_t bar = full0 + 8 * st;
-          if (GATE) {
-            tma_load_2d_pair(sa, &g.a, k, m0, bar);
-            tma_load_2d_pair(sb, bmap, k, n0, bar);
-          } else {
-            if (t.job == 0) {  // dW: rows of A are columns of [du dg]
-              tma_load_2d_pair(sa, &g.a, m0, k, bar);
-              tma_load_2d_pair(sa + 64 * 128, &g.a, m0 + 64, k, bar);
-            } else {
-              tma_load_2d_pair(sa, &g.a, k, m0, bar);
-            }
 #pragma unroll
-            for (int j = 0; j < BN / 128; ++j) tma_load_2d_pair(sb + j * 64 * 128, bmap, n0 + j * 64, k, bar);
+          for (int sub = 0; sub < SUB; ++sub) {  // past the end of K: zeros
+            unsigned char* sa = stages + st * kStage + sub * kSub;
+            unsigned char* sb = sa + kA;
+            const int k = k0 + sub * kGmK;
+            if (GATE) {
+              tma_load_2d_pair(sa, &g.a, k, m0, bar);
+              tma_load_2d_pair(sb, bmap, k, n0, bar);
+            } else {
+              if (t.job == 0) {  // dW: rows of A are columns of [du dg]
+                tma_load_2d_pair(sa, &g.a, m0, k, bar);
+                tma_load_2d_pair(sa + 64 * 128, &g.a, m0 + 64, k, bar);
+              } else {
+                tma_load_2d_pair(sa, &g.a, k, m0, bar);
+              }
+#pragma unroll
+              for (int j = 0; j < BN / 128; ++j) tma_load_2d_pair(sb + j * 64 * 128, bmap, n0 + j * 64, k, bar);
+            }
           }
           ++posted;
           if (++st == STAGES) {
@@ -309,7 +316,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGmThreads, 1)
         const uint32_t acc = tmem + ab * BN, idesc = g.idesc;
         const bool a_mn = !GATE && t.job == 0;
         const uint64_t a0 = a_mn ? mn_major : k_major, a_step = a_mn ? 128 : 2;
-        for (int k = 0; k < g.ksteps; ++k) {
+        const int steps = (g.ksteps + SUB - 1) / SUB;
+        for (int k = 0; k < steps; ++k) {
           if (!ring_wait(full0 + 8 * st, phase, abort_flag)) {
             atomicOr(&g_swiglu_status, kStatusFullWaitTimeout);
             *abort_flag = 1;
@@ -317,10 +325,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGmThreads, 1)
             break;
           }
           tc_fence_after();
-          const uint64_t da = a0 + st * kStageStep, db = b0 + st * kStageStep;
 #pragma unroll
-          for (int j = 0; j < kGmK / 16; ++j)
-            umma_f16_pair(acc, da + a_step * j, db + b_step * j, idesc, (k > 0 || j > 0) ? 1u : 0u);
+          for (int sub = 0; sub < SUB; ++sub) {
+            const uint64_t da = a0 + st * kStageStep + sub * (kSub >> 4), db = b0 + st * kStageStep + sub * (kSub >> 4);
+#pragma unroll
+            for (int j = 0; j < kGmK / 16; ++j)
+              umma_f16_pair(acc, da + a_step * j, db + b_step * j, idesc, (k > 0 || sub > 0 || j > 0) ? 1u : 0u);
+          }
           umma_commit_pair(&empty[st]);
           issued_any = true;
           if (++st == STAGES) {
@@ -574,9 +585,11 @@ cudaError_t few_t(const SwigluArgs& s, cudaStream_t st) {
   return cudaGetLastError();
 }
 
-// Time of a list of tiles on P pairs, in units of 512 cycles: a step of 64 columns of a
-// 256 x 256 tile is 1, of a 256 x 128 tile (half the products, 3/4 of the loads) 0.75, and
-// a tile's start and end that no other tile hides about 8.
+// Time of a list of tiles on P pairs, in steps of 64 columns of a 256 x 256 tile (0.42 us).
+// A step of a 256 x 128 tile counts 0.75: 0.5 alone, but it has 3/4 of the loads and twice
+// the starts and ends for its products (1531 tokens, 776 -> 2056, gate forward: 19.1 us on
+// wide tiles, 20.0 on narrow ones; dx, 42 narrow tiles or 24 wide: 21.7 and 28 us). 8: a
+// start and end that no other tile hides.
 double tiles_cost(const GemmJob& g, int BN, bool gate, int P) {
   const int n = gate ? ceil_div_i(g.cols, BN / 2) : ceil_div_i(g.cols, BN);
   const long long tiles = static_cast<long long>((g.M + kGmM - 1) / kGmM) * n;
