@@ -34,9 +34,9 @@
 // Every mbarrier wait is bounded (~2 s, a status bit on timeout).
 //
 // HBM is the floor (40 bytes a place of 64 elements, keys and values each), the ALU what
-// it meets: 8 sequences of 50000 places, 16 heads of 64, 3 tokens: 154 us for 512 MB
-// (3.3 TB/s; the logic pipe is busy 60 % of the time, DRAM 36 %, the tensor cores 15 %);
-// 8 x 50000 places, 8 heads of 128, 4 query heads each: 136 us (3.75 TB/s). A stretch of a
+// it meets: 8 sequences of 50000 places, 16 heads of 64, 3 tokens: 153 us with the join for
+// 512 MB (3.3 TB/s; the logic pipe is busy 60 % of the time, DRAM 36 %, the tensor cores
+// 15 %); 8 x 50000 places, 8 heads of 128, 4 query heads each: 132 us (3.9 TB/s). A stretch of a
 // few stages is mostly its start and end: 24 ragged sequences up to 6000 places of 8 heads
 // of 128 32 us for 72 MB.
 #include <algorithm>
