@@ -586,7 +586,8 @@ int attnres_kv4_read(const void* k_codes, const void* k_params, const void* v_co
  * dtype [batch, new_tokens, q_heads, head_dim] and lse float [batch, new_tokens,
  * q_heads] (log of the softmax's sum, NULL if not wanted), dense. A row that sees
  * nothing is zeros, its lse -inf. bf16 / fp16, head_dim 64 or 128. Workspace:
- * attnres_kv4_attention_workspace_bytes (may be 0).
+ * attnres_kv4_attention_workspace_bytes (may be 0), asked with the device current
+ * that the call will run on.
  */
 size_t attnres_kv4_attention_workspace_bytes(int kv_heads, int page_size, int head_dim, int max_pages, int batch,
                                              int new_tokens, int q_heads);

@@ -21,7 +21,15 @@ int fail(int code, const char* fmt, ...) {
   return attnres::record_error(code, buf);
 }
 
-int launched(cudaError_t e, const char* where) {
+// Runs a launch path; nothing it throws (its caches of device facts allocate) crosses the
+// C boundary.
+template <typename Launch>
+int launched(Launch&& launch, const char* where) {
+  cudaError_t e = cudaErrorMemoryAllocation;
+  try {
+    e = launch();
+  } catch (...) {
+  }
   if (e == cudaSuccess) return ATTNRES_OK;
   return fail(ATTNRES_ERR_CUDA, "%s: %s (%s)", where, cudaGetErrorName(e), cudaGetErrorString(e));
 }
@@ -164,7 +172,7 @@ int attnres_qk_norm_rope_forward(int64_t num_tokens, int64_t seq_len, int q_head
   a.out[0] = q;
   a.out[1] = k;
   a.out[2] = v;
-  return launched(attnres::qkrope_launch(false, dtype, a, static_cast<cudaStream_t>(stream)),
+  return launched([&] { return attnres::qkrope_launch(false, dtype, a, static_cast<cudaStream_t>(stream)); },
                   "attnres_qk_norm_rope_forward launch");
 }
 
@@ -194,7 +202,7 @@ int attnres_qk_norm_rope_backward(int64_t num_tokens, int64_t seq_len, int q_hea
     cudaError_t e = cudaSuccess;
     if (grad_q_weight) e = cudaMemsetAsync(grad_q_weight, 0, bytes, st);
     if (grad_k_weight && e == cudaSuccess) e = cudaMemsetAsync(grad_k_weight, 0, bytes, st);
-    return launched(e, "attnres_qk_norm_rope_backward memset");
+    return launched([&] { return e; }, "attnres_qk_norm_rope_backward memset");
   }
   if (!grad_q || !grad_k || !grad_v || !grad_strides || !grad_qkv)
     return fail(ATTNRES_ERR_INVALID_ARGUMENT, "qk norm rope backward: NULL gradient");
@@ -212,7 +220,8 @@ int attnres_qk_norm_rope_backward(int64_t num_tokens, int64_t seq_len, int q_hea
                   attnres::qkrope_workspace_bytes(head_dim));
     a.partials = static_cast<float*>(workspace);
   }
-  return launched(attnres::qkrope_launch(true, dtype, a, st), "attnres_qk_norm_rope_backward launch");
+  return launched([&] { return attnres::qkrope_launch(true, dtype, a, st); },
+                  "attnres_qk_norm_rope_backward launch");
 }
 
 int attnres_swiglu_forward(int64_t num_tokens, int in_dim, int hidden, int dtype, const void* x, int64_t x_row_stride,
@@ -230,7 +239,7 @@ int attnres_swiglu_forward(int64_t num_tokens, int in_dim, int hidden, int dtype
   a.x_stride = x_row_stride;
   a.w_stride = weight_row_stride;
   a.out = h;
-  return launched(attnres::swiglu_launch(false, dtype, a, static_cast<cudaStream_t>(stream)),
+  return launched([&] { return attnres::swiglu_launch(false, dtype, a, static_cast<cudaStream_t>(stream)); },
                   "attnres_swiglu_forward launch");
 }
 
@@ -246,9 +255,11 @@ int attnres_swiglu_backward(int64_t num_tokens, int in_dim, int hidden, int dtyp
   if (rc) return rc;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (num_tokens == 0)
-    return launched(grad_weight ? cudaMemsetAsync(grad_weight, 0, static_cast<size_t>(hidden) * in_dim * 4, st)
-                                : cudaSuccess,
-                    "attnres_swiglu_backward memset");
+    return launched(
+        [&] {
+          return grad_weight ? cudaMemsetAsync(grad_weight, 0, static_cast<size_t>(hidden) * in_dim * 4, st) : cudaSuccess;
+        },
+        "attnres_swiglu_backward memset");
   if (!grad_x && !grad_weight) return ATTNRES_OK;
   if (!grad_h) return fail(ATTNRES_ERR_INVALID_ARGUMENT, "swiglu backward: grad_h is NULL");
   if (grad_h_row_stride < hidden)
@@ -272,7 +283,8 @@ int attnres_swiglu_backward(int64_t num_tokens, int in_dim, int hidden, int dtyp
   a.dx = grad_x;
   a.dw = grad_weight;
   a.workspace = workspace;
-  return launched(attnres::swiglu_launch(true, dtype, a, st), "attnres_swiglu_backward launch");
+  return launched([&] { return attnres::swiglu_launch(true, dtype, a, st); },
+                  "attnres_swiglu_backward launch");
 }
 
 int attnres_kv4_append(void* k_codes, void* k_params, void* v_codes, void* v_params, int64_t num_pages, int kv_heads,
@@ -301,7 +313,8 @@ int attnres_kv4_append(void* k_codes, void* k_params, void* v_codes, void* v_par
     a.vs[i] = v_strides[i];
   }
   if ((rc = check_kv4_rows(a))) return rc;
-  return launched(attnres::kv4_append_launch(dtype, a, static_cast<cudaStream_t>(stream)), "attnres_kv4_append launch");
+  return launched([&] { return attnres::kv4_append_launch(dtype, a, static_cast<cudaStream_t>(stream)); },
+                  "attnres_kv4_append launch");
 }
 
 int attnres_kv4_read(const void* k_codes, const void* k_params, const void* v_codes, const void* v_params,
@@ -328,7 +341,8 @@ int attnres_kv4_read(const void* k_codes, const void* k_params, const void* v_co
   a.k_out = k;
   a.v_out = v;
   if ((rc = check_kv4_rows(a))) return rc;
-  return launched(attnres::kv4_read_launch(dtype, a, static_cast<cudaStream_t>(stream)), "attnres_kv4_read launch");
+  return launched([&] { return attnres::kv4_read_launch(dtype, a, static_cast<cudaStream_t>(stream)); },
+                  "attnres_kv4_read launch");
 }
 
 size_t attnres_kv4_attention_workspace_bytes(int kv_heads, int page_size, int head_dim, int max_pages, int batch,
@@ -384,7 +398,7 @@ int attnres_kv4_attention(const void* k_codes, const void* k_params, const void*
   const size_t need = attnres::kv4_attention_workspace_bytes(a);
   if (need && (!workspace || workspace_bytes < need))
     return fail(ATTNRES_ERR_WORKSPACE, "kv4 attention: workspace of %zu bytes, %zu needed", workspace_bytes, need);
-  return launched(attnres::kv4_attention_launch(dtype, a, static_cast<cudaStream_t>(stream)),
+  return launched([&] { return attnres::kv4_attention_launch(dtype, a, static_cast<cudaStream_t>(stream)); },
                   "attnres_kv4_attention launch");
 }
 

@@ -15,7 +15,7 @@
 // with the reciprocal, and elements within 2^-16 of a tie are redone by division, which
 // keeps the codes those of the division. 24006 tokens of 8 heads of 128 in bf16, 129 MB
 // each way: written in 42 us (3.1 TB/s, three quarters of the issue slots taken), read
-// back in 24 us (5.4 TB/s).
+// back in 18.9 us (6.8 TB/s; part of the cache is still in L2).
 #include "common.cuh"
 #include "kv4.h"
 #include "tma.cuh"
@@ -146,9 +146,22 @@ __device__ __forceinline__ Quantised quantise8(const float (&x)[8]) {
 
 // N 32-bit words next to each other.
 template <int N>
-__device__ __forceinline__ void put_words(uint32_t* p, const uint32_t (&w)[N]) {
-  if constexpr (N == 2) *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
-  else *p = w[0];
+__device__ __forceinline__ void put_words(void* p, const uint32_t (&w)[N]) {
+  if constexpr (N == 4) *static_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+  else if constexpr (N == 2) *static_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+  else *static_cast<uint32_t*>(p) = w[0];
+}
+template <int N>
+__device__ __forceinline__ void get_words(const void* p, uint32_t (&w)[N]) {
+  if constexpr (N == 4) {
+    const uint4 x = *static_cast<const uint4*>(p);
+    w[0] = x.x, w[1] = x.y, w[2] = x.z, w[3] = x.w;
+  } else if constexpr (N == 2) {
+    const uint2 x = *static_cast<const uint2*>(p);
+    w[0] = x.x, w[1] = x.y;
+  } else {
+    w[0] = *static_cast<const uint32_t*>(p);
+  }
 }
 
 template <typename T, bool PACKS, int N>
@@ -191,12 +204,18 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(const __grid_constant__
     params[i] = *reinterpret_cast<const uint32_t*>(&p);
   }
   put_words<N>(reinterpret_cast<uint32_t*>(kc) + c * G + at.g, words);
-  if constexpr (N == 2) {
-    *reinterpret_cast<uint32_t*>(vc + 2 * c * G + at.g) = __byte_perm(qv[0].codes, qv[1].codes, 0x5410);
-    *reinterpret_cast<uint32_t*>(vc + (2 * c + 1) * G + at.g) = __byte_perm(qv[0].codes, qv[1].codes, 0x7632);
-  } else {
+  if constexpr (N == 1) {
     vc[2 * c * G + at.g] = static_cast<uint16_t>(qv[0].codes);
     vc[(2 * c + 1) * G + at.g] = static_cast<uint16_t>(qv[0].codes >> 16);
+  } else {
+    uint32_t lower[N / 2], upper[N / 2];  // the groups' half words r = 2 c and 2 c + 1
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) {
+      lower[i] = __byte_perm(qv[2 * i].codes, qv[2 * i + 1].codes, 0x5410);
+      upper[i] = __byte_perm(qv[2 * i].codes, qv[2 * i + 1].codes, 0x7632);
+    }
+    put_words<N / 2>(vc + 2 * c * G + at.g, lower);
+    put_words<N / 2>(vc + (2 * c + 1) * G + at.g, upper);
   }
   if (c < 2) put_words<N>(static_cast<uint32_t*>(c == 0 ? a.c.k_params : a.c.v_params) + row * G + at.g, params);
 }
@@ -239,17 +258,24 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const __grid_constant__ K
   if (quad >= static_cast<unsigned>(a.B) * a.T * a.c.heads * (G / N)) return;
   const GroupRef at = group_ref<N>(a, quad);
   const long long row = kv4_row(a, at);
-  uint32_t kw[N] = {}, vw[N] = {};
-  __half2 kp[N] = {}, vp[N] = {};
+  uint32_t kw[N] = {}, vw[N] = {}, kp[N] = {}, vp[N] = {};
   if (row >= 0) {
-    const uint32_t* kc = reinterpret_cast<const uint32_t*>(static_cast<const unsigned char*>(a.c.k_codes) + row * (a.c.D / 2));
+    const unsigned char* kc = static_cast<const unsigned char*>(a.c.k_codes) + row * (a.c.D / 2);
     const uint16_t* vc = reinterpret_cast<const uint16_t*>(static_cast<const unsigned char*>(a.c.v_codes) + row * (a.c.D / 2));
+    get_words<N>(reinterpret_cast<const uint32_t*>(kc) + c * G + at.g, kw);
+    get_words<N>(static_cast<const uint32_t*>(a.c.k_params) + row * G + at.g, kp);
+    get_words<N>(static_cast<const uint32_t*>(a.c.v_params) + row * G + at.g, vp);
+    if constexpr (N == 1) {
+      vw[0] = vc[2 * c * G + at.g] | (static_cast<uint32_t>(vc[(2 * c + 1) * G + at.g]) << 16);
+    } else {
+      uint32_t lower[N / 2], upper[N / 2];
+      get_words<N / 2>(vc + 2 * c * G + at.g, lower);
+      get_words<N / 2>(vc + (2 * c + 1) * G + at.g, upper);
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      kw[i] = kc[c * G + at.g + i];
-      vw[i] = vc[2 * c * G + at.g + i] | (static_cast<uint32_t>(vc[(2 * c + 1) * G + at.g + i]) << 16);
-      kp[i] = static_cast<const __half2*>(a.c.k_params)[row * G + at.g + i];
-      vp[i] = static_cast<const __half2*>(a.c.v_params)[row * G + at.g + i];
+      for (int i = 0; i < N / 2; ++i) {
+        vw[2 * i] = __byte_perm(lower[i], upper[i], 0x5410);
+        vw[2 * i + 1] = __byte_perm(lower[i], upper[i], 0x7632);
+      }
     }
   } else if (row == -2) {
     atomicOr(&g_kv4_status, kStatusCacheRange);
@@ -257,18 +283,23 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const __grid_constant__ K
   const long long to = static_cast<long long>(quad) * (N * kKv4Group) + c * 8;
 #pragma unroll
   for (int i = 0; i < N; ++i) {
-    store_values<T>(static_cast<T*>(a.k_out) + to + i * kKv4Group, kw[i], kp[i], row >= 0);
-    store_values<T>(static_cast<T*>(a.v_out) + to + i * kKv4Group, vw[i], vp[i], row >= 0);
+    store_values<T>(static_cast<T*>(a.k_out) + to + i * kKv4Group, kw[i], *reinterpret_cast<const __half2*>(&kp[i]), row >= 0);
+    store_values<T>(static_cast<T*>(a.v_out) + to + i * kKv4Group, vw[i], *reinterpret_cast<const __half2*>(&vp[i]), row >= 0);
   }
 }
 
 namespace {
 
-// Two groups a thread where a head's groups come in pairs.
-int groups_a_thread(const Kv4RowsArgs& a) { return a.c.D / kKv4Group % 2 == 0 ? 2 : 1; }
+// Groups a thread, of those that a head has a multiple of: two to write (24006 tokens of 8
+// heads of 128: 42 us; with four 48, the elements of four take registers that keep other
+// warps away), four to read (18.9 us; with two 23.9).
+int groups_a_thread(const Kv4RowsArgs& a, int most) {
+  const int G = a.c.D / kKv4Group;
+  return most == 4 && G % 4 == 0 ? 4 : (G % 2 == 0 ? 2 : 1);
+}
 
-unsigned blocks_of(const Kv4RowsArgs& a) {
-  const long long threads = 4LL * a.B * a.T * a.c.heads * (a.c.D / kKv4Group / groups_a_thread(a));
+unsigned blocks_of(const Kv4RowsArgs& a, int groups) {
+  const long long threads = 4LL * a.B * a.T * a.c.heads * (a.c.D / kKv4Group / groups);
   return static_cast<unsigned>((threads + 255) / 256);
 }
 
@@ -276,17 +307,18 @@ template <typename T>
 cudaError_t append_t(const Kv4RowsArgs& a, cudaStream_t st) {
   bool packs = (reinterpret_cast<uintptr_t>(a.k) & 15u) == 0 && (reinterpret_cast<uintptr_t>(a.v) & 15u) == 0;
   for (int i = 0; i < 3; ++i) packs = packs && a.ks[i] * sizeof(T) % 16 == 0 && a.vs[i] * sizeof(T) % 16 == 0;
-  const bool two = groups_a_thread(a) == 2;
-  const auto fn = packs ? (two ? kv4_append_kernel<T, true, 2> : kv4_append_kernel<T, true, 1>)
-                        : (two ? kv4_append_kernel<T, false, 2> : kv4_append_kernel<T, false, 1>);
-  fn<<<blocks_of(a), 256, 0, st>>>(a);
+  const int n = groups_a_thread(a, 2);
+  const auto fn = packs ? (n == 2 ? kv4_append_kernel<T, true, 2> : kv4_append_kernel<T, true, 1>)
+                        : (n == 2 ? kv4_append_kernel<T, false, 2> : kv4_append_kernel<T, false, 1>);
+  fn<<<blocks_of(a, n), 256, 0, st>>>(a);
   return cudaGetLastError();
 }
 
 template <typename T>
 cudaError_t read_t(const Kv4RowsArgs& a, cudaStream_t st) {
-  const auto fn = groups_a_thread(a) == 2 ? kv4_read_kernel<T, 2> : kv4_read_kernel<T, 1>;
-  fn<<<blocks_of(a), 256, 0, st>>>(a);
+  const int n = groups_a_thread(a, 4);
+  const auto fn = n == 4 ? kv4_read_kernel<T, 4> : n == 2 ? kv4_read_kernel<T, 2> : kv4_read_kernel<T, 1>;
+  fn<<<blocks_of(a, n), 256, 0, st>>>(a);
   return cudaGetLastError();
 }
 
