@@ -45,11 +45,11 @@ namespace attnres {
 static __device__ unsigned int g_swiglu_status = 0;
 
 constexpr int kGmM = 256, kGmK = 64;  // rows of a pair's tile, columns of a stage
-constexpr int kGmRing = 5 * 32768;    // bytes of stages
-constexpr int kGmBuf = 32 * 128;      // 32 rows x 64 outputs of an epilogue warp; two each
+constexpr int kGmBuf = 32 * 128;      // 32 rows x 64 outputs of an epilogue warp
 constexpr int kGmEpiWarps = 8;
 constexpr int kGmThreads = (2 + kGmEpiWarps) * 32;
-constexpr size_t kGmSmem = 1024 + kGmRing + kGmEpiWarps * 2 * kGmBuf + 512;
+constexpr int kGmShared = 7 * 32768;  // bytes of the ring and of the epilogue's buffers
+constexpr size_t kGmSmem = 1024 + kGmShared + 512;
 
 enum GemmMode { kGateForward, kGateBackward, kGradients };
 
@@ -189,18 +189,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGmThreads, 1)
     swiglu_gemm_kernel(const __grid_constant__ GemmArgs a) {
   constexpr bool GATE = MODE != kGradients;
   // Bytes of each CTA: 64 columns of A and of B, and SUB of those a stage: a stage costs its
-  // issuer 0.16 us besides the products, as much as those of 64 columns of a narrow tile.
-  constexpr int SUB = BN == 128 ? 2 : 1;
+  // issuer 0.16 us besides the products, as much as those of 64 columns of a narrow tile
+  // (wide tiles, dx and dW of 16384 tokens: 365 us with 128 columns a stage, 385 with 64).
+  // (The gate backward's second output buffers leave its wide tiles no room for that.)
+  constexpr int BUFS = MODE == kGateBackward ? 2 : 1, kRing = kGmShared - kGmEpiWarps * BUFS * kGmBuf;
+  constexpr int SUB = BN == 128 || BUFS == 1 ? 2 : 1;
   constexpr uint32_t kA = 128 * kGmK * 2, kB = BN / 2 * kGmK * 2, kSub = kA + kB, kStage = SUB * kSub;
-  constexpr int STAGES = kGmRing / kStage, F = BN / 2;                               // F: outputs of a gate tile
+  constexpr int STAGES = kRing / kStage, F = BN / 2;                               // F: outputs of a gate tile
   // 64 columns a chunk; a gate tile of one chunk goes to either half of the epilogue warps in turn
   constexpr int CHUNKS = GATE ? F / 64 : BN / 64;
   constexpr bool ALTERNATE = CHUNKS == 1;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* stages =
       reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  unsigned char* bufs = stages + kGmRing;  // [epilogue warps][2] output buffers
-  uint64_t* full = reinterpret_cast<uint64_t*>(bufs + kGmEpiWarps * 2 * kGmBuf);  // the even CTA's are used
+  unsigned char* bufs = stages + kRing;  // [epilogue warps][BUFS] output buffers
+  uint64_t* full = reinterpret_cast<uint64_t*>(bufs + kGmEpiWarps * BUFS * kGmBuf);  // the even CTA's are used
   uint64_t* empty = full + STAGES;
   uint64_t* acc_full = empty + STAGES;
   uint64_t* acc_empty = acc_full + 2;  // the even CTA's are used
@@ -351,8 +354,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGmThreads, 1)
     const int q = warp & 3, half = (warp - 2) >> 2;
     const uint32_t lane_off = static_cast<uint32_t>(q * 32) << 16;
     const uint32_t freed[2] = {map_to_rank(smem_u32(&acc_empty[0]), 0), map_to_rank(smem_u32(&acc_empty[1]), 0)};
-    unsigned char* buf0 = bufs + (warp - 2) * 2 * kGmBuf;
-    unsigned char* buf1 = buf0 + kGmBuf;
+    unsigned char* buf0 = bufs + (warp - 2) * BUFS * kGmBuf;
+    unsigned char* buf1 = buf0 + (BUFS - 1) * kGmBuf;
     uint64_t* dh_bar = &dh_full[warp - 2];
     const int row0 = rank * 128 + q * 32, step = ALTERNATE ? 2 : 1;
     auto fetch_dh = [&](const TileRef& t) {  // lane 0, once buf0 is free
@@ -435,7 +438,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGmThreads, 1)
 #pragma unroll 1
         for (int k = 0; k < CHUNKS / 2; ++k) {
           const int chunk = half * (CHUNKS / 2) + k;
-          unsigned char* buf = k & 1 ? buf1 : buf0;
 #pragma unroll
           for (int c = 0; c < 64; c += 32) {
             uint32_t r[2][16];
@@ -449,7 +451,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGmThreads, 1)
               float y[8];
 #pragma unroll
               for (int e = 0; e < 8; ++e) y[e] = __uint_as_float(r[j >> 1][(j & 1) * 8 + e]);
-              store8<T>(reinterpret_cast<T*>(piece_at(buf, lane, c / 8 + j)), y);
+              store8<T>(reinterpret_cast<T*>(piece_at(buf0, lane, c / 8 + j)), y);
             }
           }
           if (k == CHUNKS / 2 - 1) tc_fence_before();
@@ -458,9 +460,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGmThreads, 1)
           if (lane == 0) {
             if (k == CHUNKS / 2 - 1) mbar_arrive_cluster(freed[ab]);
             const int c0 = t.n * BN + chunk * 64;
-            if (c0 < g.cols && r0 < g.M) tma_store_2d(&g.out, c0, r0, buf);
+            if (c0 < g.cols && r0 < g.M) tma_store_2d(&g.out, c0, r0, buf0);
             bulk_commit_group();
-            if (k == CHUNKS / 2 - 1) bulk_wait_group_read0();  // both buffers free for the next tile
+            bulk_wait_group_read0();
           }
           __syncwarp();
         }
