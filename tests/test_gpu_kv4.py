@@ -1,13 +1,13 @@
 """The 4-bit cache on the GPU: kv4_append / kv4_read against the quantiser's definition,
 kv4_attention against a float64 softmax over the values that the cache stands for.
 
-Tolerances of the attention. Weights times step are rounded to the data's type before
-they multiply (r = 2^-8 bf16, 2^-11 f16 of each term; independent, so four times the
-root of the sum of the squares bounds their sum), the output is rounded once, and the
-fp32 sums behind a score, whose terms carry the offset 128 or 1024 of the codes, leave
-it off by at most 2^-13 at these sizes (sqrt(128) terms of |q| <= 5 times 1024 times
-2^-24, times a step below 1 and the scale), which moves the output by 2^-12 of the
-weighted sum of |v| at most.
+Tolerances of the attention, with r = 2^-8 for bf16 and 2^-11 for f16 outputs. Weights and
+values are rounded to f16 before they are multiplied, which leaves each term of the
+output's sum within r of itself; the roundings are independent, so four times r times the
+root of the sum of the terms' squares bounds their sum. The output is rounded once. The fp32
+sums behind a score leave it off by less than 2^-13 at these sizes (sums of up to 128
+products of |q| <= 5 with codes up to 15, times a step below 1 and the scale), which moves
+the output by 2^-12 of the weighted sum of |v| at most.
 """
 import pytest
 import torch
