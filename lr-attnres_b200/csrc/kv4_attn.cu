@@ -5,7 +5,10 @@
 // Token t of a sequence with `length` keys and `count` new tokens stands at place
 // length - count + t and sees the places up to its own. Query head h reads key head
 // h / (Hq / Hkv): the query heads of one key head, times the new tokens, are the rows
-// that share one pass over its keys. A row that sees nothing gives zeros.
+// that share one pass over its keys. A row that sees nothing gives zeros: its sum of
+// weights is 0, which no row that sees a place has. A row with a score that is NaN, or with
+// an infinity or NaN in its query, is NaN by its sum; the maximum alone does not tell
+// (comparisons drop NaN, so it stays -inf over NaN scores).
 //
 // One pass with the running maximum and sum of the softmax. The products run on
 // mma.sync with the cache as the 16-row operand and the query rows as its 8 columns
@@ -260,9 +263,10 @@ __global__ void __launch_bounds__(kAtWarps * 32, NT == 1 ? (D == 64 ? 5 : 4) : 2
     }
 #pragma unroll
     for (int s = 1; s < 4; s <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, s));
-    // 2^(10 - exponent of the largest element), from the exponent's bits; 1 for an infinity
+    // 2^(10 - exponent of the largest element), from the exponent's bits. An infinity makes
+    // the row NaN: its scores are infinite or NaN, and over infinite ones the softmax is NaN.
     const int exponent = __float_as_int(most) >> 23;
-    const float up = exponent == 255 ? 1.f : __int_as_float(min(264 - exponent, 250) << 23);
+    const float up = exponent == 255 ? __int_as_float(0x7fffffff) : __int_as_float(min(264 - exponent, 250) << 23);
 #pragma unroll
     for (int i = 0; i < G; ++i) {
       uint32_t w[4];
@@ -577,9 +581,9 @@ __global__ void __launch_bounds__(kAtWarps * 32, NT == 1 ? (D == 64 ? 5 : 4) : 2
     if (L.splits == 1) {
       const long long to_row = out_index(L, b, h, row);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) y[e] = top == -INFINITY ? 0.f : y[e] / total;
+      for (int e = 0; e < 4; ++e) y[e] = total == 0.f ? 0.f : y[e] / total;
       store_pack<T, 4>(static_cast<T*>(a.out) + to_row * D + d, y);
-      if (a.lse && d == 0) a.lse[to_row] = top == -INFINITY ? -INFINITY : (top + log2f(total)) / kLog2e;
+      if (a.lse && d == 0) a.lse[to_row] = total == 0.f ? -INFINITY : (top + log2f(total)) / kLog2e;
     } else {
       store_pack<float, 4>(L.part_o + (unit * ROWS + r) * D + d, y);
       if (d == 0) L.part_ml[unit * ROWS + r] = make_float2(top, total);
@@ -611,16 +615,14 @@ __global__ void __launch_bounds__(128) kv4_join_kernel(const __grid_constant__ A
   __syncthreads();
   top = fmaxf(fmaxf(warp_top[0], warp_top[1]), fmaxf(warp_top[2], warp_top[3]));
   float y[VEC] = {}, total = 0.f;
-  if (top != -INFINITY) {
 #pragma unroll 4
-    for (int s = warp; s < n; s += 4) {
-      const float2 x = ml[static_cast<long long>(s) * tile_rows];
-      const Pack<float, VEC> p = load_pack<float, VEC>(part + static_cast<long long>(s) * tile_rows * D);
-      const float f = x.x == -INFINITY ? 0.f : exp2f(x.x - top);
-      total += f * x.y;
+  for (int s = warp; s < n; s += 4) {
+    const float2 x = ml[static_cast<long long>(s) * tile_rows];
+    const Pack<float, VEC> p = load_pack<float, VEC>(part + static_cast<long long>(s) * tile_rows * D);
+    const float f = x.x == -INFINITY ? 0.f : exp2f(x.x - top);
+    total += f * x.y;  // NaN where the stretch's sum is, whatever f
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) y[e] += f * p.e[e];
-    }
+    for (int e = 0; e < VEC; ++e) y[e] += f * p.e[e];
   }
 #pragma unroll
   for (int e = 0; e < VEC; ++e) warp_sum_of[warp][lane * VEC + e] = y[e];
@@ -631,9 +633,9 @@ __global__ void __launch_bounds__(128) kv4_join_kernel(const __grid_constant__ A
   if (threadIdx.x < D) {
     const int d = threadIdx.x;
     const float v = (warp_sum_of[0][d] + warp_sum_of[1][d]) + (warp_sum_of[2][d] + warp_sum_of[3][d]);
-    static_cast<T*>(a.out)[to_row * D + d] = Elem<T>::from_f(top == -INFINITY ? 0.f : v / total);
+    static_cast<T*>(a.out)[to_row * D + d] = Elem<T>::from_f(total == 0.f ? 0.f : v / total);
   }
-  if (a.lse && threadIdx.x == 0) a.lse[to_row] = top == -INFINITY ? -INFINITY : (top + log2f(total)) / kLog2e;
+  if (a.lse && threadIdx.x == 0) a.lse[to_row] = total == 0.f ? -INFINITY : (top + log2f(total)) / kLog2e;
 }
 
 namespace {
