@@ -27,8 +27,9 @@
 // in their keys read different halves of the banks.
 //
 // A value that some rows may not see must not reach them as 0 * NaN: in the stage
-// around a sequence's end, values that nobody sees count as zero, and so do those with
-// an infinity or NaN, which turn the rows that do see them into NaN through their sum.
+// around a sequence's end, values that nobody sees count as zero, and so do groups with
+// an infinity or NaN, which are written into the sums of the rows that do see them as the
+// NaN that any weight for them makes, 0 included.
 //
 // A CTA takes a stretch of places of one (sequence, key head, 8 NT query rows); its four
 // warps walk through it 32 or 64 places at a time, each with a ring of its own that bulk
@@ -430,18 +431,30 @@ __global__ void __launch_bounds__(kAtWarps * 32, NT == 1 ? (D == 64 ? 5 : 4) : 2
       }
       if constexpr (MASKED) {
         const int key0 = mt * 16 + (g ^ swap);
+        uint32_t odd = 0;  // bit 4 e + i: group i of key key0 + 8 e has an infinity or NaN
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           uint32_t mine[G];
           load_words<G>(vp + (key0 + 8 * e) * 4 * G, mine);
-          bool odd = false;
 #pragma unroll
-          for (int i = 0; i < G; ++i) odd |= not_finite(mine[i]);
+          for (int i = 0; i < G; ++i) odd |= static_cast<uint32_t>(not_finite(mine[i])) << (4 * e + i);
+        }
+        if (__any_sync(0xffffffffu, odd != 0)) {
+          const int end = rows16[stage * PIECES + mt] >= 0 ? to : 0;
 #pragma unroll
           for (int j = 0; j < NT; ++j)
 #pragma unroll
-            for (int r = 0; r < 2; ++r)
-              if (odd && z[mt][j][2 * e + r] > 0.f) l[j][r] = __int_as_float(0x7fffffff);
+            for (int r = 0; r < 2; ++r) {
+              uint32_t seen = 0;  // groups of this lane's two keys that row 8 j + 2 c + r sees
+              if (at + key0 < min(end, last[j][r] + 1)) seen |= odd & 15u;
+              if (at + key0 + 8 < min(end, last[j][r] + 1)) seen |= odd >> 4;
+#pragma unroll
+              for (int i = 0; i < G; ++i)
+                if (__ballot_sync(0xffffffffu, (seen >> i) & 1u) & (0x11111111u << c)) {
+                  const float nan = __int_as_float(0x7fffffff);
+                  o[j][2 * i][r] = o[j][2 * i][2 + r] = o[j][2 * i + 1][r] = o[j][2 * i + 1][2 + r] = nan;
+                }
+            }
         }
       }
       // the weights in f16; for f16 outputs also what that rounding left, as a second product:
