@@ -29,7 +29,9 @@
 // A value that some rows may not see must not reach them as 0 * NaN: in the stage
 // around a sequence's end, values that nobody sees count as zero, and so do groups with
 // an infinity or NaN, which are written into the sums of the rows that do see them as the
-// NaN that any weight for them makes, 0 included.
+// NaN that any weight for them makes, 0 included. Groups whose largest value lies beyond
+// f16 (finite step and low reach 2^20) are multiplied in units of 2^5. A stage takes the
+// longer way that looks at all this if it lies around an end or its value params ask for it.
 //
 // A CTA takes a stretch of places of one (sequence, key head, 8 NT query rows); its four
 // warps walk through it 32 or 64 places at a time, each with a ring of its own that bulk
@@ -94,6 +96,10 @@ __device__ __forceinline__ uint32_t half_fma(uint32_t a, uint32_t b, uint32_t c)
                             *reinterpret_cast<const __half2*>(&c));
   return *reinterpret_cast<const uint32_t*>(&r);
 }
+__device__ __forceinline__ uint32_t half_mul(uint32_t a, uint32_t b) {
+  const __half2 r = __hmul2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
 __device__ __forceinline__ uint32_t half_pack(float a, float b) {
   const __half2 r = __floats2half2_rn(a, b);
   return *reinterpret_cast<const uint32_t*>(&r);
@@ -101,6 +107,19 @@ __device__ __forceinline__ uint32_t half_pack(float a, float b) {
 // Whether either half of a pair of params is an infinity or NaN.
 __device__ __forceinline__ bool not_finite(uint32_t p) {
   return (p & 0x7c00u) == 0x7c00u || (p & 0x7c000000u) == 0x7c000000u;
+}
+
+// Whether one of two groups has a value beyond f16 or none at all: low + 15 step, rounded,
+// is infinite or NaN. steps, lows: the two groups' params, taken apart.
+__device__ __forceinline__ bool leaves_f16(uint32_t steps, uint32_t lows) {
+  return not_finite(half_fma(steps, 0x4b804b80u, lows));
+}
+// The same over the value params of a stage, four groups a lane.
+__device__ __forceinline__ bool stage_leaves_f16(const unsigned char* params, int lane) {
+  const uint4 p = *reinterpret_cast<const uint4*>(params + lane * 16);
+  const bool mine = leaves_f16(__byte_perm(p.x, p.y, 0x5410u), __byte_perm(p.x, p.y, 0x7632u)) ||
+                    leaves_f16(__byte_perm(p.z, p.w, 0x5410u), __byte_perm(p.z, p.w, 0x7632u));
+  return __any_sync(0xffffffffu, mine);
 }
 
 __device__ __forceinline__ uint32_t transposed(uint32_t x) {
@@ -142,6 +161,10 @@ __device__ __forceinline__ void load_words(const unsigned char* p, uint32_t (&w)
     w[0] = *reinterpret_cast<const uint32_t*>(p);
   }
 }
+
+enum StageKind { kPlain, kMasked, kCareful };
+template <StageKind K>
+using Kind = std::integral_constant<StageKind, K>;
 
 // Sequence b's keys and new tokens: the length clipped to what its page table can hold.
 struct SeqFacts {
@@ -310,10 +333,12 @@ __global__ void __launch_bounds__(kAtWarps * 32, NT == 1 ? (D == 64 ? 5 : 4) : 2
 #pragma unroll
   for (int j = 0; j < NT; ++j) m[j][0] = m[j][1] = -INFINITY;
   const int swap = (g >> 1) & 1;          // keys in the order i ^ ((i >> 1) & 1)
-  // One stage. MASKED: some of its places may not be seen by some row; a copy of its own,
-  // as the tests, predicated away, would still take a third of the common one's issue slots.
-  auto attend = [&](const unsigned char* kc, int at, int stage, auto masked) {
-    constexpr bool MASKED = decltype(masked)::value;
+  // One stage, in three copies: as tests that are predicated away, what the rarer ones do
+  // besides would take a third of the common one's issue slots. MASKED: some of its places
+  // may not be seen by some row. CAREFUL: some value params, of any place, are not finite or
+  // stand for values beyond f16 (in places that were not fetched, anything may).
+  auto attend = [&](const unsigned char* kc, int at, int stage, auto kind) {
+    constexpr bool MASKED = decltype(kind)::value != kPlain, CAREFUL = decltype(kind)::value == kCareful;
     const unsigned char* vc = kc + kCode;
     const unsigned char* kp = kc + 2 * kCode;
     const unsigned char* vp = kp + kParam;
@@ -426,10 +451,10 @@ __global__ void __launch_bounds__(kAtWarps * 32, NT == 1 ? (D == 64 ? 5 : 4) : 2
           const bool there = rows16[stage * PIECES + mt] >= 0 && at + key < to;
 #pragma unroll
           for (int i2 = 0; i2 < G; ++i2)
-            if (!there || not_finite(par[k][i2])) par[k][i2] = 0;
+            if (!there || (CAREFUL && not_finite(par[k][i2]))) par[k][i2] = 0;
         }
       }
-      if constexpr (MASKED) {
+      if constexpr (CAREFUL) {
         const int key0 = mt * 16 + (g ^ swap);
         uint32_t odd = 0;  // bit 4 e + i: group i of key key0 + 8 e has an infinity or NaN
 #pragma unroll
@@ -477,6 +502,32 @@ __global__ void __launch_bounds__(kAtWarps * 32, NT == 1 ? (D == 64 ? 5 : 4) : 2
       for (int i = 0; i < G; ++i) {
         const uint32_t pick = (i & 1) ? 0x7632u : 0x5410u;
         uint32_t f[2][4];
+        uint32_t wa[PARTS][NT], wb[PARTS][NT];
+#pragma unroll
+        for (int part = 0; part < PARTS; ++part)
+#pragma unroll
+          for (int j = 0; j < NT; ++j) {
+            wa[part][j] = pa[part][j];
+            wb[part][j] = pb[part][j];
+          }
+        if constexpr (CAREFUL) {
+          bool beyond = false;
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            beyond |= leaves_f16(__byte_perm(par[2 * e][i], par[2 * e + 1][i], 0x5410u),
+                                 __byte_perm(par[2 * e][i], par[2 * e + 1][i], 0x7632u));
+          if (__any_sync(0xffffffffu, beyond)) {  // the values by 2^-5, the weights (up to 2^kSlack) by 2^5
+#pragma unroll
+            for (int k = 0; k < 4; ++k) par[k][i] = half_mul(par[k][i], 0x28002800u);
+#pragma unroll
+            for (int part = 0; part < PARTS; ++part)
+#pragma unroll
+              for (int j = 0; j < NT; ++j) {
+                wa[part][j] = half_mul(wa[part][j], 0x50005000u);
+                wb[part][j] = half_mul(wb[part][j], 0x50005000u);
+              }
+          }
+        }
 #pragma unroll
         for (int e = 0; e < 2; ++e) {  // the pairs of keys 2c, 2c + 1 and 2c + 8, 2c + 9
           const uint32_t w = __byte_perm(words[2 * e][i >> 1], words[2 * e + 1][i >> 1], pick);
@@ -490,8 +541,8 @@ __global__ void __launch_bounds__(kAtWarps * 32, NT == 1 ? (D == 64 ? 5 : 4) : 2
         for (int part = 0; part < PARTS; ++part)
 #pragma unroll
           for (int j = 0; j < NT; ++j) {
-            mma_16816<__half>(o[j][2 * i], f[0][0], f[0][1], f[1][0], f[1][1], pa[part][j], pb[part][j]);
-            mma_16816<__half>(o[j][2 * i + 1], f[0][2], f[0][3], f[1][2], f[1][3], pa[part][j], pb[part][j]);
+            mma_16816<__half>(o[j][2 * i], f[0][0], f[0][1], f[1][0], f[1][1], wa[part][j], wb[part][j]);
+            mma_16816<__half>(o[j][2 * i + 1], f[0][2], f[0][3], f[1][2], f[1][3], wa[part][j], wb[part][j]);
           }
       }
     }
@@ -515,9 +566,11 @@ __global__ void __launch_bounds__(kAtWarps * 32, NT == 1 ? (D == 64 ? 5 : 4) : 2
       const int2 r = *reinterpret_cast<const int2*>(rows16 + stage * 2);
       rows = r.x | r.y;
     }
+    const unsigned char* const kc = ring + slot * kStage;
+    if (stage_leaves_f16(kc + 2 * kCode + kParam, lane)) attend(kc, at, stage, Kind<kCareful>{});
     // nothing masked: places that are there and that every row sees (least < to)
-    if (rows >= 0 && at + KEYS - 1 <= least) attend(ring + slot * kStage, at, stage, std::false_type{});
-    else attend(ring + slot * kStage, at, stage, std::true_type{});
+    else if (rows >= 0 && at + KEYS - 1 <= least) attend(kc, at, stage, Kind<kPlain>{});
+    else attend(kc, at, stage, Kind<kMasked>{});
     __syncwarp();  // every lane has read the stage
     if (stage + STAGES * kAtWarps < count) fetch(stage + STAGES * kAtWarps, slot);
     if (++slot == STAGES) {
