@@ -564,7 +564,9 @@ int attnres_swiglu_backward(int64_t num_tokens, int in_dim, int hidden, int dtyp
  * (element strides {sequence, token, head}, last dim dense) into places start[b] ..
  * start[b] + counts[b] (counts NULL: new_tokens each):
  *   step = f16((max - min) / 15), low = f16(min), code = clamp(rint((x - low) / step))
- * A group with an infinity or NaN reads back as NaN.
+ * A group with an infinity or NaN reads back as NaN, and so does one whose step or low
+ * overflows float16: a least value beyond +-65504, or a range beyond 15 times that. Within
+ * that, bf16 and fp32 values may exceed 65504 and read back as such.
  * attnres_kv4_read writes the values of the same places, dtype [batch, new_tokens,
  * kv_heads, head_dim] dense, zeros where there is none.
  */

@@ -260,7 +260,8 @@ def kv4_append(cache: KV4Cache, k: Tensor, v: Tensor, page_table: Tensor, start:
     [B, max_pages]; start int32 [B] (how many keys the sequence holds already); counts int32 [B]
     (default T): how many of the T tokens sequence b really has. Step and low are rounded to float16
     and each code is the nearest value to what will be read back. Groups that hold an infinity or a NaN
-    read back as NaN. No gradient."""
+    read back as NaN, and so do those whose step or low overflows float16 (a least value beyond +-65504, or
+    a range beyond 15 times that). No gradient."""
     if _eager(k, v, page_table, start, counts):
         _load().kv4_append(cache.k_codes, cache.k_params, cache.v_codes, cache.v_params, k, v, page_table, start, counts)
     else:

@@ -18,6 +18,11 @@ namespace attnres {
 constexpr int kKv4Group = 32;
 constexpr int kKv4MaxDim = 512;
 
+// Whether either half of a pair of params is an infinity or NaN.
+__device__ __forceinline__ bool not_finite(uint32_t p) {
+  return (p & 0x7c00u) == 0x7c00u || (p & 0x7c000000u) == 0x7c000000u;
+}
+
 struct Kv4Cache {
   void *k_codes, *k_params, *v_codes, *v_params;  // [pages, heads, page, D / 2], [pages, heads, page, G, 2]
   long long pages;

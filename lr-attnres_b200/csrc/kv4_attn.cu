@@ -104,11 +104,6 @@ __device__ __forceinline__ uint32_t half_pack(float a, float b) {
   const __half2 r = __floats2half2_rn(a, b);
   return *reinterpret_cast<const uint32_t*>(&r);
 }
-// Whether either half of a pair of params is an infinity or NaN.
-__device__ __forceinline__ bool not_finite(uint32_t p) {
-  return (p & 0x7c00u) == 0x7c00u || (p & 0x7c000000u) == 0x7c000000u;
-}
-
 // Whether one of two groups has a value beyond f16 or none at all: low + 15 step, rounded,
 // is infinite or NaN. steps, lows: the two groups' params, taken apart.
 __device__ __forceinline__ bool leaves_f16(uint32_t steps, uint32_t lows) {

@@ -3,8 +3,9 @@
 //   step = f16((max - min) / 15), low = f16(min)
 //   code = clamp(rint((x - low) / step), 0, 15), 0 where step is 0
 // with the rounded step and low, so the code is the nearest of the 16 values that will
-// be read back. A group that holds an infinity or a NaN gets NaN for step and low and
-// reads back as NaN.
+// be read back. A group that holds an infinity or a NaN, or whose step or low overflows
+// float16 (a least value that rounds beyond +-65504, a range of 15 times that), gets NaN for step and low
+// and reads back as NaN.
 //
 // Four lanes share a group (8 elements each, two shuffles for its extremes), and a
 // thread does the same part of a key and of its value, of two groups next to each other
@@ -105,10 +106,10 @@ __device__ __forceinline__ Quantised quantise8(const float (&x)[8]) {
     top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
     low = min_nan(low, __shfl_xor_sync(0xffffffffu, low, o));
   }
-  const float range = __fsub_rn(top, low), nan = __int_as_float(0x7fffffff);
-  const bool odd = !(range <= 3.402823466e38f);  // an infinity or a NaN among them
   Quantised r;
-  r.params = odd ? __floats2half2_rn(nan, nan) : __floats2half2_rn(__fmul_rn(range, 1.f / 15.f), low);
+  r.params = __floats2half2_rn(__fmul_rn(__fsub_rn(top, low), 1.f / 15.f), low);
+  // an infinity or a NaN among the elements leaves one here
+  if (not_finite(*reinterpret_cast<const uint32_t*>(&r.params))) r.params = __float2half2_rn(__int_as_float(0x7fffffff));
   const float step = __low2float(r.params), base = __high2float(r.params);
   const float inv = step > 0.f ? __fdividef(1.f / 15.f, step) : 0.f;  // codes of 0 where there is no step
   float worst = 0.f, off[8];
