@@ -583,13 +583,14 @@ int attnres_kv4_read(const void* k_codes, const void* k_params, const void* v_co
  * Attention of new tokens over that cache, their own keys and values in it already.
  * lengths[b] counts the sequence's keys with the new ones; token t < counts[b]
  * (NULL: new_tokens) stands at place lengths[b] - counts[b] + t and sees the places
- * up to its own. q dtype [batch, new_tokens, q_heads, head_dim] with element strides
- * {sequence, token, head}; query head h reads key head h / (q_heads / kv_heads). out
- * dtype [batch, new_tokens, q_heads, head_dim] and lse float [batch, new_tokens,
- * q_heads] (log of the softmax's sum, NULL if not wanted), dense. A row that sees
- * nothing is zeros, its lse -inf. bf16 / fp16, head_dim 64 or 128. Workspace:
- * attnres_kv4_attention_workspace_bytes (may be 0), asked with the device current
- * that the call will run on.
+ * up to its own, as far as its page table goes: a length beyond the table, like a
+ * page that is not there, sets bit 8 of the status word. q dtype [batch, new_tokens,
+ * q_heads, head_dim] with element strides {sequence, token, head}; query head h reads
+ * key head h / (q_heads / kv_heads). out dtype [batch, new_tokens, q_heads, head_dim]
+ * and lse float [batch, new_tokens, q_heads] (log of the softmax's sum, NULL if not
+ * wanted), dense. A row that sees nothing is zeros, its lse -inf. bf16 / fp16, head_dim
+ * 64 or 128. Workspace: attnres_kv4_attention_workspace_bytes (may be 0), asked with the
+ * device current that the call will run on.
  */
 size_t attnres_kv4_attention_workspace_bytes(int kv_heads, int page_size, int head_dim, int max_pages, int batch,
                                              int new_tokens, int q_heads);

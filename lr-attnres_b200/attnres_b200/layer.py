@@ -285,7 +285,7 @@ def kv4_attention(q: Tensor, cache: KV4Cache, page_table: Tensor, lengths: Tenso
     q [B, T, heads, head_dim] float16 or bfloat16, head_dim 64 or 128; query head h reads key head
     h // (heads / kv_heads). lengths int32 [B] counts a sequence's keys, the new ones among them; its
     token t < counts[b] (int32, default T) stands at place lengths[b] - counts[b] + t and sees the
-    places up to its own. scale defaults to head_dim ** -0.5. Returns out [B, T, heads, head_dim] in
+    places up to its own, as far as the table goes (bit 8 of the status word tells of lengths beyond it). scale defaults to head_dim ** -0.5. Returns out [B, T, heads, head_dim] in
     q's type, with return_lse also the log of the softmax's sum, float32 [B, T, heads]. A token that
     sees nothing gives zeros and -inf. Meant for one to a few new tokens: the cache is read once for
     every 16 query rows of a key head. No gradient."""

@@ -161,14 +161,14 @@ enum StageKind { kPlain, kMasked, kCareful };
 template <StageKind K>
 using Kind = std::integral_constant<StageKind, K>;
 
-// Sequence b's keys and new tokens: the length clipped to what its page table can hold.
+// Sequence b's keys and new tokens, and how many of the keys its page table can hold.
 struct SeqFacts {
-  int length, count;
+  int length, count, held;
 };
 __device__ __forceinline__ SeqFacts seq_facts(const Kv4AttnArgs& a, int b) {
   SeqFacts s;
-  const long long room = static_cast<long long>(a.max_pages) * a.c.page;
-  s.length = static_cast<int>(min(static_cast<long long>(max(a.lengths[b], 0)), room));
+  s.length = max(a.lengths[b], 0);
+  s.held = min(s.length, a.max_pages * a.c.page);  // the host refuses tables of more than 2^30 places
   s.count = a.counts ? min(max(a.counts[b], 0), a.T) : a.T;
   return s;
 }
@@ -201,7 +201,8 @@ __global__ void __launch_bounds__(kAtWarps * 32, NT == 1 ? (D == 64 ? 5 : 4) : 2
   const int from = split * L.stretch, first_slot = (from + static_cast<int>(threadIdx.x) * 16) / a.c.page;
   const int first_page = first_slot < a.max_pages ? a.table[b * a.table_stride + first_slot] : -1;
   const SeqFacts seq = seq_facts(a, b);
-  const int to = min(from + L.stretch, seq.length);
+  const int to = min(from + L.stretch, seq.held);
+  if (from == 0 && threadIdx.x == 0 && seq.held < seq.length) atomicOr(&g_kv4_attn_status, kStatusCacheRange);
   // the join may take up its place on the GPU; it waits for this grid's end before it reads
   if (L.splits > 1) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (from >= to && L.splits > 1) return;  // the join knows how many stretches there are
@@ -315,7 +316,7 @@ __global__ void __launch_bounds__(kAtWarps * 32, NT == 1 ? (D == 64 ? 5 : 4) : 2
     }
   }
   if constexpr (SHARED_Q) __syncthreads();
-  int least = 0x7fffffff;  // places up to this one are seen by all rows that see any
+  int least = to - 1;  // places up to this one are seen by all rows that see any
 #pragma unroll
   for (int j = 0; j < NT; ++j)
 #pragma unroll
@@ -563,7 +564,7 @@ __global__ void __launch_bounds__(kAtWarps * 32, NT == 1 ? (D == 64 ? 5 : 4) : 2
     }
     const unsigned char* const kc = ring + slot * kStage;
     if (stage_leaves_f16(kc + 2 * kCode + kParam, lane)) attend(kc, at, stage, Kind<kCareful>{});
-    // nothing masked: places that are there and that every row sees (least < to)
+    // nothing masked: places that are there and that every row sees
     else if (rows >= 0 && at + KEYS - 1 <= least) attend(kc, at, stage, Kind<kPlain>{});
     else attend(kc, at, stage, Kind<kMasked>{});
     __syncwarp();  // every lane has read the stage
@@ -665,7 +666,7 @@ __global__ void __launch_bounds__(128) kv4_join_kernel(const __grid_constant__ A
   const int h = bh % a.c.heads, b = bh / a.c.heads;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const SeqFacts seq = seq_facts(a, b);
-  const int n = (seq.length + L.stretch - 1) / L.stretch;
+  const int n = (seq.held + L.stretch - 1) / L.stretch;
   const long long first = (static_cast<long long>(bh) * L.row_tiles + row / tile_rows) * L.splits * tile_rows + row % tile_rows;
   const float2* ml = L.part_ml + first;  // of stretch s: s * tile_rows on
   const float* part = L.part_o + first * D + lane * VEC;
