@@ -85,18 +85,39 @@ def norm_heads(x: Tensor, heads: int) -> Tensor:
 class RotaryEmbedding(nn.Module):
     def __init__(self, cfg: GPTConfig):
         super().__init__()
-        dim = cfg.n_embd // cfg.n_head
-        inv_freq = 1.0 / (cfg.rope_theta ** (torch.arange(0, dim, 2) / dim))
-        freq = torch.outer(torch.arange(cfg.block_size), inv_freq)
-        self.register_buffer("sin", freq.sin()[None, None])
-        self.register_buffer("cos", freq.cos()[None, None])
-        # [block_size, head_dim / 2] float32 whatever the module is cast to: what qk_norm_rope takes
-        self.tables = (freq.cos().contiguous(), freq.sin().contiguous())
+        self.cfg = cfg
+        cos, sin = self._angles()
+        self.register_buffer("sin", sin[None, None])
+        self.register_buffer("cos", cos[None, None])
+        self._exact = cos.float().clone(), sin.float().clone()
+
+    def _angles(self, device=None):
+        """Cosines and sines [block_size, head_dim / 2] of the config."""
+        dim = self.cfg.n_embd // self.cfg.n_head
+        inv_freq = 1.0 / (self.cfg.rope_theta ** (torch.arange(0, dim, 2, device=device) / dim))
+        freq = torch.outer(torch.arange(self.cfg.block_size, device=device), inv_freq)
+        return freq.cos(), freq.sin()
+
+    @property
+    def tables(self):
+        """Cosines and sines as qk_norm_rope takes them: [block_size, head_dim / 2] on the module's device, float32
+        whatever it is cast to."""
+        device = self.sin.device
+        if self._exact[0].device == device:
+            return self._exact
+        if self._exact[0].is_meta:  # the module was built without data
+            self._exact = self._angles("cpu")
+        self._exact = tuple(t.to(device, torch.float32) for t in self._exact)
+        return self._exact
 
     def _apply(self, fn, recurse=True):
         super()._apply(fn, recurse)
-        self.tables = tuple(t.to(self.sin.device) for t in self.tables)  # follow the module's device, not its type
+        self.tables  # moved with the module, on the same stream
         return self
+
+    def _load_from_state_dict(self, *args, **kwargs):
+        super()._load_from_state_dict(*args, **kwargs)
+        self.tables
 
     def rotate(self, x: Tensor) -> Tensor:
         T = x.size(-2)
