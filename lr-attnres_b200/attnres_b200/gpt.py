@@ -90,6 +90,7 @@ class RotaryEmbedding(nn.Module):
         self.register_buffer("sin", sin[None, None])
         self.register_buffer("cos", cos[None, None])
         self._exact = cos.float().clone(), sin.float().clone()
+        self._made = None
 
     def _angles(self, device=None):
         """Cosines and sines [block_size, head_dim / 2] of the config."""
@@ -100,19 +101,39 @@ class RotaryEmbedding(nn.Module):
 
     @property
     def tables(self):
-        """Cosines and sines as qk_norm_rope takes them: [block_size, head_dim / 2] on the module's device, float32
-        whatever it is cast to."""
-        device = self.sin.device
-        if self._exact[0].device == device:
-            return self._exact
-        if self._exact[0].is_meta:  # the module was built without data
-            self._exact = self._angles("cpu")
-        self._exact = tuple(t.to(device, torch.float32) for t in self._exact)
-        return self._exact
+        """Cosines and sines as qk_norm_rope takes them: [block_size, head_dim / 2] float32 on the module's device, of
+        the values that its cos and sin buffers hold. Made again when a buffer was replaced or written to."""
+        buffers = self.cos, self.sin
+        if torch.compiler.is_compiling():
+            return self._follow(buffers)
+        versions = tuple(None if b.is_inference() else b._version for b in buffers)
+        if self._made is not None:
+            of, at, made = self._made
+            if of[0] is buffers[0] and of[1] is buffers[1] and at == versions:
+                return made
+        made = self._follow(buffers)
+        if made[0].is_cuda:
+            if torch.cuda.is_current_stream_capturing():
+                return made  # the graph's own
+            torch.cuda.current_stream(made[0].device).synchronize()  # any stream may use them next
+        self._made = buffers, versions, made
+        return made
+
+    def _follow(self, buffers):
+        """The buffers in float32. Where a 16-bit buffer holds the config's values rounded, the values (chosen on the
+        device: nothing waits for it)."""
+        device = buffers[0].device
+        if self._exact[0].device != device and not torch.compiler.is_compiling():
+            if self._exact[0].is_meta:  # the module was built without data
+                self._exact = self._angles("cpu")
+            self._exact = tuple(t.to(device, torch.float32) for t in self._exact)
+        return tuple(b[0, 0] if b.dtype == torch.float32
+                     else torch.where((b[0, 0] == e.to(b.dtype)).all(), e, b[0, 0].float())
+                     for b, e in zip(buffers, self._exact))
 
     def _apply(self, fn, recurse=True):
         super()._apply(fn, recurse)
-        self.tables  # moved with the module, on the same stream
+        self.tables  # made here rather than in the middle of a step
         return self
 
     def _load_from_state_dict(self, *args, **kwargs):
