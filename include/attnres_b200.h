@@ -51,7 +51,9 @@ extern "C" {
 typedef enum attnres_dtype {
   ATTNRES_DTYPE_F32 = 0,
   ATTNRES_DTYPE_F16 = 1,
-  ATTNRES_DTYPE_BF16 = 2
+  ATTNRES_DTYPE_BF16 = 2,
+  /* or'ed into the dtype of attnres_qk_norm_rope_*: its norm weights and their gradients are float */
+  ATTNRES_WEIGHTS_F32 = 0x100
 } attnres_dtype;
 
 typedef enum attnres_status {
@@ -499,12 +501,13 @@ int attnres_base_backward(int num_sources, int64_t num_tokens, int value_dim, in
  * positions_are_64) [num_tokens], NULL for n % seq_len. A position outside
  * [0, table_rows) makes the rotated elements of the token's q and k NaN. interleaved: pairs
  * (2i, 2i+1), else (i, i + rotary_dim/2). normalize 0 leaves the norm out.
- * q_weight / k_weight dtype [head_dim] or NULL. q [num_tokens, q_heads, head_dim],
+ * q_weight / k_weight dtype (float with ATTNRES_WEIGHTS_F32 or'ed into dtype)
+ * [head_dim] or NULL. q [num_tokens, q_heads, head_dim],
  * k, v [num_tokens, kv_heads, head_dim], dense. head_dim up to 512.
  *
  * Backward: grad_q/k/v dtype with element strides grad_strides[9] = {sequence,
- * token, head} of each, last dim dense; grad_qkv dense; weight gradients dtype
- * [head_dim], NULL where not wanted, summed over tokens and heads in fp32 in a
+ * token, head} of each, last dim dense; grad_qkv dense; weight gradients of the
+ * weights' type [head_dim], NULL where not wanted, summed over tokens and heads in fp32 in a
  * fixed order, and only they need the workspace.
  */
 int attnres_qk_norm_rope_forward(int64_t num_tokens, int64_t seq_len, int q_heads, int kv_heads, int head_dim,

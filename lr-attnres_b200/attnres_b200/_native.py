@@ -10,6 +10,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libattnres_b200.so")
 
 DTYPE_F32, DTYPE_F16, DTYPE_BF16 = 0, 1, 2
+WEIGHTS_F32 = 0x100  # or'ed into the dtype of attnres_qk_norm_rope_*
 QUERY_STATIC, QUERY_DYNAMIC, QUERY_GATED = 0, 1, 2
 NORM_NONE, NORM_PER_HEAD, NORM_ROW = 0, 1, 2
 MAX_SOURCES = 64

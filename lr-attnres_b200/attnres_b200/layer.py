@@ -119,7 +119,8 @@ def qk_norm_rope(qkv: Tensor, num_heads: int, num_kv_heads: int, cos: Tensor, si
     positions [B, T] int32 or int64 (default: the token's index in its sequence); a token whose
     position lies outside the tables gets NaN in the rotated elements of its queries and keys. interleaved pairs elements
     (2i, 2i + 1), otherwise (i, i + rotary_dim / 2). q_weight, k_weight [head_dim] multiply the normed
-    heads. normalize=False leaves the norm out; eps defaults to float32's, as the model's norms have it.
+    heads in their own type (float32 weights beside a 16-bit qkv are not rounded to it, nor their
+    gradients). normalize=False leaves the norm out; eps defaults to float32's, as the model's norms have it.
     Differentiable in qkv and the weights."""
     eps = F32_EPS if eps is None else eps
     if _eager(qkv, cos, sin, positions, q_weight, k_weight):

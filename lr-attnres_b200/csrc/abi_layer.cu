@@ -38,8 +38,11 @@ bool known_dtype(int dtype) {
   return dtype == ATTNRES_DTYPE_F32 || dtype == ATTNRES_DTYPE_F16 || dtype == ATTNRES_DTYPE_BF16;
 }
 
+// Whether dtype asks for fp32 norm weights beside 16-bit data (fp32 data has none other).
+int weights_f32(int dtype) { return (dtype & ATTNRES_WEIGHTS_F32) && dtype != (ATTNRES_DTYPE_F32 | ATTNRES_WEIGHTS_F32); }
+
 int check_qk_norm_rope(const attnres::QkRopeArgs& a, int dtype) {
-  if (!known_dtype(dtype)) return fail(ATTNRES_ERR_INVALID_ARGUMENT, "unknown dtype %d", dtype);
+  if (!known_dtype(dtype & ~ATTNRES_WEIGHTS_F32)) return fail(ATTNRES_ERR_INVALID_ARGUMENT, "unknown dtype %d", dtype);
   if (a.N < 0 || a.T < 1 || a.N % a.T)
     return fail(ATTNRES_ERR_INVALID_ARGUMENT, "qk norm rope: num_tokens=%lld must be a multiple of seq_len=%lld", a.N, a.T);
   if (a.Hq < 1 || a.Hkv < 1 || a.D < 1 || a.Hq > 4096 || a.Hkv > 4096)
@@ -168,6 +171,8 @@ int attnres_qk_norm_rope_forward(int64_t num_tokens, int64_t seq_len, int q_head
                                        k_weight, normalize, eps, interleaved);
   int rc = check_qk_norm_rope(a, dtype);
   if (rc || num_tokens == 0) return rc;
+  a.w32 = weights_f32(dtype);
+  dtype &= ~ATTNRES_WEIGHTS_F32;
   if (!q || !k || !v) return fail(ATTNRES_ERR_INVALID_ARGUMENT, "qk norm rope: an output is NULL");
   a.out[0] = q;
   a.out[1] = k;
@@ -194,11 +199,13 @@ int attnres_qk_norm_rope_backward(int64_t num_tokens, int64_t seq_len, int q_hea
                                        k_weight, normalize, eps, interleaved);
   int rc = check_qk_norm_rope(a, dtype);
   if (rc) return rc;
+  a.w32 = weights_f32(dtype);
+  dtype &= ~ATTNRES_WEIGHTS_F32;
   if ((grad_q_weight && !q_weight) || (grad_k_weight && !k_weight))
     return fail(ATTNRES_ERR_INVALID_ARGUMENT, "qk norm rope backward: a weight gradient without its weight");
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (num_tokens == 0) {
-    const size_t bytes = static_cast<size_t>(head_dim) * (dtype == ATTNRES_DTYPE_F32 ? 4 : 2);
+    const size_t bytes = static_cast<size_t>(head_dim) * (dtype == ATTNRES_DTYPE_F32 || a.w32 ? 4 : 2);
     cudaError_t e = cudaSuccess;
     if (grad_q_weight) e = cudaMemsetAsync(grad_q_weight, 0, bytes, st);
     if (grad_k_weight && e == cudaSuccess) e = cudaMemsetAsync(grad_k_weight, 0, bytes, st);

@@ -79,7 +79,8 @@ struct RopeHow {
 struct RopeCall {
   Tensor qkv, cos, sin, positions, wq, wk;
   int64_t B, T, D, stride;
-  int code, wide;
+  int code, wide;  // the ABI's dtype; 64-bit positions
+  at::ScalarType wtype;
   RopeHow how;
 
   RopeCall(const Tensor& qkv_, const Tensor& cos_, const Tensor& sin_, const Tensor& positions_, const Tensor& wq_,
@@ -124,8 +125,13 @@ struct RopeCall {
     for (const Tensor* w : {&wq_, &wk_})
       TORCH_CHECK(!w->defined() || (w->dim() == 1 && w->size(0) == D),
                   "attnres_b200: qk_norm_rope weights are [head_dim] = [", D, "]");
-    if (wq_.defined()) wq = wq_.to(qkv.scalar_type()).contiguous();
-    if (wk_.defined()) wk = wk_.to(qkv.scalar_type()).contiguous();
+    // weights of the data's type go as they are, others in fp32
+    wtype = qkv.scalar_type();
+    for (const Tensor* w : {&wq_, &wk_})
+      if (w->defined() && w->scalar_type() != qkv.scalar_type()) wtype = at::kFloat;
+    if (wq_.defined()) wq = wq_.to(wtype).contiguous();
+    if (wk_.defined()) wk = wk_.to(wtype).contiguous();
+    if (wtype != qkv.scalar_type()) code |= ATTNRES_WEIGHTS_F32;
   }
   int64_t tokens() const { return B * T; }
   int64_t seq() const { return T > 0 ? T : 1; }
@@ -174,8 +180,8 @@ std::vector<Tensor> rope_backward(const std::array<Tensor, 3>& grads, const Tens
     const Launch on(c.qkv);
     bytes = attnres_qk_norm_rope_backward_workspace_bytes(c.D);
     workspace = fresh(qkv, {static_cast<int64_t>(bytes)}, at::kByte);
-    if (want_wq) dwq = fresh(qkv, {c.D});
-    if (want_wk) dwk = fresh(qkv, {c.D});
+    if (want_wq) dwq = fresh(qkv, {c.D}, c.wtype);
+    if (want_wk) dwk = fresh(qkv, {c.D}, c.wtype);
   }
   const Launch on(c.qkv);
   check_status(attnres_qk_norm_rope_backward(

@@ -34,6 +34,13 @@ __device__ __forceinline__ long long rope_position(const QkRopeArgs& a, long lon
   return (p >= 0 && p < a.table_rows) ? p : -1;
 }
 
+// Element j of the norm weight of the queries (0) or keys (1): fp32 weights multiply as they
+// are, and their gradients are not rounded to the data's type either.
+template <typename T>
+__device__ __forceinline__ float rope_weight(const QkRopeArgs& a, int part, int j) {
+  return a.w32 ? static_cast<const float*>(a.w[part])[j] : Elem<T>::to_f(static_cast<const T*>(a.w[part])[j]);
+}
+
 __device__ __forceinline__ float quiet_nan() { return __int_as_float(0x7fffffff); }
 
 // Which of q / k / v head r of a token is, and its index there.
@@ -77,7 +84,7 @@ __global__ void __launch_bounds__(kRopeWarps * 32) qkrope_fwd_any_kernel(const _
     for (int j = lane; j < a.D; j += 32) y[j] = x[j];
     return;
   }
-  const T* w = static_cast<const T*>(a.w[hr.part]);
+  const bool w = a.w[hr.part] != nullptr;
   float ss = 0.f;
   for (int j = lane; j < a.D; j += 32) {
     const float v = Elem<T>::to_f(x[j]);
@@ -93,8 +100,8 @@ __global__ void __launch_bounds__(kRopeWarps * 32) qkrope_fwd_any_kernel(const _
     const int i0 = a.interleaved ? 2 * i : i, i1 = a.interleaved ? 2 * i + 1 : i + half;
     float u = buf[i0] * inv, v = buf[i1] * inv;
     if (w) {
-      u *= Elem<T>::to_f(w[i0]);
-      v *= Elem<T>::to_f(w[i1]);
+      u *= rope_weight<T>(a, hr.part, i0);
+      v *= rope_weight<T>(a, hr.part, i1);
     }
     const float c = p < 0 ? quiet_nan() : a.cos[p * half + i], s = p < 0 ? quiet_nan() : a.sin[p * half + i];
     y[i0] = Elem<T>::from_f(u * c - v * s);
@@ -102,7 +109,7 @@ __global__ void __launch_bounds__(kRopeWarps * 32) qkrope_fwd_any_kernel(const _
   }
   for (int j = a.rot + lane; j < a.D; j += 32) {
     const float u = buf[j] * inv;
-    y[j] = Elem<T>::from_f(w ? u * Elem<T>::to_f(w[j]) : u);
+    y[j] = Elem<T>::from_f(w ? u * rope_weight<T>(a, hr.part, j) : u);
   }
 }
 
@@ -132,7 +139,7 @@ __global__ void __launch_bounds__(kRopeWarps * 32) qkrope_bwd_any_kernel(const _
       continue;
     }
     const T* x = static_cast<const T*>(a.qkv) + n * a.qkv_stride + static_cast<long long>(r) * D;
-    const T* w = static_cast<const T*>(a.w[hr.part]);
+    const bool w = a.w[hr.part] != nullptr;
     __syncwarp();
     float ss = 0.f;
     for (int j = lane; j < D; j += 32) {
@@ -157,7 +164,7 @@ __global__ void __launch_bounds__(kRopeWarps * 32) qkrope_bwd_any_kernel(const _
       const float xh = xb[j] * inv;
       float e = gb[j];
       if (weighted) acc[hr.part * D + j] += e * xh;
-      if (w) e *= Elem<T>::to_f(w[j]);
+      if (w) e *= rope_weight<T>(a, hr.part, j);
       gb[j] = e;
       dot = fmaf(e, xh, dot);
     }
@@ -301,9 +308,12 @@ __device__ __forceinline__ void scale(float (&x)[VEC], float w) {
   for (int i = 0; i < VEC / 2; ++i) mul2(x[2 * i], x[2 * i + 1], w, x[2 * i], x[2 * i + 1]);
 }
 
-template <typename T, int G, bool INTERLEAVED, bool WEIGHTED>
+// W: the weights' type, void without weights (as a test at run time the type took registers:
+// the half-split forward 19.4 us instead of 17.8 at 1237 x 3 tokens of 20 + 4 heads of 128).
+template <typename T, int G, bool INTERLEAVED, typename W>
 __global__ void __launch_bounds__(kRopeVecThreads, sizeof(T) == 2 ? 4 : 3)
     qkrope_fwd_kernel(const __grid_constant__ QkRopeArgs a) {
+  constexpr bool WEIGHTED = !std::is_void<W>::value;
   constexpr int VEC = 16 / sizeof(T), ROUND = 32 / G, ROUNDS = rope_rounds(false, WEIGHTED);
   const int lane = threadIdx.x & 31, l = lane % G;
   const int H = a.Hq + 2 * a.Hkv, Hqk = a.Hq + a.Hkv;
@@ -332,11 +342,11 @@ __global__ void __launch_bounds__(kRopeVecThreads, sizeof(T) == 2 ? 4 : 3)
   if (first < Hqk) {
     turn = rope_lane<VEC, INTERLEAVED>(a, p, l, 1.f);
     from = rope_partner_lane(a, turn.turns, l, VEC);
-    if (WEIGHTED) {
+    if constexpr (WEIGHTED) {
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
-        wq[e] = a.w[0] && mine ? Elem<T>::to_f(static_cast<const T*>(a.w[0])[l * VEC + e]) : 1.f;
-        wk[e] = a.w[1] && mine ? Elem<T>::to_f(static_cast<const T*>(a.w[1])[l * VEC + e]) : 1.f;
+        wq[e] = a.w[0] && mine ? Elem<W>::to_f(static_cast<const W*>(a.w[0])[l * VEC + e]) : 1.f;
+        wk[e] = a.w[1] && mine ? Elem<W>::to_f(static_cast<const W*>(a.w[1])[l * VEC + e]) : 1.f;
       }
     }
   }
@@ -360,20 +370,21 @@ __global__ void __launch_bounds__(kRopeVecThreads, sizeof(T) == 2 ? 4 : 3)
 
 // WEIGHTED also carries the weight gradients: a lane keeps its columns' sums over
 // the units its warp walks through, the block adds its lanes in a fixed order.
-template <typename T, int G, bool INTERLEAVED, bool WEIGHTED>
-__global__ void __launch_bounds__(kRopeVecThreads, WEIGHTED ? 2 : 3)
+template <typename T, int G, bool INTERLEAVED, typename W>
+__global__ void __launch_bounds__(kRopeVecThreads, std::is_void<W>::value ? 3 : 2)
     qkrope_bwd_kernel(const __grid_constant__ QkRopeArgs a) {
+  constexpr bool WEIGHTED = !std::is_void<W>::value;
   constexpr int VEC = 16 / sizeof(T), ROUND = 32 / G, ROUNDS = rope_rounds(true, WEIGHTED);
   const int lane = threadIdx.x & 31, l = lane % G;
   const int H = a.Hq + 2 * a.Hkv, Hqk = a.Hq + a.Hkv;
   const unsigned units = (H + ROUNDS * ROUND - 1) / (ROUNDS * ROUND);
   const bool mine = l * VEC < a.D;
   float wq[VEC], wk[VEC], acc[2][VEC];
-  if (WEIGHTED) {
+  if constexpr (WEIGHTED) {
 #pragma unroll
     for (int e = 0; e < VEC; ++e) {
-      wq[e] = a.w[0] && mine ? Elem<T>::to_f(static_cast<const T*>(a.w[0])[l * VEC + e]) : 1.f;
-      wk[e] = a.w[1] && mine ? Elem<T>::to_f(static_cast<const T*>(a.w[1])[l * VEC + e]) : 1.f;
+      wq[e] = a.w[0] && mine ? Elem<W>::to_f(static_cast<const W*>(a.w[0])[l * VEC + e]) : 1.f;
+      wk[e] = a.w[1] && mine ? Elem<W>::to_f(static_cast<const W*>(a.w[1])[l * VEC + e]) : 1.f;
       acc[0][e] = acc[1][e] = 0.f;
     }
   }
@@ -452,16 +463,16 @@ __global__ void __launch_bounds__(kRopeVecThreads, WEIGHTED ? 2 : 3)
 
 // dw[j] = sum over the blocks' partials in a fixed order: one warp per column,
 // lane l adds blocks l, l + 32, ..., then a butterfly.
-template <typename T>
+template <typename W>
 __global__ void __launch_bounds__(128) rope_weight_sum_kernel(const float* __restrict__ partials, int blocks, int D,
-                                                              T* __restrict__ dwq, T* __restrict__ dwk) {
+                                                              W* __restrict__ dwq, W* __restrict__ dwk) {
   const int col = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (col >= 2 * D) return;
   float s = 0.f;
   for (int b = lane; b < blocks; b += 32) s += partials[static_cast<long long>(b) * 2 * D + col];
   s = warp_sum(s);
-  T* out = col < D ? dwq : dwk;
-  if (lane == 0 && out) out[col < D ? col : col - D] = Elem<T>::from_f(s);
+  W* out = col < D ? dwq : dwk;
+  if (lane == 0 && out) out[col < D ? col : col - D] = Elem<W>::from_f(s);
 }
 
 // ---------------------------------------------------------------------------
@@ -472,14 +483,14 @@ namespace {
 constexpr int kRopePartialBlocksPerSm = 4;
 
 // Lanes of a head row when it can be moved in 16-byte packs of which each turns
-// whole or not at all, else 0: rows, tables and weights 16-byte aligned, at most
+// whole or not at all, else 0: rows and tables 16-byte aligned, at most
 // 32 packs a head.
 template <typename T>
 int pack_lanes(const QkRopeArgs& a, bool backward) {
   constexpr int VEC = 16 / sizeof(T);
   const auto bad = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) != 0; };
   if (a.D % VEC || a.D > 32 * VEC || a.qkv_stride % VEC || a.rot % (a.interleaved ? VEC : 2 * VEC)) return 0;
-  if (bad(a.qkv) || (a.rot && (bad(a.cos) || bad(a.sin))) || bad(a.w[0]) || bad(a.w[1])) return 0;
+  if (bad(a.qkv) || (a.rot && (bad(a.cos) || bad(a.sin)))) return 0;
   for (int i = 0; i < 3; ++i) {
     if (backward) {
       if (bad(a.g[i])) return 0;
@@ -498,13 +509,13 @@ int pack_lanes(const QkRopeArgs& a, bool backward) {
 template <typename T, int G>
 cudaError_t vector_t(bool backward, const QkRopeArgs& a, unsigned blocks, cudaStream_t st) {
   using Kernel = void (*)(QkRopeArgs);
-  static const Kernel kernels[2][2][2] = {
-      {{qkrope_fwd_kernel<T, G, false, false>, qkrope_fwd_kernel<T, G, false, true>},
-       {qkrope_fwd_kernel<T, G, true, false>, qkrope_fwd_kernel<T, G, true, true>}},
-      {{qkrope_bwd_kernel<T, G, false, false>, qkrope_bwd_kernel<T, G, false, true>},
-       {qkrope_bwd_kernel<T, G, true, false>, qkrope_bwd_kernel<T, G, true, true>}}};
+  static const Kernel kernels[2][2][3] = {  // without weights, of the data's type, fp32
+      {{qkrope_fwd_kernel<T, G, false, void>, qkrope_fwd_kernel<T, G, false, T>, qkrope_fwd_kernel<T, G, false, float>},
+       {qkrope_fwd_kernel<T, G, true, void>, qkrope_fwd_kernel<T, G, true, T>, qkrope_fwd_kernel<T, G, true, float>}},
+      {{qkrope_bwd_kernel<T, G, false, void>, qkrope_bwd_kernel<T, G, false, T>, qkrope_bwd_kernel<T, G, false, float>},
+       {qkrope_bwd_kernel<T, G, true, void>, qkrope_bwd_kernel<T, G, true, T>, qkrope_bwd_kernel<T, G, true, float>}}};
   const size_t smem = a.partials ? kRopeVecThreads * 2 * (16 / sizeof(T)) * sizeof(float) : 0;
-  kernels[backward][a.interleaved != 0][a.w[0] || a.w[1]]<<<blocks, kRopeVecThreads, smem, st>>>(a);
+  kernels[backward][a.interleaved != 0][a.w[0] || a.w[1] ? 1 + a.w32 : 0]<<<blocks, kRopeVecThreads, smem, st>>>(a);
   return cudaGetLastError();
 }
 
@@ -532,8 +543,10 @@ cudaError_t run_t(bool backward, const QkRopeArgs& a, cudaStream_t st) {
     }
   }
   if (e != cudaSuccess || !a.partials) return e;
-  rope_weight_sum_kernel<T><<<(2 * a.D + 3) / 4, 128, 0, st>>>(a.partials, static_cast<int>(blocks), a.D,
-                                                             static_cast<T*>(a.dw[0]), static_cast<T*>(a.dw[1]));
+  const unsigned sums = (2 * a.D + 3) / 4;
+  const int n = static_cast<int>(blocks);
+  if (a.w32) rope_weight_sum_kernel<<<sums, 128, 0, st>>>(a.partials, n, a.D, static_cast<float*>(a.dw[0]), static_cast<float*>(a.dw[1]));
+  else rope_weight_sum_kernel<<<sums, 128, 0, st>>>(a.partials, n, a.D, static_cast<T*>(a.dw[0]), static_cast<T*>(a.dw[1]));
   return cudaGetLastError();
 }
 

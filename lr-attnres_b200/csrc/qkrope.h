@@ -18,6 +18,7 @@ struct QkRopeArgs {
   const void* positions;  // [N] int32 / int64, or null: n % T
   int positions64;
   const void* w[2];  // q and k weights [D], or null
+  int w32;           // weights and dw are fp32 beside 16-bit data
   int normalize, interleaved;
   float eps, inv_D;
   void* out[3];  // q [N, Hq, D], k, v [N, Hkv, D]
