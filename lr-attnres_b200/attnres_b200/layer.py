@@ -13,9 +13,10 @@ device's current stream through the C ABI. There is no CPU fallback: a CPU tenso
 is a RuntimeError, as is any argument that a check turns down.
 
 Eager calls go straight to the compiled binding (_layer.so, csrc/layer_binding.cpp),
-which checks, allocates and carries autograd. Under torch.compile, and for fake
-tensors, a call is the attnres:: torch.library op of the same name, which traces and
-has the same autograd formula.
+which checks, allocates and carries autograd. Under torch.compile and other tracers,
+dispatch modes and function transforms, and for fake tensors, a call is the attnres::
+torch.library op of the same name, which traces and has the same autograd formula.
+There are no forward-mode derivatives: a tensor with a tangent is a RuntimeError.
 """
 from typing import Optional
 
@@ -26,6 +27,8 @@ from . import _native as N
 from .ops import F32_EPS
 
 _EAGER_TYPES = (Tensor, torch.nn.Parameter)
+_dispatch_modes, _jit_tracing = torch._C._len_torch_dispatch_stack, torch._C._is_tracing
+_transform, _transforms = torch._C._functorch.peek_interpreter_stack, torch._C._functorch.get_interpreter_stack
 _binding = None
 
 
@@ -44,8 +47,15 @@ def _load():
 
 
 def _eager(*tensors):
-    """Whether a call on these tensors may go straight to the binding."""
+    """Whether a call on these tensors may go straight to the binding: nobody traces, transforms or watches PyTorch's
+    operators, which the binding's calls are none of."""
     if torch.compiler.is_compiling():
+        return False
+    if _dispatch_modes() or _jit_tracing():
+        return False
+    if _transform() is not None:
+        if any(t.key() == torch._C._functorch.TransformType.Jvp for t in _transforms()):
+            raise RuntimeError("attnres_b200: the layer operators have no forward-mode derivative")
         return False
     for t in tensors:
         if t is not None and type(t) not in _EAGER_TYPES:

@@ -65,6 +65,12 @@ void check_first_order(const char* what) {
   TORCH_CHECK(!at::GradMode::is_enabled(), "attnres_b200: ", what, " cannot be differentiated twice (create_graph)");
 }
 
+// Nor is there a forward-mode derivative.
+void check_no_tangent(const char* what, std::initializer_list<const Tensor*> ts) {
+  for (const Tensor* t : ts)
+    TORCH_CHECK(!t->defined() || !t->_fw_grad(0).defined(), "attnres_b200: ", what, " has no forward-mode derivative");
+}
+
 // ---------------------------------------------------------------------------
 // qk_norm_rope
 // ---------------------------------------------------------------------------
@@ -234,6 +240,7 @@ py::tuple py_qk_norm_rope(const Tensor& qkv, int64_t q_heads, int64_t kv_heads, 
                           bool normalize, bool interleaved) {
   const RopeHow how{q_heads, kv_heads, normalize, eps, interleaved};
   const Tensor pos = or_undefined(positions), wq = or_undefined(q_weight), wk = or_undefined(k_weight);
+  check_no_tangent("qk_norm_rope", {&qkv, &cos, &sin, &wq, &wk});
   if (wants_grad({&qkv, &wq, &wk}))
     return tuple3(QkNormRope::apply(qkv, cos, sin, positions, q_weight, k_weight, how));
   return tuple3(rope_forward(qkv, cos, sin, pos, wq, wk, how));
@@ -349,6 +356,7 @@ struct Swiglu : torch::autograd::Function<Swiglu> {
 };
 
 Tensor py_swiglu(const Tensor& x, const Tensor& w) {
+  check_no_tangent("swiglu_projection", {&x, &w});
   if (wants_grad({&x, &w})) return Swiglu::apply(x, w);
   return swiglu_forward(x, w);
 }
@@ -413,6 +421,7 @@ Tensor rows4(const char* what, const char* name, const Tensor& t, int64_t B, int
 }
 
 void no_gradient(const char* what, std::initializer_list<const Tensor*> ts) {
+  check_no_tangent(what, ts);
   TORCH_CHECK(!wants_grad(ts), "attnres_b200: ", what, " has no gradient; call it under torch.no_grad() or detach its inputs");
 }
 
