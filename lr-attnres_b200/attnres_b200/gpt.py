@@ -378,6 +378,8 @@ class GPT(nn.Module):
             T = idx.size(1)
             if cache.used + T > cache.max_tokens:
                 raise RuntimeError(f"attnres_b200: the cache holds {cache.used} of {cache.max_tokens} tokens, {T} more do not fit")
+            if cache.used:
+                self._check_cached_attention()
             positions = cache.lengths[:, None] + torch.arange(T, device=idx.device, dtype=torch.int32)
             lengths = cache.lengths + T
             pasts = [LayerPast(cache, li, positions, lengths) for li in range(c.n_layer)]
@@ -420,12 +422,23 @@ class GPT(nn.Module):
             cache.used += T
         return x if return_hidden else self.logits(x)
 
+    def _check_cached_attention(self):
+        """Raises where kv4_attention will not take the model's heads: better now than after the prompt's work."""
+        c, weight = self.cfg, self.transformer.wte.weight
+        dtype = torch.get_autocast_dtype(weight.device.type) if torch.is_autocast_enabled(weight.device.type) else weight.dtype
+        head_dim = c.n_embd // c.n_head
+        if dtype not in (torch.float16, torch.bfloat16) or head_dim not in (64, 128):
+            raise RuntimeError("attnres_b200: tokens behind a cache's go through kv4_attention, which is built for float16 and "
+                               f"bfloat16 and heads of 64 and 128, not for {dtype} and {head_dim}")
+
     @torch.no_grad()
     def generate(self, idx: Tensor, new_tokens: int, cache: Optional[GPTCache] = None) -> Tensor:
         """The prompts idx [B, T] with `new_tokens` tokens appended to each, the likeliest at every
         step. Pass a cache to go on from it later; the last token chosen is not in it yet."""
         if new_tokens < 1:
             return idx
+        if new_tokens > 1 or (cache is not None and cache.used):
+            self._check_cached_attention()
         if cache is None:
             cache = GPTCache(self.cfg, idx.size(0), idx.size(1) + new_tokens - 1, device=idx.device)
         out, step = [idx], idx
