@@ -246,6 +246,10 @@ class GPTCache:
         self.page_table = torch.arange(batch * per, device=device, dtype=torch.int32).view(batch, per)
         self.lengths = torch.zeros(batch, device=device, dtype=torch.int32)
 
+    def check_room(self, tokens: int):
+        if self.used + tokens > self.max_tokens:
+            raise RuntimeError(f"attnres_b200: the cache holds {self.used} of {self.max_tokens} tokens, {tokens} more do not fit")
+
 
 class LayerPast:
     """What a layer's attention takes of a GPTCache for one call: new tokens are written behind the
@@ -376,8 +380,7 @@ class GPT(nn.Module):
         pasts = [None] * c.n_layer
         if cache is not None:
             T = idx.size(1)
-            if cache.used + T > cache.max_tokens:
-                raise RuntimeError(f"attnres_b200: the cache holds {cache.used} of {cache.max_tokens} tokens, {T} more do not fit")
+            cache.check_room(T)
             if cache.used:
                 self._check_cached_attention()
             positions = cache.lengths[:, None] + torch.arange(T, device=idx.device, dtype=torch.int32)
@@ -441,6 +444,7 @@ class GPT(nn.Module):
             self._check_cached_attention()
         if cache is None:
             cache = GPTCache(self.cfg, idx.size(0), idx.size(1) + new_tokens - 1, device=idx.device)
+        cache.check_room(idx.size(1) + new_tokens - 1)
         out, step = [idx], idx
         for _ in range(new_tokens):
             step = self.logits(self(step, return_hidden=True, cache=cache)[:, -1:]).argmax(-1)

@@ -1,0 +1,27 @@
+"""GPT and its blocks as their callers have them, on the CPU."""
+import pytest
+import torch
+from torch import nn
+
+KW = dict(n_layer=2, n_head=2, n_embd=128, vocab_size=33, block_size=32, lrid_rank=32)
+
+
+def model(**kw):
+    from attnres_b200.gpt import GPT, GPTConfig
+
+    return GPT(GPTConfig(**{**KW, **kw}))
+
+
+def test_generate_refuses_what_does_not_fit_before_it_works():
+    from attnres_b200.gpt import GPTCache
+
+    m = model().to(torch.bfloat16)
+    calls = []
+    m.transformer.wte.register_forward_hook(lambda *a: calls.append(1))
+    cache = GPTCache(m.cfg, 1, 12, page_size=16, device="cpu")
+    idx = torch.zeros(1, 8, dtype=torch.int64)
+    with pytest.raises(RuntimeError, match="do not fit"):
+        m.generate(idx, 6, cache=cache)  # 8 and 5 more; the last choice is not written
+    with pytest.raises(RuntimeError, match="positions"):
+        m.generate(idx, 26)
+    assert not calls and cache.used == 0
