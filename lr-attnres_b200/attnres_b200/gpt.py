@@ -300,7 +300,7 @@ class Block(nn.Module):
         return out, key
 
     def forward_attention(self, x, x_is_normalized=False, past=None):
-        return self._sublayer(self.attn, x, x_is_normalized, past)
+        return self._sublayer(self.attn, x, x_is_normalized, *(() if past is None else (past,)))
 
     def forward_mlp(self, x, x_is_normalized=False):
         return self._sublayer(self.mlp, x, x_is_normalized)
@@ -405,10 +405,8 @@ class GPT(nn.Module):
             for sub in (0, 1):
                 site = 2 * li + sub
                 x = read(site) if site > 0 else (norm(x) if fused_read_norm else x)
-                if sub == 0:
-                    out, key = block.forward_attention(x, x_is_normalized=fused_read_norm, past=pasts[li])
-                else:
-                    out, key = block.forward_mlp(x, x_is_normalized=fused_read_norm)
+                f, past = ((block.forward_attention, pasts[li]), (block.forward_mlp, None))[sub]
+                out, key = f(x, x_is_normalized=fused_read_norm, **({} if past is None else {"past": past}))
                 part_n += 1
                 part, part_src = self._summary(part, out, part_n)
                 part_key = key if part_n == 1 else part_key + key

@@ -25,3 +25,30 @@ def test_generate_refuses_what_does_not_fit_before_it_works():
     with pytest.raises(RuntimeError, match="positions"):
         m.generate(idx, 26)
     assert not calls and cache.used == 0
+
+
+def test_blocks_call_their_attention_as_before():
+    """An attention module that takes the hidden states alone, as the reference's does, still fits into a block."""
+    from attnres_b200.gpt import Block, GPTConfig
+
+    class Plain(nn.Module):
+        def forward(self, x):
+            return 2 * x, x[..., :32]
+
+    block = Block(GPTConfig(**KW))
+    block.attn = Plain()
+    x = torch.randn(1, 3, 128)
+    seen = []
+    block.attn.register_forward_pre_hook(lambda module, args: seen.append(len(args)))
+    out, key = block.forward_attention(x, x_is_normalized=True)
+    assert out.shape == x.shape and key.shape == (1, 3, 32) and seen == [1]
+
+
+def test_a_model_calls_its_blocks_as_before():
+    m = model(fused=False)
+    idx = torch.randint(0, 33, (2, 7))
+    want = m(idx)
+    for block in m.transformer.layers:
+        of = type(block).forward_attention
+        block.forward_attention = lambda x, x_is_normalized=False, block=block, of=of: of(block, x, x_is_normalized)
+    assert torch.equal(m(idx), want)
