@@ -116,6 +116,13 @@ int check_swiglu(int64_t n, int in_dim, int hidden, int dtype, const void* x, in
   return ATTNRES_OK;
 }
 
+constexpr int kKv4MaxGrid = 65535;           // sequences, key heads: a grid's y and z
+constexpr int64_t kKv4MaxPlaces = 1LL << 30;  // places of a sequence
+
+bool too_many_query_rows(int batch, int new_tokens, int q_heads) {
+  return static_cast<double>(batch) * new_tokens * q_heads > 0x3fffffff;
+}
+
 // The pool, the page table and the counts, as every cache entry takes them.
 int check_kv4(const attnres::Kv4Cache& c, int max_pages, int64_t table_stride, int batch, int new_tokens) {
   if (c.pages < 0 || c.heads < 1 || c.page < 1 || c.D < 1 || max_pages < 0 || batch < 0 || new_tokens < 0)
@@ -123,9 +130,9 @@ int check_kv4(const attnres::Kv4Cache& c, int max_pages, int64_t table_stride, i
   if (c.page % 16 || c.D % attnres::kKv4Group || c.D > attnres::kKv4MaxDim)
     return fail(ATTNRES_ERR_UNSUPPORTED, "kv4 cache: page_size=%d must be a multiple of 16, head_dim=%d of 32 up to %d",
                 c.page, c.D, attnres::kKv4MaxDim);
-  if (batch > 65535 || c.heads > 65535)
-    return fail(ATTNRES_ERR_UNSUPPORTED, "kv4 cache: batch=%d and kv_heads=%d up to 65535", batch, c.heads);
-  if (static_cast<int64_t>(max_pages) * c.page > (1LL << 30))
+  if (batch > kKv4MaxGrid || c.heads > kKv4MaxGrid)
+    return fail(ATTNRES_ERR_UNSUPPORTED, "kv4 cache: batch=%d and kv_heads=%d up to %d", batch, c.heads, kKv4MaxGrid);
+  if (static_cast<int64_t>(max_pages) * c.page > kKv4MaxPlaces)
     return fail(ATTNRES_ERR_UNSUPPORTED, "kv4 cache: a sequence of %d pages of %d places is too long", max_pages, c.page);
   if (static_cast<double>(c.pages) * c.heads * (c.page / 16) > 0x7fffffff)
     return fail(ATTNRES_ERR_UNSUPPORTED, "kv4 cache: a pool of %lld pages is too large", c.pages);
@@ -356,6 +363,10 @@ size_t attnres_kv4_attention_workspace_bytes(int kv_heads, int page_size, int he
                                              int new_tokens, int q_heads) {
   if (kv_heads < 1 || page_size < 1 || head_dim < 1 || max_pages < 0 || batch < 1 || new_tokens < 1 || q_heads < kv_heads)
     return 0;
+  // sizes that the call refuses: the plan's numbers would not hold them
+  if (batch > kKv4MaxGrid || kv_heads > kKv4MaxGrid || static_cast<int64_t>(max_pages) * page_size > kKv4MaxPlaces ||
+      too_many_query_rows(batch, new_tokens, q_heads))
+    return 0;
   attnres::Kv4AttnArgs a{};
   a.c = kv4_cache(nullptr, nullptr, nullptr, nullptr, 0, kv_heads, page_size, head_dim);
   a.max_pages = max_pages;
@@ -381,7 +392,7 @@ int attnres_kv4_attention(const void* k_codes, const void* k_params, const void*
   if (q_heads < 1 || q_heads % kv_heads)
     return fail(ATTNRES_ERR_INVALID_ARGUMENT, "kv4 attention: q_heads=%d must be a multiple of kv_heads=%d", q_heads,
                 kv_heads);
-  if (static_cast<double>(batch) * new_tokens * q_heads > 0x3fffffff)
+  if (too_many_query_rows(batch, new_tokens, q_heads))
     return fail(ATTNRES_ERR_UNSUPPORTED, "kv4 attention: too many query rows for one launch");
   if (batch == 0 || new_tokens == 0) return ATTNRES_OK;
   if ((rc = check_kv4_buffers(a.c, page_table, max_pages, lengths))) return rc;

@@ -15,3 +15,12 @@ def test_rope_takes_float_weights_beside_any_type(dtype):
     assert N.load().attnres_qk_norm_rope_backward(4, 2, 2, 1, 64, 64, dtype | N.WEIGHTS_F32, P, 256, P, P, 8, None, 0, P, None, 1,
                                                   1e-6, 1, P, P, P, STRIDES, P, P, None, ctypes.c_void_p(0), 0,
                                                   None) == WORKSPACE
+
+
+def test_attention_workspace_of_sizes_that_the_call_refuses():
+    need = N.load().attnres_kv4_attention_workspace_bytes
+    big = (1 << 31) - 1
+    assert need(2, 16, 64, 4096, 2, 1, 4) > 0
+    for sizes in ((2, 16, 64, 4096, 2, big, 4096), (1, 16, 64, 4096, 1, 1 << 20, 1 << 11), (2, 16, 64, big, 2, 1, 4),
+                  (2, 1 << 30, 64, big, 2, 1, 4), (2, 16, 64, 4096, 70000, 1, 4), (70000, 16, 64, 4096, 1, 1, 70000)):
+        assert need(*sizes) == 0, sizes
