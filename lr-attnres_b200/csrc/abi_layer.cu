@@ -54,7 +54,7 @@ int check_qk_norm_rope(const attnres::QkRopeArgs& a, int dtype) {
     return fail(ATTNRES_ERR_INVALID_ARGUMENT, "qk norm rope: rotary_dim=%d must be even and in [0, head_dim]", a.rot);
   if (a.qkv_stride < static_cast<long long>(a.Hq + 2 * a.Hkv) * a.D)
     return fail(ATTNRES_ERR_INVALID_ARGUMENT, "qk norm rope: qkv_row_stride below (q_heads + 2 kv_heads) * head_dim");
-  if (a.N > (1LL << 33) / (a.Hq + 2 * a.Hkv))
+  if (a.N > ((1LL << 33) - 4) / (a.Hq + 2 * a.Hkv))  // blocks of four head rows
     return fail(ATTNRES_ERR_UNSUPPORTED, "qk norm rope: num_tokens=%lld is too many for one launch", a.N);
   if (a.N == 0) return ATTNRES_OK;
   if (!a.qkv) return fail(ATTNRES_ERR_INVALID_ARGUMENT, "qk norm rope: qkv is NULL");

@@ -4,7 +4,7 @@ import ctypes
 import pytest
 
 from attnres_b200 import _native as N
-from test_layer_cpu import INVALID, P, STRIDES, WORKSPACE, rope
+from test_layer_cpu import INVALID, P, STRIDES, UNSUPPORTED, WORKSPACE, rope
 
 
 @pytest.mark.parametrize("dtype", [N.DTYPE_F32, N.DTYPE_F16, N.DTYPE_BF16])
@@ -24,3 +24,7 @@ def test_attention_workspace_of_sizes_that_the_call_refuses():
     for sizes in ((2, 16, 64, 4096, 2, big, 4096), (1, 16, 64, 4096, 1, 1 << 20, 1 << 11), (2, 16, 64, big, 2, 1, 4),
                   (2, 1 << 30, 64, big, 2, 1, 4), (2, 16, 64, 4096, 70000, 1, 4), (70000, 16, 64, 4096, 1, 1, 70000)):
         assert need(*sizes) == 0, sizes
+
+
+def test_rope_refuses_more_rows_than_a_grid_holds():
+    assert rope(n=1 << 31, T=1) == UNSUPPORTED  # 2^33 head rows, four a block: one block more than a grid has
