@@ -590,12 +590,11 @@ cudaError_t few_t(const SwigluArgs& s, cudaStream_t st) {
 // Time of a list of tiles on P pairs, in steps of 64 columns of a 256 x 256 tile (0.42 us).
 // A step of a 256 x 128 tile counts 0.75: 0.5 alone, but it has 3/4 of the loads and twice
 // the starts and ends for its products (1531 tokens, 776 -> 2056, gate forward: 19.1 us on
-// wide tiles, 20.0 on narrow ones; dx, 42 narrow tiles or 24 wide: 21.7 and 28 us). 8: a
-// start and end that no other tile hides.
+// wide tiles, 20.0 on narrow ones; dx, 42 narrow tiles or 24 wide: 21.7 and 28 us).
 double tiles_cost(const GemmJob& g, int BN, bool gate, int P) {
   const int n = gate ? ceil_div_i(g.cols, BN / 2) : ceil_div_i(g.cols, BN);
   const long long tiles = static_cast<long long>((g.M + kGmM - 1) / kGmM) * n;
-  return static_cast<double>((tiles + P - 1) / P) * g.ksteps * (BN == 256 ? 1.0 : 0.75) + 8.0;
+  return static_cast<double>((tiles + P - 1) / P) * g.ksteps * (BN == 256 ? 1.0 : 0.75);
 }
 
 template <typename T, int MODE, int BN>
