@@ -104,17 +104,22 @@ __device__ __forceinline__ uint32_t half_pack(float a, float b) {
   const __half2 r = __floats2half2_rn(a, b);
   return *reinterpret_cast<const uint32_t*>(&r);
 }
-// Whether one of two groups has a value beyond f16 or none at all: low + 15 step, rounded,
-// is infinite or NaN. steps, lows: the two groups' params, taken apart.
-__device__ __forceinline__ bool leaves_f16(uint32_t steps, uint32_t lows) {
-  return not_finite(half_fma(steps, 0x4b804b80u, lows));
+// The largest values of two groups, low + 15 step: rounded to f16 they are infinite or NaN if
+// one leaves it. steps, lows: the groups' params, taken apart.
+__device__ __forceinline__ __half2 largest_values(uint32_t steps, uint32_t lows) {
+  const uint32_t top = half_fma(steps, 0x4b804b80u, lows);
+  return __habs2(*reinterpret_cast<const __half2*>(&top));
+}
+// Whether one of four groups has a value beyond f16 or none at all.
+__device__ __forceinline__ bool leave_f16(__half2 a, __half2 b) {
+  const uint32_t inf = 0x7c007c00u;
+  return !__hblt2(__hmax2_nan(a, b), *reinterpret_cast<const __half2*>(&inf));
 }
 // The same over the value params of a stage, four groups a lane.
 __device__ __forceinline__ bool stage_leaves_f16(const unsigned char* params, int lane) {
   const uint4 p = *reinterpret_cast<const uint4*>(params + lane * 16);
-  const bool mine = leaves_f16(__byte_perm(p.x, p.y, 0x5410u), __byte_perm(p.x, p.y, 0x7632u)) ||
-                    leaves_f16(__byte_perm(p.z, p.w, 0x5410u), __byte_perm(p.z, p.w, 0x7632u));
-  return __any_sync(0xffffffffu, mine);
+  return __any_sync(0xffffffffu, leave_f16(largest_values(__byte_perm(p.x, p.y, 0x5410u), __byte_perm(p.x, p.y, 0x7632u)),
+                                           largest_values(__byte_perm(p.z, p.w, 0x5410u), __byte_perm(p.z, p.w, 0x7632u))));
 }
 
 __device__ __forceinline__ uint32_t transposed(uint32_t x) {
@@ -507,12 +512,12 @@ __global__ void __launch_bounds__(kAtWarps * 32, NT == 1 ? (D == 64 ? 5 : 4) : 2
             wb[part][j] = pb[part][j];
           }
         if constexpr (CAREFUL) {
-          bool beyond = false;
+          __half2 top[2];
 #pragma unroll
           for (int e = 0; e < 2; ++e)
-            beyond |= leaves_f16(__byte_perm(par[2 * e][i], par[2 * e + 1][i], 0x5410u),
-                                 __byte_perm(par[2 * e][i], par[2 * e + 1][i], 0x7632u));
-          if (__any_sync(0xffffffffu, beyond)) {  // the values by 2^-5, the weights (up to 2^kSlack) by 2^5
+            top[e] = largest_values(__byte_perm(par[2 * e][i], par[2 * e + 1][i], 0x5410u),
+                                    __byte_perm(par[2 * e][i], par[2 * e + 1][i], 0x7632u));
+          if (__any_sync(0xffffffffu, leave_f16(top[0], top[1]))) {  // the values by 2^-5, the weights (up to 2^kSlack) by 2^5
 #pragma unroll
             for (int k = 0; k < 4; ++k) par[k][i] = half_mul(par[k][i], 0x28002800u);
 #pragma unroll
