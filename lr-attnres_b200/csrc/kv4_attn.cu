@@ -6,9 +6,9 @@
 // length - count + t and sees the places up to its own. Query head h reads key head
 // h / (Hq / Hkv): the query heads of one key head, times the new tokens, are the rows
 // that share one pass over its keys. A row that sees nothing gives zeros: its sum of
-// weights is 0, which no row that sees a place has. A row with a score that is NaN, or with
-// an infinity or NaN in its query, is NaN by its sum; the maximum alone does not tell
-// (comparisons drop NaN, so it stays -inf over NaN scores).
+// weights is 0 (as that of a row whose finite scores all overflow fp32 to -inf). A row with
+// a score that is NaN, or with an infinity or NaN in its query, is NaN by its sum; the
+// maximum alone does not tell (comparisons drop NaN, so it stays -inf over NaN scores).
 //
 // One pass with the running maximum and sum of the softmax. The products run on
 // mma.sync with the cache as the 16-row operand and the query rows as its 8 columns
@@ -20,8 +20,11 @@
 //           2^-24 of the largest. z = step * sum_d q_d n_d + low Q, Q the sum of the
 //           group's q: exact products, fp32 sums
 //   output  0x6400 | n is 1024 + n and 0x5400 | n << 4 is 64 + n; the difference to 1024 or
-//           64 is exact, step n + low is rounded once, weights are too (f16 outputs: to twice
-//           the bits)
+//           64 is exact, step n + low is rounded once to f16, and so are the weights (for f16
+//           outputs they are the sum of two f16 numbers: one rounding less of the output's
+//           own size). Weights below f16's normal range, 2^-14, are off by up to 2^-25 either
+//           way; a warp's weights are relative to its own maximum over at most 1024 places,
+//           so this adds up to less than 2^-15 of the largest
 // The row of a key is an accumulator's row and a value's column: weights change sides
 // by movmatrix. Keys are taken in the order i ^ ((i >> 1) & 1) so that lanes that differ
 // in their keys read different halves of the banks.
@@ -39,12 +42,14 @@
 // the warps are joined in shared memory, those of the stretches by kv4_join_kernel.
 // Every mbarrier wait is bounded (~2 s, a status bit on timeout).
 //
-// HBM is the floor (40 bytes a place of 64 elements, keys and values each), the ALU what
-// it meets: 8 sequences of 50000 places, 16 heads of 64, 3 tokens: 153 us with the join for
-// 512 MB (3.3 TB/s; the logic pipe is busy 60 % of the time, DRAM 36 %, the tensor cores
-// 15 %); 8 x 50000 places, 8 heads of 128, 4 query heads each: 132 us (3.9 TB/s). A stretch of a
-// few stages is mostly its start and end: 24 ragged sequences up to 6000 places of 8 heads
-// of 128 32 us for 72 MB.
+// HBM is the floor (40 bytes a place of 64 elements, keys and values each): 8 sequences of
+// 50000 places, 16 heads of 64, 3 tokens: 158 us with the join for 512 MB (3.2 TB/s); 8 x
+// 50000 places, 8 heads of 128, 4 query heads each: 134 us (3.8 TB/s). No unit is full there
+// (logic pipe 61 %, issue slots 61 %, DRAM 34 %, tensor cores 15 %): with the 16 or 20 warps
+// an SM that the registers leave, a quarter of its places, the steps of a stage wait for one
+// another. A stretch of a few stages is mostly its start and end: 24 ragged sequences up to
+// 6000 places of 8 heads of 128 32 us for 72 MB. The look at each stage's value params costs
+// 1 to 3 % of these times.
 #include <algorithm>
 
 #include "common.cuh"
@@ -717,10 +722,14 @@ size_t attn_smem(int D, int NT) {
   return std::max(ring, sums);
 }
 
-// Stretches: about two CTAs for every one that fits on the GPU (24 x 6000 places of 8
-// heads of 128: 62 us; with three CTAs for every two that fit 70, with four for one 69),
-// of at least 128 places. Sequences of up to 512 places stay whole: one launch instead of
-// two (one sequence of 300: 8.8 -> 7.6 us on the GPU).
+// Stretches for about eight CTAs an SM, of at least 128 places: two for every one that fits
+// at head_dim 128 with up to 8 query rows a key head (24 x 6000 places of 8 heads: 62 us;
+// with six CTAs an SM 70, with sixteen 69), 1.6 at head_dim 64, four with more rows, for
+// which other counts were not measured. Sequences of up to 512 places stay whole: one launch
+// instead of two (one sequence of 300: 8.8 -> 7.6 us on the GPU). The lengths lie on the
+// device, so the page table's width stands for them: under a table much wider than its
+// sequences the stretches are few and long (8 heads of 128, one sequence of 2000 places:
+// 9.1 us, under a table of 131072 places 19.0; 8 of 4000 places: 22.6 and 67.2).
 AttnLaunch plan(const Kv4AttnArgs& a) {
   AttnLaunch L{};
   L.a = a;

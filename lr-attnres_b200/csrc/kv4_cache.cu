@@ -4,13 +4,14 @@
 //   code = clamp(rint((x - low) / step), 0, 15), 0 where step is 0
 // with the rounded step and low, so the code is the nearest of the 16 values that will
 // be read back. A group that holds an infinity or a NaN, or whose step or low overflows
-// float16 (a least value that rounds beyond +-65504, a range of 15 times that), gets NaN for step and low
-// and reads back as NaN.
+// float16 (a least value that rounds beyond +-65504, a range of 15 times that), gets NaN for
+// step and low and reads back as NaN.
 //
 // Four lanes share a group (8 elements each, two shuffles for its extremes), and a
 // thread does the same part of a key and of its value, of two groups next to each other
-// where a head has an even number: four loads in flight, and one look at the page table. HBM is the floor, issue slots are what it meets first (a thread has 20 bytes
-// for every 16 elements it forms), so the work per element is kept to a subtraction, a
+// where a head has an even number: four loads in flight, and one look at the page table.
+// HBM is the floor, issue slots are what it meets first (a thread has 20 bytes for every
+// 16 elements it forms), so the work per element is kept to a subtraction, a
 // product, a sum that rounds (adding 1.5 * 2^23 leaves the integer in the low bits), a
 // multiply-add into the packed word, and the distance to a tie: the quotient is formed
 // with the reciprocal, and elements within 2^-16 of a tie are redone by division, which
