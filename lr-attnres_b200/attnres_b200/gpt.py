@@ -112,7 +112,7 @@ class RotaryEmbedding(nn.Module):
             if of[0] is buffers[0] and of[1] is buffers[1] and at == versions:
                 return made
         made = self._follow(buffers)
-        if made[0].is_cuda:
+        if made[0].is_cuda and type(made[0]) is Tensor:  # not a fake one, which no stream makes
             if torch.cuda.is_current_stream_capturing():
                 return made  # the graph's own
             torch.cuda.current_stream(made[0].device).synchronize()  # any stream may use them next

@@ -135,3 +135,15 @@ def test_fused_layer_and_cache_turn_as_the_unfused_layer_does(compiled):
             stale = model(**kw, fused_layer=True).cuda().to(torch.bfloat16)
             stale.load_state_dict({k: v for k, v in state.items() if "rope" not in k}, strict=False)
             assert float((stale.eval()(idx).float() - want).norm()) > 3 * float(plain)  # the bases do differ
+
+
+def test_a_model_of_fake_tensors_runs_without_a_device():
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    torch.set_default_dtype(torch.bfloat16)
+    try:
+        with FakeTensorMode(), torch.device("cuda"):
+            m = model(fused_layer=True)
+            assert m(torch.zeros(1, 4, dtype=torch.int64)).shape == (1, 4, KW["vocab_size"])
+    finally:
+        torch.set_default_dtype(torch.float32)
